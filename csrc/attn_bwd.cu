@@ -17,8 +17,11 @@
 // the MMAs of its neighbours.  Bound: about 1700 cycles of MMA per step (S^T, dP^T and dQ^T with N = 64 are limited by the
 // 128 bytes per cycle that shared memory delivers: 48 instead of 32 cycles per instruction).
 // D = rowsum(dO * O) comes from a small pre-pass; scale and bf16 of dQ are applied by a post-pass, of dK at the end.
+// Instantiations beyond plain causal attention (attn_mods.cuh): with t = tanh(scale s / cap), dS^T gets the factor 1 - t^2, and a key tile
+// walks over the queries between its first key's first query and its last key's last one.
 #include <stdio.h>
 
+#include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
 
@@ -54,6 +57,7 @@ struct BwdArgs {
   int head_parts;      // CTAs that share a key tile of a KV head, each with a part of its query heads
   float scale, scale_log2;
   int causal;
+  AttnMods mods;
 };
 
 YF_DEVINL void tma_reduce_add_3d(const CUtensorMap* m, const void* smem_src, int x, int y, int z) {
@@ -90,7 +94,7 @@ int head_group_size(int n_pos, int n_heads, long long accum_bytes, int n_sms) {
 }
 
 // SHARED: head_parts > 1 (an instantiation of its own: the parts' addresses cost the other one registers it does not have)
-template <bool SHARED>
+template <bool SHARED, int MODS>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                 const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ CUtensorMap tma_do,
@@ -113,7 +117,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   uint64_t* vk_done = dq_full + 2;
   uint64_t* dq_read = vk_done + 2;
   uint64_t* all_done = dq_read + 2;         // every MMA of the walk (waiting two phases ahead on vk_done would not do)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  uint64_t* kv_land = all_done + 1;         // MODS: bytes of K and V, and of a stage's Q and dO, before padded rows are cleared
+  uint64_t* q_land = kv_land + 1;           // [STAGES]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(MODS == 0 ? all_done + 1 : q_land + STAGES);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -124,8 +130,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   const int heads = args.Hq / args.Hkv / head_parts;  // query heads of this CTA
   const int h0 = hk * (args.Hq / args.Hkv) + part * heads;
   const int kv0 = jt * BKV;
-  const int i_start = args.causal ? kv0 / BQ : 0;          // first query tile
-  const int per_head = (args.S + BQ - 1) / BQ - i_start;   // at least one: the tile that holds these keys' own rows
+  int i_start = args.causal ? kv0 / BQ : 0;          // first query tile
+  int per_head = (args.S + BQ - 1) / BQ - i_start;   // at least one: the tile that holds these keys' own rows
+  // ranges of queries by key, padded tokens by tile
+  const int2* spans = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
+  const int* padding = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * ((args.S + BKV - 1) / BKV);
+  if (MODS != 0 && spans != nullptr) {
+    const int keys = min(BKV, args.S - kv0), n_qt = (args.S + BQ - 1) / BQ;
+    i_start = max(__ldg(spans + kv0).x, 0) / BQ;
+    per_head = min((__ldg(spans + kv0 + keys - 1).y + BQ - 1) / BQ, n_qt) - i_start;
+    if (__ldg(padding + jt) >= keys || per_head < 0) per_head = 0;  // nothing but padding
+  }
   const int n_it = per_head * heads;
 
   if (threadIdx.x == 0) {
@@ -136,8 +151,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     tma_prefetch_desc(&tma_dq);
     mbar_init(kv_full, 1);
     mbar_init(all_done, 1);
+    if (MODS != 0) {
+      mbar_init(kv_land, 1);
+      for (int i = 0; i < STAGES; ++i) mbar_init(&q_land[i], 1);
+    }
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&q_full[i], 2);
+      mbar_init(&q_full[i], MODS == 0 ? 2 : 1);
       mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -160,23 +179,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   const uint32_t tdV = tmem_base + 256, tdK = tmem_base + 384;  // set p of S^T | dP^T: tmem_base + 128 p, + 64
 
   if (warp == 12) {
-    if (elect_one()) {
-      mbar_expect_tx(kv_full, 2 * TILE);
-      tma_load_3d(sK, &tma_k, kv_full, hk * HD, kv0, b);
-      tma_load_3d(sK + ATOM, &tma_k, kv_full, hk * HD + 64, kv0, b);
-      tma_load_3d(sV, &tma_v, kv_full, hk * HD, kv0, b);
-      tma_load_3d(sV + ATOM, &tma_v, kv_full, hk * HD + 64, kv0, b);
+    if ((MODS == 0 || n_it > 0) && elect_one()) {
+      uint64_t* kv_bar = MODS == 0 ? kv_full : kv_land;
+      mbar_expect_tx(kv_bar, 2 * TILE);
+      tma_load_3d(sK, &tma_k, kv_bar, hk * HD, kv0, b);
+      tma_load_3d(sK + ATOM, &tma_k, kv_bar, hk * HD + 64, kv0, b);
+      tma_load_3d(sV, &tma_v, kv_bar, hk * HD, kv0, b);
+      tma_load_3d(sV + ATOM, &tma_v, kv_bar, hk * HD + 64, kv0, b);
       int h = h0, i = 0;
       for (int it = 0, st = 0, ph = 1; it < n_it; ++it) {
         if (!mbar_wait(&q_empty[st], ph, 200)) break;
         const int q0 = (i_start + i) * BQ;
         uint8_t* sQ = sRing + st * 2 * QTILE;
         uint8_t* sdO = sQ + QTILE;
-        mbar_expect_tx(&q_full[st], 2 * QTILE);
-        tma_load_3d(sQ, &tma_q, &q_full[st], h * HD, q0, b);
-        tma_load_3d(sQ + QATOM, &tma_q, &q_full[st], h * HD + 64, q0, b);
-        tma_load_3d(sdO, &tma_do, &q_full[st], h * HD, q0, b);
-        tma_load_3d(sdO + QATOM, &tma_do, &q_full[st], h * HD + 64, q0, b);
+        uint64_t* q_bar = MODS == 0 ? &q_full[st] : &q_land[st];
+        mbar_expect_tx(q_bar, 2 * QTILE);
+        tma_load_3d(sQ, &tma_q, q_bar, h * HD, q0, b);
+        tma_load_3d(sQ + QATOM, &tma_q, q_bar, h * HD + 64, q0, b);
+        tma_load_3d(sdO, &tma_do, q_bar, h * HD, q0, b);
+        tma_load_3d(sdO + QATOM, &tma_do, q_bar, h * HD + 64, q0, b);
         if (++i == per_head) { i = 0; ++h; }
         if (++st == STAGES) { st = 0; ph ^= 1; }
       }
@@ -196,7 +217,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         dl[e] = ok ? args.delta[at + r] : 0.f;
       }
     };
-    fetch();
+    if (MODS == 0 || n_it > 0) fetch();
+    if (MODS != 0 && n_it > 0 && __all_sync(0xffffffffu, mbar_wait(kv_land, 0, 202))) {
+      if (padding != nullptr && __ldg(padding + jt) > 0) {  // dQ^T = K^T dS^T would multiply what padding holds by zeros
+        zero_padded_rows(sK, ATOM, BKV, kv0, args.S, spans);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(kv_full);
+    }
     for (int it = 0, st = 0, ph = 1; it < n_it; ++it) {
       if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[st], ph, 201))) break;
       float* stat = sStat + st * STAT_FLOATS;
@@ -205,6 +234,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         stat[lane + 32 * e] = nl[e];
         stat[BQ + lane + 32 * e] = dl[e];
       }
+      if (MODS != 0) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&q_land[st], ph ^ 1, 203))) break;
+        const int q0 = (i_start + i) * BQ;
+        if (padding != nullptr && __ldg(padding + q0 / BKV) > 0) {  // dK and dV: as above
+          uint8_t* sQ = sRing + st * 2 * QTILE;
+          zero_padded_rows(sQ, QATOM, BQ, q0, args.S, spans);
+          zero_padded_rows(sQ + QTILE, QATOM, BQ, q0, args.S, spans);
+          fence_proxy_async_smem();
+        }
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[st]);
       if (++i == per_head) { i = 0; ++h; }
@@ -212,7 +251,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (++st == STAGES) { st = 0; ph ^= 1; }
     }
   } else if (warp == 13) {
-    if (elect_one()) {
+    if ((MODS == 0 || n_it > 0) && elect_one()) {
       const uint32_t id_s = umma_idesc_bf16(128, BQ, 0, 0);    // S^T, dP^T: both operands K-major (K = head dim)
       const uint32_t id_g = umma_idesc_bf16(128, HD, 0, 1);    // dV, dK: A from TMEM (K = queries), dO / Q MN-major
       const uint32_t id_q = umma_idesc_bf16(128, BQ, 1, 1);    // dQ^T: K tile MN-major (M = head dim), dS^T MN-major
@@ -277,7 +316,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const float sl2 = args.scale_log2;
     uint8_t* ds_row = sdS + p * DS_BYTES + row * 128;
     bool alive = true;
-    int st = p, ph = 0, i = p % per_head;     // ring stage and its parity, query tile of step p
+    int st = p, ph = 0, i = MODS != 0 && n_it == 0 ? 0 : p % per_head;  // ring stage and its parity, query tile of step p
+    int2 span = make_int2(key, args.S);       // queries [x, y) that see this key, with MODS
+    if (MODS != 0 && (spans != nullptr || key >= args.S)) span = key < args.S ? __ldg(spans + key) : make_int2(0, 0);
+    const float cap_inv = (MODS & MOD_CAP) ? 1.f / args.mods.cap_log2 : 0.f;
     for (int it = p; it < n_it; it += 2) {
       const int q0 = (i_start + i) * BQ;
       // a bounded wait that runs out ends the warp's work (the lanes decide together: TMEM accesses are warp-wide)
@@ -286,7 +328,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       const float4* stat = reinterpret_cast<const float4*>(sStat + st * STAT_FLOATS);
       // queries [0, hidden) of the tile do not see this key: those in front of it, all when the key is past the end
       const int hidden = key >= args.S ? BQ : (args.causal ? key - q0 : 0);
-      const bool any_hidden = __any_sync(0xffffffffu, hidden > 0);
+      const bool any_hidden = __any_sync(0xffffffffu, MODS == 0 ? hidden > 0 : (q0 < span.x || q0 + BQ > span.y));
+      const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h0 + it / per_head) * 1.4426950408889634f : 0.f;
+      const float far = (float)(q0 - key);
       // 32 queries at a time: all but a few words (28 bytes, 52 with shared key tiles) stay in registers; a spill goes to the L2, as
       // shared memory leaves no L1
 #pragma unroll
@@ -295,6 +339,40 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tmem_ld32(t + c * 32, s);
         tmem_ld32(t + 64 + c * 32, dp);
         tmem_ld_wait();
+        if (MODS != 0) {
+          if (MODS & MOD_CAP) cap_scores(s, args.mods);
+          const uint32_t seen = bit_range(span.x - q0 - c * 32, span.y - q0 - c * 32);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const float4 nl4 = stat[c * 8 + v], dl4 = stat[BQ / 4 + c * 8 + v];
+            const float nl[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, dl[4] = {dl4.x, dl4.y, dl4.z, dl4.w};
+            float x[4], g[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float y = __uint_as_float(s[4 * v + e]);
+              g[e] = __uint_as_float(dp[4 * v + e]) - dl[e];
+              if (MODS & MOD_CAP) {
+                const float t = y * cap_inv;
+                g[e] *= fmaf(-t, t, 1.f);
+                y += nl[e];
+              } else {
+                y = fmaf(y, sl2, nl[e]);
+              }
+              if (MODS & MOD_BIAS) y = fmaf(-slope, fabsf(far + (float)(c * 32 + 4 * v + e)), y);
+              x[e] = fast_exp2(y);
+              g[e] *= x[e];
+            }
+            if (any_hidden) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!((seen >> (4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
+            }
+            pk[2 * v] = pack_bf16x2(x[0], x[1]);
+            pk[2 * v + 1] = pack_bf16x2(x[2], x[3]);
+            dk[2 * v] = pack_bf16x2(g[0], g[1]);
+            dk[2 * v + 1] = pack_bf16x2(g[2], g[3]);
+          }
+        } else
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
           const float4 nl = stat[c * 8 + v], dl = stat[BQ / 4 + c * 8 + v];
@@ -328,7 +406,17 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (st >= STAGES) { st -= STAGES; ph ^= 1; }
     }
     // the results: the even steps' warps write dV, the odd steps' warps dK (TMEM lane == key)
-    if (alive && __all_sync(0xffffffffu, mbar_wait(all_done, 0, 222))) {
+    if (MODS != 0 && n_it == 0) {  // nothing but padding: zeros
+      if (key < args.S) {
+        if (SHARED) {
+          float4* dst = args.dkv_parts + part_tile(part, args.B, b, (args.S + BKV - 1) / BKV, jt, args.Hkv, hk, p == 0 ? 1 : 0) + row;
+          for (int v = 0; v < HD / 4; ++v) dst[v * BKV] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>((p == 0 ? args.dv : args.dk) + ((long long)b * args.S + key) * args.dkv_stride + hk * HD);
+          for (int v = 0; v < HD / 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    } else if (alive && __all_sync(0xffffffffu, mbar_wait(all_done, 0, 222))) {
       tc_fence_after();
       const uint32_t src = (p == 0 ? tdV : tdK) + ((uint32_t)((warp & 3) * 32) << 16);
       const float f = p == 0 ? 1.f : args.scale;
@@ -573,12 +661,13 @@ int head_parts_for(int B, int S, int Hq, int Hkv) {
 
 // The three launches of one backward pass (delta pre-pass, main kernel, dQ conversion), shared by both entry points.
 // Allocates nothing: the tensor maps come by reference from the caller, the scratch by pointer.
+template <int MODS>
 static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
                            const CUtensorMap& mdq, const void* out,
                            const void* dout, const float* lse, float* delta, float* dq_accum, void* dq, void* dk, void* dv, int B,
                            int S, int Hq, int Hkv, long long o_stride, long long do_stride, long long dq_stride,
-                           long long dkv_stride, float scale, int causal, cudaStream_t st) {
-  const auto kernel = dkv_parts != nullptr ? attn_bwd_kernel<true> : attn_bwd_kernel<false>;
+                           long long dkv_stride, float scale, int causal, const AttnMods& mods, cudaStream_t st) {
+  const auto kernel = dkv_parts != nullptr ? attn_bwd_kernel<true, MODS> : attn_bwd_kernel<false, MODS>;
   static bool optin[2][64] = {};  // the shared-memory opt-in is a per-device attribute
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -613,6 +702,7 @@ static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, 
   a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal ? 1 : 0;
+  a.mods = mods;
   const int n_kt = (S + BKV - 1) / BKV;
   a.head_group = head_group_size(n_kt, B * Hkv * head_parts, T * Hq * HD * 4, yf_num_sms());  // the dQ accumulator
   const long long ctas = (long long)n_kt * B * Hkv * head_parts;
@@ -642,10 +732,10 @@ extern "C" int yf_attn_bwd_head_parts(int B, int S, int Hq, int Hkv) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
   return head_parts_for(B, S, Hq, Hkv);
 }
-extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+static int attn_bwd_any(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                                  float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, const float* rope, void* dq, void* dk, void* dv, int B,
                                  int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
-                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, void* stream) {
+                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, int which, const AttnMods& mods, void* stream) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
   if (head_parts < 1 || (Hq / Hkv) % head_parts || (head_parts > 1) != (dkv_parts != nullptr)) return -1;
   if (dkv_parts != nullptr && dkv_floats < 4 * part_tile(head_parts, B, 0, (S + BKV - 1) / BKV, 0, Hkv, 0, 0)) return -1;
@@ -662,8 +752,32 @@ extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, co
   const CUtensorMap* md = yf_tensor_map_3d(dout, (uint64_t)Hq * HD, S, B, do_stride, (uint64_t)S * do_stride, 64, BQ, 1, 2, 1);
   const CUtensorMap* mdq = yf_tensor_map_3d(dq_accum, (uint64_t)Hq * HD, S, B, (uint64_t)Hq * HD, (uint64_t)S * Hq * HD, 32, BQ, 1, 4, 0);
   if (!mq || !mk || !mv || !md || !mdq) return -2;
-  return attn_bwd_launch(head_parts, dkv_parts, rope, *mq, *mk, *mv, *md, *mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv,
-                         o_stride, do_stride, dq_stride, dkv_stride, scale, causal, st);
+  const auto launch = which == 0 ? attn_bwd_launch<0>
+                      : which == MOD_SPANS ? attn_bwd_launch<MOD_SPANS>
+                      : which == (MOD_SPANS | MOD_CAP) ? attn_bwd_launch<MOD_SPANS | MOD_CAP>
+                      : which == (MOD_SPANS | MOD_BIAS) ? attn_bwd_launch<MOD_SPANS | MOD_BIAS>
+                                                        : attn_bwd_launch<MOD_SPANS | MOD_CAP | MOD_BIAS>;
+  return launch(head_parts, dkv_parts, rope, *mq, *mk, *mv, *md, *mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv,
+                o_stride, do_stride, dq_stride, dkv_stride, scale, causal, mods, st);
+}
+extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                                 float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, const float* rope, void* dq, void* dk, void* dv, int B,
+                                 int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
+                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, void* stream) {
+  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, rope, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
+                      o_stride, do_stride, dq_stride, dkv_stride, scale, causal, 0, AttnMods{}, stream);
+}
+// Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal).
+extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta,
+                                float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S,
+                                int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
+                                long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding,
+                                void* stream) {
+  if (!(softcap >= 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7)) return -1;
+  const AttnMods m = attn_mods(scale, softcap, slopes, key_spans, padding);
+  const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
+  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, nullptr, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
+                      o_stride, do_stride, dq_stride, dkv_stride, scale, 1, mods, m, stream);
 }
 extern "C" int yf_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                            float* delta, float* dq_accum, void* dq, void* dk, void* dv, int B, int S, int Hq, int Hkv,
@@ -752,6 +866,6 @@ extern "C" int yf_attn_bwd_noalloc(const void* q, const void* k, const void* v, 
       yf_tensor_map_3d_encode(&md, dout, (uint64_t)Hq * HD, S, B, do_stride, (uint64_t)S * do_stride, 64, BQ, 1, 2, 1) != 0 ||
       yf_tensor_map_3d_encode(&mdq, dq_accum, (uint64_t)Hq * HD, S, B, (uint64_t)Hq * HD, (uint64_t)S * Hq * HD, 32, BQ, 1, 4, 0) != 0)
     return -2;
-  return attn_bwd_launch(1, nullptr, nullptr, mq, mk, mv, md, mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv, o_stride, do_stride, dq_stride,
-                         dkv_stride, scale, causal, st);
+  return attn_bwd_launch<0>(1, nullptr, nullptr, mq, mk, mv, md, mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv, o_stride, do_stride, dq_stride,
+                         dkv_stride, scale, causal, AttnMods{}, st);
 }

@@ -1,0 +1,86 @@
+// What the attention kernels do to a score between Q K^T and the softmax, and which keys a query sees, beyond the plain causal form:
+//   score = cap tanh(scale q.k / cap) - slope_h |i - j|       (either part optional)
+//   query i sees the keys spans[i] = [lo, hi); key j is seen by the queries key_spans[j]; padding sees and is seen by nothing
+// The kernels are instantiated for sets of these bits (0: plain causal attention, without any of this):
+#pragma once
+#include "common.cuh"
+
+constexpr int MOD_SPANS = 1;  // ranges from memory, or causal without any
+constexpr int MOD_CAP = 2;
+constexpr int MOD_BIAS = 4;
+
+struct AttnMods {
+  const int2* spans;    // [B, S] by query (forward) or by key (backward); null: causal
+  const int* padding;   // [B, ceil(S / 128)] padded tokens of every 128; null with spans
+  const float* slopes;  // [Hq]
+  float cap_log2;       // cap * log2(e)
+  float cap_exp;        // 2 log2(e) scale / cap: tanh of a raw product s is 1 - 2 / (1 + 2^(s * cap_exp))
+  float poly_max;       // |s| up to here: cap_log2 * tanh(s * scale / cap) = s * (poly[0] + poly[1] s^2 + ...)
+  float poly[5];
+};
+
+// The host's part: tanh(x) / x as a polynomial in x^2, fitted for the least relative error (6e-7) on |x| <= 3/4, with the scale and
+// the cap multiplied in.  Caps so small that the factors would leave fp32 do without.
+inline AttnMods attn_mods(float scale, float softcap, const float* slopes, const int* spans, const int* padding) {
+  AttnMods m = {};
+  m.spans = reinterpret_cast<const int2*>(spans);
+  m.padding = padding;
+  m.slopes = slopes;
+  if (softcap > 0.f) {
+    const double fit[5] = {0.999999435, -0.333282511, 0.132589789, -0.0500561567, 0.0129294833};
+    const double x = (double)scale / (double)softcap, cap = 1.4426950408889634 * (double)softcap;
+    m.cap_log2 = (float)cap;
+    m.cap_exp = (float)(2.8853900817779268 * x);
+    m.poly_max = x < 1000. ? (float)(0.75 / x) : -1.f;
+    double power = cap * x;
+    for (int i = 0; i < 5; ++i, power *= x * x) m.poly[i] = x < 1000. ? (float)(fit[i] * power) : 0.f;
+  }
+  return m;
+}
+
+// cap * log2(e) * tanh(s * scale / cap) for a raw product s: the polynomial where it holds, else from the exponential (absolute error
+// about 2^-22 of the cap; the hardware's tanh is good to 2^-11 relative, 2 % of a probability at a cap of 50).  Both in one:
+YF_DEVINL float capped_small(float s, const AttnMods& m) {
+  const float z = s * s;
+  return s * fmaf(fmaf(fmaf(fmaf(m.poly[4], z, m.poly[3]), z, m.poly[2]), z, m.poly[1]), z, m.poly[0]);
+}
+YF_DEVINL float capped_any(float s, const AttnMods& m) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * m.cap_exp)));
+  return fabsf(s) <= m.poly_max ? capped_small(s, m) : fmaf(-2.f * m.cap_log2, r, m.cap_log2);
+}
+// 32 scores in place.  What becomes of a score does not depend on its neighbours.
+YF_DEVINL void cap_scores(uint32_t (&s)[32], const AttnMods& m) {
+  float far = 0.f;
+#pragma unroll
+  for (int t = 0; t < 32; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
+  if (far <= m.poly_max) {
+#pragma unroll
+    for (int t = 0; t < 32; ++t) s[t] = __float_as_uint(capped_small(__uint_as_float(s[t]), m));
+  } else {
+#pragma unroll
+    for (int t = 0; t < 32; ++t) s[t] = __float_as_uint(capped_any(__uint_as_float(s[t]), m));
+  }
+}
+
+// bits [from, to) of a word, for ends anywhere
+YF_DEVINL uint32_t bit_range(int from, int to) {
+  const uint32_t below_to = to >= 32 ? 0xffffffffu : to <= 0 ? 0u : (1u << to) - 1u;
+  const uint32_t below_from = from >= 32 ? 0xffffffffu : from <= 0 ? 0u : (1u << from) - 1u;
+  return below_to & ~below_from;
+}
+
+// Zeros in the padded rows of a shared-memory tile of `rows` tokens from `t0` on, two swizzled halves of 128 bytes a row `half_bytes`
+// apart: padding is multiplied by probabilities of zero, but may hold anything, infinities and NaN included.  One warp; `spans` of
+// the sequence (padding: an empty range).
+YF_DEVINL void zero_padded_rows(uint8_t* tile, int half_bytes, int rows, int t0, int S, const int2* spans) {
+  for (int r = threadIdx.x & 31; r < rows; r += 32) {
+    if (t0 + r >= S) break;  // past the end: zeros already
+    const int2 s = __ldg(spans + t0 + r);
+    if (s.x < s.y) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + h * half_bytes + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}

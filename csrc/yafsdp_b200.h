@@ -107,6 +107,16 @@ int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* o
                       int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
                       long long dkv_stride, float scale, int causal, void* stream);
 
+/* The same with scores capped at +-softcap (0: not), less slopes[h] * distance (fp32, null: not), and ranges of keys (queries in the backward
+   pass) for every token, as yf_document_mask gives them (null: causal).  A token without keys: zeros, lse -inf. */
+int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq, int Hkv, long long q_stride,
+                     long long kv_stride, long long out_stride, float scale, float softcap, const float* slopes, const int* spans,
+                     const int* padding, void* stream);
+int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta,
+                     float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S, int Hq,
+                     int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
+                     long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding, void* stream);
+
 // No counterpart in the reference.  yf_attn_bwd for callers that cannot allocate device memory (a plain C host
 // without a tensor framework, or a job whose own pool already holds the whole GPU): the delta / dQ-accumulator
 // scratch is a fixed device array inside the library (about 16.1 MiB per GPU, held until exit), so the call takes
@@ -117,6 +127,21 @@ int yf_attn_bwd_noalloc(const void* q, const void* k, const void* v, const void*
                         void* dq, void* dk, void* dv, int B, int S, int Hq, int Hkv, long long q_stride, long long kv_stride,
                         long long o_stride, long long do_stride, long long dq_stride, long long dkv_stride, float scale,
                         int causal, void* stream);
+
+// ---- packed batches (packed.cu)
+int yf_document_mask(const void* ids, int ids_64, const void* prefix, int* spans, int* key_spans, int* positions, int* padding, int B, int S,
+                     long long ids_stride, long long prefix_stride, int window, void* stream);
+int yf_rotary(const void* q, const void* k, void* q_out, void* k_out, const void* positions, int pos_64, long long axis_stride, const void* table,
+              long long tokens, int q_heads, int k_heads, int head_dim, long long q_token, long long q_head, long long k_token, long long k_head,
+              long long q_out_token, long long k_out_token, int dtype, int sign, void* stream);
+
+// ---- the norms between two blocks, their gate and the residual add (residual_norm.cu)
+int yf_residual_norm_fwd(const void* x, const void* y, const void* weight, const void* post, const void* gate, int gate_rows, void* h, void* n,
+                         float* rstd, int T, int D, float scale, float eps, int dtype, void* stream);
+int yf_residual_norm_parts(int T, int D, int gate_rows);
+int yf_residual_norm_bwd(const void* x, const void* y, const void* weight, const void* post, const void* gate, int gate_rows, const float* rstd,
+                         const void* dh, const void* dn, void* dx, void* dy, void* dw, int dw_kind, float* dw_sumsq, void* dpost, int dpost_kind,
+                         float* dpost_sumsq, void* dgate, float* parts, long long parts_floats, int T, int D, float scale, int dtype, void* stream);
 
 // ---- peer-memory collectives over NVLink (comm.cu); peer arrays are host arrays of `world` device pointers
 int yf_allgather_pull(void* const* peer_in, void* out, long long shard_bytes, int rank, int world, int n_ctas, void* stream);

@@ -400,3 +400,392 @@ def head_logits(h: torch.Tensor, w_norm: torch.Tensor, w_head: torch.Tensor, eps
     if h.is_cuda:
         return HeadLogitsFn.apply(h, w_norm, w_head, eps)
     return F.linear(rmsnorm_ref(h, w_norm, eps), w_head)
+
+
+# ------------------------------------------------------------------------------------- packed documents
+def _elsewhere(t: torch.Tensor) -> bool:
+    return t.is_cuda and t.device.index != torch._C._cuda_getDevice()
+
+
+def _one_device(what: str, *ts: torch.Tensor | None) -> None:
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devices))}")
+
+
+@dataclass(frozen=True)
+class DocumentMask:
+    """Which tokens of a packed batch see each other (:func:`document_mask`): query ``i`` of a row sees the keys ``spans[i, 0] <= j <
+    spans[i, 1]``, key ``j`` is seen by the queries ``key_spans[j, 0] <= i < key_spans[j, 1]``.  ``positions``: index of a token in its
+    document.  ``padding``: padded tokens in every 128 of a row."""
+
+    spans: torch.Tensor  # [B, S, 2] int32
+    key_spans: torch.Tensor  # [B, S, 2] int32
+    positions: torch.Tensor  # [B, S] int32
+    padding: torch.Tensor  # [B, ceil(S / 128)] int32
+
+
+def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None, window: int = 0) -> DocumentMask:
+    """The mask of packed rows ``document_ids [B, S]`` (int32 or int64).  Tokens see each other inside a document, which is a run of equal ids
+    >= 0, and causally; negative ids are padding, which sees and is seen by nothing.  ``prefix [B, S]`` (bool): the flagged tokens
+    that a document starts with also see each other backwards.  ``window``: keys ``window`` or more tokens back are hidden (0: none are)."""
+    if document_ids.dim() != 2 or document_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"document_mask: document_ids must be [B, S] int32 or int64, got {list(document_ids.shape)} {document_ids.dtype}")
+    if prefix is not None and (prefix.shape != document_ids.shape or prefix.dtype != torch.bool):
+        raise ValueError(f"document_mask: prefix must be bool {list(document_ids.shape)}, got {list(prefix.shape)} {prefix.dtype}")
+    if not 0 <= window < 1 << 31:
+        raise ValueError(f"document_mask: window must be at least 0 and below 2^31, got {window}")
+    if document_ids.shape[1] > 1 << 30:
+        raise ValueError(f"document_mask: rows of at most 2^30 tokens, got {document_ids.shape[1]}")
+    _one_device("document_mask", document_ids, prefix)
+    if not document_ids.is_cuda:
+        return _document_mask_ref(document_ids, prefix, window)
+    if _elsewhere(document_ids):
+        with torch.cuda.device(document_ids.device):
+            return document_mask(document_ids, prefix, window)
+    ids, flags = (t if t is None or t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous() for t in (document_ids, prefix))
+    return DocumentMask(*kernels.document_mask(ids, flags, window))
+
+
+def _document_mask_ref(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -> DocumentMask:
+    b, s = ids.shape
+    at = torch.arange(s).expand(b, s)
+    if b * s == 0:
+        empty = torch.zeros((b, s, 2), dtype=torch.int32)
+        return DocumentMask(empty, empty.clone(), torch.zeros((b, s), dtype=torch.int32), torch.zeros((b, (s + 127) // 128), dtype=torch.int32))
+    starts = torch.cat([torch.ones((b, 1), dtype=torch.bool), ids[:, 1:] != ids[:, :-1]], 1)
+    start = torch.where(starts, at, 0).cummax(1).values
+    end = torch.where(starts.roll(-1, 1), at + 1, s).flip(1).cummin(1).values.flip(1)
+    lead, run_end = torch.zeros_like(starts), end
+    if prefix is not None:
+        lead = torch.where(prefix, -1, at).cummax(1).values < start
+        run_end = torch.minimum(end, torch.where(prefix, s, at).flip(1).cummin(1).values.flip(1))
+    lo, hi = start, torch.where(lead, run_end, at + 1)
+    first, stop = torch.where(lead, start, at), end
+    if window:
+        lo, stop = torch.maximum(lo, at - window + 1), torch.minimum(stop, at + window)
+    pad = ids < 0
+    lo, hi, first, stop = (torch.where(pad, at, t) for t in (lo, hi, first, stop))
+    padding = F.pad(pad, (0, -s % 128)).view(b, -1, 128).sum(2)
+    return DocumentMask(torch.stack([lo, hi], -1).int(), torch.stack([first, stop], -1).int(), torch.where(pad, 0, at - start).int(), padding.int())
+
+
+class RotaryAxes:
+    """Frequencies of rotary positions with one or several axes.  Pair ``j`` of a head (dims ``j`` and ``j + head_dim / 2``) turns by
+    ``positions[axis of j] * theta ** (-2 j / head_dim)``.  ``sections``: how many pairs follow each axis (their sum is ``head_dim / 2``; one
+    axis by default).  The pairs of an axis lie side by side, or, with ``interleaved``, are dealt to the axes in turn as long as an
+    axis has pairs left."""
+
+    def __init__(self, head_dim: int, theta: float, sections: "tuple[int, ...] | None" = None, interleaved: bool = False):
+        if head_dim <= 0 or head_dim % 16 or head_dim > 512:
+            raise ValueError(f"RotaryAxes: head_dim must be a multiple of 16 up to 512, got {head_dim}")
+        if not theta > 0:
+            raise ValueError(f"RotaryAxes: theta must be positive, got {theta}")
+        half = head_dim // 2
+        self.sections = (half,) if sections is None else tuple(sections)
+        if any(n < 0 for n in self.sections) or sum(self.sections) != half:
+            raise ValueError(f"RotaryAxes: sections must add up to head_dim / 2 = {half}, got {self.sections}")
+        self.head_dim, self.theta = head_dim, theta
+        self.axis = [a for a, n in enumerate(self.sections) for _ in range(n)]
+        if interleaved:
+            left, self.axis = list(self.sections), []
+            while any(left):
+                for a in range(len(left)):
+                    if left[a]:
+                        left[a] -= 1
+                        self.axis.append(a)
+        self.frequency = [theta ** (-2.0 * j / head_dim) for j in range(half)]
+        self._tables: dict[torch.device, torch.Tensor] = {}
+
+    def table(self, device: torch.device) -> torch.Tensor:
+        """``[head_dim / 2, 2]`` int64: the fraction of a turn per position in 2^-64, and the axis.  Made once per device, outside of graph
+        captures."""
+        t = self._tables.get(device)
+        if t is None:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("RotaryAxes: call rotary() or table() on this device once before capturing a graph")
+            turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequency]
+            t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64).to(device)
+            self._tables[device] = t
+        return t
+
+
+def _tokens(t: torch.Tensor) -> torch.Tensor:
+    """``[B, S, H, D]`` as ``[B*S, H, D]`` that the kernels can read in place, or a copy that they can."""
+    t = t.detach().reshape(-1, t.shape[2], t.shape[3])
+    step = 16 // t.element_size()
+    good = (t.stride(2) == 1 and (t.shape[0] <= 1 or t.stride(0) % step == 0) and (t.shape[1] <= 1 or t.stride(1) % step == 0) and t.data_ptr() % 16 == 0)
+    if not good:
+        t = t.clone(memory_format=torch.contiguous_format)
+    if t.shape[0] > 1 and t.shape[1] > 1:
+        return t
+    # strides of axes that have one element may be anything
+    return t.as_strided(t.shape, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2], t.stride(1) if t.shape[1] > 1 else t.shape[2], 1))
+
+
+class RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor) -> Any:  # type: ignore[override]
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, table)
+        q2, k2 = kernels.rotary(_tokens(q), _tokens(k), positions, table)
+        assert q2 is not None and k2 is not None
+        return q2.view(q.shape), k2.view(k.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
+    def backward(ctx: Any, dq: torch.Tensor | None, dk: torch.Tensor | None) -> Any:  # type: ignore[override]
+        positions, table = ctx.saved_tensors
+        if dq is None and dk is None:
+            return None, None, None, None
+        gq, gk = kernels.rotary(None if dq is None else _tokens(dq), None if dk is None else _tokens(dk), positions, table, backward=True)
+        return None if dq is None else gq.view(dq.shape), None if dk is None else gk.view(dk.shape), None, None
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> tuple[torch.Tensor, torch.Tensor]:
+    """``q [B, S, Hq, D]`` and ``k [B, S, Hk, D]`` (bf16, fp16 or fp32) turned by ``positions`` (int32 or int64): ``[B, S]`` for one axis, else
+    ``[axes, B, S]``.  Angles are exact to 2^-31 of a turn at any position."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != axes.head_dim or k.shape[3] != axes.head_dim:
+        raise ValueError(f"rotary: q and k must be [B, S, heads, {axes.head_dim}] of the same batch, got {list(q.shape)} and {list(k.shape)}")
+    if q.dtype != k.dtype or q.dtype not in kernels._DTYPES:
+        raise TypeError(f"rotary: q and k must both be bf16, fp16 or fp32, got {q.dtype} and {k.dtype}")
+    n, tokens = len(axes.sections), q.shape[:2]
+    if positions.dtype not in (torch.int32, torch.int64) or (positions.shape != (n, *tokens) and not (n == 1 and positions.shape == tokens)):
+        raise ValueError(f"rotary: positions must be int32 or int64 {[n, *tokens]}, got {list(positions.shape)} {positions.dtype}")
+    _one_device("rotary", q, k, positions)
+    if not q.is_cuda:
+        return _rotary_ref(q, positions, axes), _rotary_ref(k, positions, axes)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return rotary(q, k, positions, axes)
+    pos = positions.reshape(n, -1)
+    if pos.shape[1] > 1 and pos.stride(1) != 1:
+        pos = pos.contiguous()
+    return RotaryFn.apply(q, k, pos, axes.table(q.device))  # type: ignore[no-any-return]
+
+
+def _rotary_ref(t: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
+    pos = positions.reshape(-1, *t.shape[:2])[axes.axis].permute(1, 2, 0).double()
+    ang = pos * torch.tensor(axes.frequency, dtype=torch.float64)
+    cos, sin = ang.cos().float().unsqueeze(2), ang.sin().float().unsqueeze(2)
+    a, b = t.float().chunk(2, dim=-1)
+    return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(t.dtype)
+
+
+# ------------------------------------------------------------------------------------- attention with masks, capped scores and a distance bias
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``[B, S, H, 128]`` as ``[B*S, H*128]`` rows that the kernels can read in place, or a copy that they can."""
+    width = t.shape[2] * t.shape[3]
+    r = t.detach().reshape(t.shape[0] * t.shape[1], width)
+    if r.data_ptr() % 16 or r.stride(1) != 1 or (r.shape[0] > 1 and (r.stride(0) % 8 or r.stride(0) < width)):
+        r = r.clone(memory_format=torch.contiguous_format)
+    return r if r.shape[0] > 1 else r.as_strided(r.shape, (width, 1))  # the stride of an axis with one element may be anything
+
+
+class AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,  # type: ignore[override]
+                slopes: torch.Tensor | None, keep: bool) -> torch.Tensor:
+        b, s, hq, _ = q.shape
+        hkv = k.shape[2]
+        q2, k2, v2 = _rows(q), _rows(k), _rows(v)
+        if k2.stride(0) != v2.stride(0):
+            k2, v2 = k2.contiguous(), v2.contiguous()
+        plain = mask is None and softcap == 0 and slopes is None
+        if q2.numel() == 0:
+            out, lse = torch.empty_like(q2, memory_format=torch.contiguous_format), q2.new_empty((b, hq, s), dtype=torch.float32)
+        elif plain:
+            out, lse = kernels.attn_fwd(q2, k2, v2, b, s, hq, hkv, scale)
+        else:
+            spans, padding = (None, None) if mask is None else (mask.spans, mask.padding)
+            out, lse = kernels.attn_fwd_mods(q2, k2, v2, b, s, hq, hkv, scale, softcap, slopes, spans, padding)
+        if keep:
+            ctx.save_for_backward(q2, k2, v2, out, lse, slopes, *((None, None) if mask is None else (mask.key_spans, mask.padding)))
+            ctx.args = (b, s, hq, hkv, scale, softcap, plain)
+        return out.view(q.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
+    def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
+        q, k, v, out, lse, slopes, key_spans, padding = ctx.saved_tensors
+        b, s, hq, hkv, scale, softcap, plain = ctx.args
+        dq, dk, dv = torch.empty_like(out), *(torch.empty((b * s, hkv * 128), device=k.device, dtype=k.dtype) for _ in range(2))
+        if out.numel() > 0:
+            g = _rows(dout)
+            if plain:
+                kernels.attn_bwd(q, k, v, out, g, lse, dq, dk, dv, b, s, hq, hkv, scale)
+            else:
+                kernels.attn_bwd_mods(q, k, v, out, g, lse, dq, dk, dv, b, s, hq, hkv, scale, softcap, slopes, key_spans, padding)
+        return dq.view(b, s, hq, 128), dk.view(b, s, hkv, 128), dv.view(b, s, hkv, 128), None, None, None, None, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None = None, *, scale: float | None = None, softcap: float = 0.0,
+              slopes: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``q [B, S, Hq, D]`` over ``k``, ``v [B, S, Hkv, D]`` (query head ``h`` reads key head ``h // (Hq // Hkv)``), causal or under
+    ``mask``; the result has the shape of ``q``, zeros where a token sees nothing.  The score of query ``i`` and key ``j`` is ``t = scale *
+    q.k`` (``scale``: ``D ** -0.5``), ``softcap * tanh(t / softcap)`` with a ``softcap``, less ``slopes[h] * |i - j|`` with ``slopes [Hq]``
+    (constants: they get no gradient).  On CUDA: bf16, ``D`` = 128.  Tensors whose heads lie side by side in rows at a pitch of
+    16 bytes are read in place (parts of a fused projection), others are copied first.  What padding holds does not matter; any other
+    value is taken to be finite: an infinity or NaN of one document may reach the documents that share a tile of 128 tokens with it."""
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"attention: q [B, S, Hq, D], k and v [B, S, Hkv, D] expected, got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"attention: {q.shape[2]} query heads are no multiple of {k.shape[2]} key heads")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"attention: q, k and v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap)
+    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
+        raise ValueError(f"attention: scale must be positive and softcap not negative, got {scale} and {softcap}")
+    if mask is not None and (mask.spans.shape[:2] != q.shape[:2] or mask.key_spans.shape[:2] != q.shape[:2]):
+        raise ValueError(f"attention: the mask is for {list(mask.spans.shape[:2])} tokens, q has {list(q.shape[:2])}")
+    if slopes is not None and slopes.shape != (q.shape[2],):
+        raise ValueError(f"attention: slopes must have one value for each of {q.shape[2]} query heads, got {list(slopes.shape)}")
+    if slopes is not None and slopes.requires_grad:
+        raise ValueError("attention: slopes get no gradient; pass slopes.detach()")
+    _one_device("attention", q, k, v, slopes, None if mask is None else mask.spans)
+    if not q.is_cuda:
+        return _attention_ref(q, k, v, mask, scale, softcap, slopes)
+    if q.dtype != torch.bfloat16 or q.shape[3] != 128:
+        raise TypeError(f"attention: the CUDA kernels take bf16 heads of 128, got {q.dtype} heads of {q.shape[3]}")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes)
+    if slopes is not None:
+        slopes = _c(slopes.float())
+    return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes, torch.is_grad_enabled())  # type: ignore[no-any-return]
+
+
+def _attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,
+                   slopes: torch.Tensor | None) -> torch.Tensor:
+    s, group = q.shape[1], q.shape[2] // k.shape[2]
+    at = torch.arange(s)
+    if mask is None:
+        seen = (at[None, :] <= at[:, None])[None]
+    else:
+        seen = (at >= mask.spans[..., :1]) & (at < mask.spans[..., 1:])
+    score = torch.einsum("bihd,bjhd->bhij", q.float(), k.float().repeat_interleave(group, 2)) * scale
+    if softcap:
+        score = softcap * torch.tanh(score / softcap)
+    if slopes is not None:
+        score = score - slopes.float()[:, None, None] * (at[:, None] - at[None, :]).abs()
+    # a row without keys is given all of them, and zeros afterwards
+    some = seen.any(2)[:, None, :, None]
+    p = score.masked_fill(~seen[:, None] & some, -math.inf).softmax(-1) * some
+    return torch.einsum("bhij,bjhd->bihd", p, v.float().repeat_interleave(group, 2)).to(q.dtype)
+
+
+# ------------------------------------------------------------------------------------- the residual step between two blocks
+class ResidualNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,  # type: ignore[override]
+                gate_rows: int, scale: float, eps: float, keep: bool) -> Any:
+        ctx.set_materialize_grads(False)
+        d = x.shape[-1]
+        x2, y2, w = _aligned(x).view(-1, d), _aligned(y).view(-1, d), _aligned(weight)
+        p, g = None if post is None else _aligned(post), None if gate is None else _aligned(gate)
+        if x2.shape[0] > 0:
+            h, n, rstd = kernels.residual_norm_fwd(x2, y2, w, p, g, gate_rows, scale, eps, keep)
+        else:
+            h, n, rstd = torch.empty_like(x2), torch.empty_like(x2), None
+        if keep:
+            # the inputs themselves, as torch's own layers do: the values of a sharded parameter are gathered anew for the backward pass
+            ctx.save_for_backward(x, y, weight, post, gate, rstd)
+            ctx.params = (weight, post)  # as parameters of a group they know where their gradients go
+            ctx.args = (gate_rows, scale)
+        return h.view(x.shape), n.view(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
+    def backward(ctx: Any, dh: torch.Tensor | None, dn: torch.Tensor | None) -> Any:  # type: ignore[override]
+        x, y, w, p, g, rstd = ctx.saved_tensors
+        gate_rows, scale = ctx.args
+        if x.numel() == 0:
+            return *(None if t is None else torch.zeros_like(t) for t in (x, y, w, p, g)), None, None, None, None
+        shape, gate_shape = x.shape, None if g is None else g.shape
+        x, y, w, p, g = (None if t is None else _aligned(t) for t in (x, y, w, p, g))
+        x, y = x.view(-1, shape[-1]), y.view(-1, shape[-1])
+        outs = [None if t is None else _ParamGrad(t, x.dtype) for t in ctx.params]
+        a, b = outs[0], outs[1]
+        assert a is not None
+        dx, dy, dgate = kernels.residual_norm_bwd(
+            x, y, w, p, g, gate_rows, rstd, *(None if t is None else _aligned(t).view(x.shape) for t in (dh, dn)), scale, a.out, None if b is None else b.out,
+            add_dw=a.add, add_dpost=b is not None and b.add, dw_sumsq=a.sumsq, dpost_sumsq=None if b is None else b.sumsq)
+        return (dx.view(shape), dy.view(shape), a.result(), None if b is None else b.result(), None if dgate is None else dgate.view(gate_shape),
+                None, None, None, None)
+
+
+class _ParamGrad:
+    """Where a kernel that finishes a whole norm weight gradient in one go writes it: the parameter's fp32 sink when it has one, else a tensor of
+    the parameter's type."""
+
+    def __init__(self, p: torch.Tensor, dtype: torch.dtype):
+        self.sink, self.add, self.sumsq = _sink(p), False, None
+        self.pushed = self.sink is not None and self.sink.pushes()
+        self.sunk = self.sink is not None and not self.pushed and self.sink.local_ok
+        if self.sunk:
+            self.out, self.add = self.sink.begin()
+            self.sumsq = self.sink.norm_target(self.add)
+        else:
+            self.out = torch.empty(p.shape, device=p.device, dtype=torch.float32 if self.pushed else dtype)
+
+    def result(self) -> torch.Tensor | None:
+        if self.pushed:
+            self.sink.push_from(self.out)
+        return None if self.pushed or self.sunk else self.out
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    t = _c(t.detach())
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
+    """How many rows of ``x.shape[-1]`` the gate has, each for as many consecutive tokens."""
+    lead = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape[:-1])
+    same = 0
+    while same < len(lead) and lead[same] == x.shape[same]:
+        same += 1
+    if gate.dim() == 0 or gate.dim() > x.dim() or gate.shape[-1] != x.shape[-1] or any(n != 1 for n in lead[same:]):
+        raise ValueError(f"residual_norm: gate must have the shape of x, {list(x.shape)}, with trailing axes before the last left out or of size one, got {list(gate.shape)}")
+    return math.prod(lead)
+
+
+def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                  scale: float = 1.0, eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor]:
+    """The residual step between two blocks, in one kernel: ``h = x + scale * gate * u``, where ``u`` is the block's output ``y``, normalised
+    with ``post_weight`` if that is given, and ``n = rmsnorm(h) * weight``, the input of the next block.  Returns ``(h, n)``.  ``x``, ``y``: ``[...,
+    D]``; weights ``[D]``; ``gate``: ``[D]`` for every channel, ``[B, 1, D]`` for every sample of ``[B, S, D]``, or the shape of ``x``.  All of
+    one type (bf16, fp16 or fp32); sums are fp32 and each result is rounded once.  ``D``: a multiple of 8 up to 16384 on CUDA."""
+    if x.dim() < 1 or x.shape != y.shape:
+        raise ValueError(f"residual_norm: x and y must have one shape [..., D], got {list(x.shape)} and {list(y.shape)}")
+    for t in (weight, post_weight):
+        if t is not None and t.shape != x.shape[-1:]:
+            raise ValueError(f"residual_norm: weights must be [{x.shape[-1]}], got {list(t.shape)}")
+    if any(t is not None and t.dtype != x.dtype for t in (y, weight, post_weight, gate)) or x.dtype not in kernels._DTYPES:
+        raise TypeError(f"residual_norm: all tensors must have one type (bf16, fp16 or fp32), got {[str(t.dtype) for t in (x, y, weight, post_weight, gate) if t is not None]}")
+    scale, eps = float(scale), float(eps)
+    if not math.isfinite(scale) or not 0.0 < eps < math.inf:
+        raise ValueError(f"residual_norm: scale must be finite and eps positive, got {scale} and {eps}")
+    rows = 0 if gate is None else _gate_rows(gate, x)
+    _one_device("residual_norm", x, y, weight, post_weight, gate)
+    if not x.is_cuda:
+        return _residual_norm_ref(x, y, weight, post_weight, gate, scale, eps)
+    if x.shape[-1] % 8 or not 0 < x.shape[-1] <= 16384:
+        raise ValueError(f"residual_norm: the CUDA kernels take widths that are multiples of 8 up to 16384, got {x.shape[-1]}")
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)
+    return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps, torch.is_grad_enabled())  # type: ignore[no-any-return]
+
+
+def _residual_norm_ref(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, scale: float,
+                       eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    u = y.float()
+    if post is not None:
+        u = u * torch.rsqrt(u.pow(2).mean(-1, keepdim=True) + eps) * post.float()
+    if gate is not None:
+        u = u * gate.float()
+    h = x.float() + scale * u
+    n = h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
+    return h.to(x.dtype), n.to(x.dtype)

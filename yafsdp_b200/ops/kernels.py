@@ -479,3 +479,120 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
                                            dout.stride(0), dq.stride(0), dk.stride(0), float(scale), int(causal), _stream()),
            "yf_attn_bwd")
     _launches += 2  # delta pre-pass and dq conversion post-pass
+
+
+def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float,
+                  softcap: float, slopes: torch.Tensor | None, spans: torch.Tensor | None, padding: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`attn_fwd` with scores capped by ``softcap * tanh(score / softcap)`` (0: not), less ``slopes[h] * distance`` (fp32 ``[Hq]``), under
+    the key ranges of :func:`document_mask` (``None``: causal)."""
+    t = batch * seq
+    assert q.shape == (t, n_heads * 128) and k.shape == (t, n_kv_heads * 128) and v.shape == k.shape
+    assert q.stride(1) == 1 and k.stride(1) == 1 and v.stride(1) == 1 and k.stride(0) == v.stride(0)
+    out = torch.empty((t, n_heads * 128), device=q.device, dtype=torch.bfloat16)
+    lse = torch.empty((batch, n_heads, seq), device=q.device, dtype=torch.float32)
+    _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, seq, n_heads, n_kv_heads,
+                                          q.stride(0), k.stride(0), out.stride(0), scale, softcap, _ptr(slopes), _ptr(spans), _ptr(padding), _stream()),
+           "yf_attn_fwd_mods")
+    return out, lse
+
+
+def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor, lse: torch.Tensor, dq: torch.Tensor,
+                  dk: torch.Tensor, dv: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float, softcap: float,
+                  slopes: torch.Tensor | None, key_spans: torch.Tensor | None, padding: torch.Tensor | None, head_parts: int = 0) -> None:
+    """Backward of :func:`attn_fwd_mods` into the given views, as :func:`attn_bwd`."""
+    assert dout.stride(1) == 1 and out.stride(1) == 1 and dq.stride(1) == 1 and dk.stride(1) == 1 and dv.stride(1) == 1
+    assert dk.stride(0) == dv.stride(0)
+    delta = torch.empty((batch, n_heads, seq), device=q.device, dtype=torch.float32)
+    dq_acc = torch.empty((batch * seq, n_heads * 128), device=q.device, dtype=torch.float32)
+    parts = _attn_bwd_head_parts(batch, seq, n_heads, n_kv_heads, q.device.index) if head_parts == 0 else head_parts
+    dkv_parts = torch.empty((parts, 2, batch, (seq + 127) // 128 * 128, n_kv_heads * 128), device=q.device, dtype=torch.float32) if parts > 1 else None
+    global _launches
+    _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+                                          dq_acc.data_ptr(), _ptr(dkv_parts), 0 if dkv_parts is None else dkv_parts.numel(), parts, dq.data_ptr(),
+                                          dk.data_ptr(), dv.data_ptr(), batch, seq, n_heads, n_kv_heads, q.stride(0), k.stride(0), out.stride(0),
+                                          dout.stride(0), dq.stride(0), dk.stride(0), scale, softcap, _ptr(slopes), _ptr(key_spans), _ptr(padding),
+                                          _stream()), "yf_attn_bwd_mods")
+    _launches += 2  # delta pre-pass and dq conversion post-pass
+
+
+# --------------------------------------------------------------------------------------- packed batches
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def document_mask(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(spans [B,S,2], key_spans [B,S,2], positions [B,S], padding [B,ceil(S/128)])``, int32, of ``ids [B,S]`` (int32 or int64) and
+    optional flags ``prefix [B,S]`` (bool)."""
+    b, s = ids.shape
+    assert ids.dtype in (torch.int32, torch.int64) and (prefix is None or prefix.dtype == torch.bool)
+    assert all(t is None or s < 2 or t.stride(1) == 1 for t in (ids, prefix))
+    spans = torch.empty((2, b, s, 2), device=ids.device, dtype=torch.int32)
+    positions = torch.empty((b, s), device=ids.device, dtype=torch.int32)
+    padding = torch.empty((b, (s + 127) // 128), device=ids.device, dtype=torch.int32)
+    if b * s > 0:
+        _check(_native.lib().yf_document_mask(ids.data_ptr(), int(ids.dtype == torch.int64), _ptr(prefix), spans.data_ptr(),
+                                              spans.data_ptr() + 8 * b * s, positions.data_ptr(), padding.data_ptr(), b, s, ids.stride(0),
+                                              0 if prefix is None else prefix.stride(0), window, _stream()), "yf_document_mask")
+    return spans[0], spans[1], positions, padding
+
+
+def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
+           backward: bool = False) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """``q [T,Hq,D]`` and ``k [T,Hk,D]`` (either may be ``None``) turned by ``positions [axes,T]``; ``table [D/2,2]`` int64: a pair's frequency
+    (2^64 a whole turn) and its axis.  ``backward``: turned back.  Heads and tokens may lie apart by multiples of 16 bytes."""
+    some = q if q is not None else k
+    assert some is not None and positions.dtype in (torch.int32, torch.int64) and table.dtype == torch.int64
+    (t, _, d), dev, dtype = some.shape, some.device, some.dtype
+    assert positions.shape[1] == t and (t < 2 or positions.stride(1) == 1)
+    assert all(x is None or (x.shape[0] == t and x.shape[2] == d and x.stride(2) == 1 and x.dtype == dtype) for x in (q, k))
+    outs = [None if x is None else torch.empty(x.shape, device=dev, dtype=dtype) for x in (q, k)]
+    heads = [0 if x is None else x.shape[1] for x in (q, k)]
+    if t * sum(heads) > 0:
+        strides = [0 if x is None else x.stride(i) for x in (q, k) for i in (0, 1)]
+        _check(_native.lib().yf_rotary(_ptr(q), _ptr(k), _ptr(outs[0]), _ptr(outs[1]), positions.data_ptr(), int(positions.dtype == torch.int64),
+                                       positions.stride(0), table.data_ptr(), t, heads[0], heads[1], d, *strides, heads[0] * d, heads[1] * d,
+                                       _DTYPES[dtype], -1 if backward else 1, _stream()), "yf_rotary")
+    return outs[0], outs[1]
+
+
+# --------------------------------------------------------------------------------------- the residual step between two blocks
+def residual_norm_fwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, gate_rows: int,
+                      scale: float, eps: float, keep: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``h = x + scale * gate * norm(y) * post``, ``n = norm(h) * weight`` of ``[T,D]`` tensors of one type, and the norms' factors ``[T,2]`` (with
+    ``keep``).  ``gate``: ``gate_rows`` rows of ``D``, each for as many tokens in a row."""
+    t, d = x.shape
+    h, n = torch.empty_like(x), torch.empty_like(x)
+    rstd = torch.empty((t, 2), device=x.device, dtype=torch.float32) if keep else None
+    _check(_native.lib().yf_residual_norm_fwd(x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, h.data_ptr(), n.data_ptr(),
+                                              _ptr(rstd), t, d, scale, eps, _DTYPES[x.dtype], _stream()), "yf_residual_norm_fwd")
+    return h, n, rstd
+
+
+@functools.lru_cache(maxsize=4096)
+def _residual_norm_parts(t: int, d: int, gate_rows: int, device: int | None) -> int:
+    rows = _native.lib().yf_residual_norm_parts(t, d, gate_rows)
+    if rows < 1:
+        raise RuntimeError(f"yf_residual_norm_parts failed with code {rows}")
+    return rows
+
+
+def residual_norm_bwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, gate_rows: int,
+                      rstd: torch.Tensor, dh: torch.Tensor | None, dn: torch.Tensor | None, scale: float, dw: torch.Tensor, dpost: torch.Tensor | None,
+                      *, add_dw: bool = False, add_dpost: bool = False, dw_sumsq: torch.Tensor | None = None,
+                      dpost_sumsq: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``(dx, dy, dgate)``; ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the weights' gradients and
+    ``*_sumsq`` the squares of them."""
+    t, d = x.shape
+    dx, dy = torch.empty_like(x), torch.empty_like(x)
+    dgate = None if gate is None else torch.empty((gate_rows, d), device=x.device, dtype=x.dtype)
+    rows = _residual_norm_parts(t, d, gate_rows, x.device.index)
+    two = post is not None or (gate is not None and gate_rows != t)
+    parts = torch.empty((2 if two else 1) * rows * d, device=x.device, dtype=torch.float32)
+    kinds = [0 if o is None or o.dtype == x.dtype and not add else 2 if add else 1 for o, add in ((dw, add_dw), (dpost, add_dpost))]
+    assert all(o is None or (o.is_contiguous() and o.numel() == d and (kind == 0 or o.dtype == torch.float32)) for o, kind in zip((dw, dpost), kinds))
+    _check(_native.lib().yf_residual_norm_bwd(
+        x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, rstd.data_ptr(), _ptr(dh), _ptr(dn), dx.data_ptr(),
+        dy.data_ptr(), dw.data_ptr(), kinds[0], _ptr(dw_sumsq), _ptr(dpost), kinds[1], _ptr(dpost_sumsq), _ptr(dgate), parts.data_ptr(), parts.numel(),
+        t, d, scale, _DTYPES[x.dtype], _stream()), "yf_residual_norm_bwd")
+    global _launches
+    _launches += 1  # the parameters' sums
+    return dx, dy, dgate
