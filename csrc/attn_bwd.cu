@@ -521,7 +521,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 
 // delta[b,h,s] = sum_d dO * O, and the fp32 dQ accumulator of the same (token, head) cleared on the way (the main kernel
 // adds into it): sixteen lanes per (token, head), one 16-byte load of O and of dO and two 16-byte stores of zeros per lane.
-__global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
+// LO: O is the sum of two bf16 tensors (attn_mods.cuh).
+template <bool LO>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_lo, const __nv_bfloat16* __restrict__ d_o,
                                                          float* __restrict__ delta, float* __restrict__ dq_zero, int B, int S, int Hq,
                                                          long long o_stride, long long do_stride) {
   const long long total = (long long)B * S * Hq;
@@ -541,6 +543,11 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __
     const float2 a0 = unpack_bf16x2(a.x), a1 = unpack_bf16x2(a.y), a2 = unpack_bf16x2(a.z), a3 = unpack_bf16x2(a.w);
     const float2 g0 = unpack_bf16x2(g.x), g1 = unpack_bf16x2(g.y), g2 = unpack_bf16x2(g.z), g3 = unpack_bf16x2(g.w);
     float s = a0.x * g0.x + a0.y * g0.y + a1.x * g1.x + a1.y * g1.y + a2.x * g2.x + a2.y * g2.y + a3.x * g3.x + a3.y * g3.y;
+    if (LO) {
+      const uint4 l = *reinterpret_cast<const uint4*>(o_lo + t * o_stride + h * HD + sub * 8);
+      const float2 l0 = unpack_bf16x2(l.x), l1 = unpack_bf16x2(l.y), l2 = unpack_bf16x2(l.z), l3 = unpack_bf16x2(l.w);
+      s += l0.x * g0.x + l0.y * g0.y + l1.x * g1.x + l1.y * g1.y + l2.x * g2.x + l2.y * g2.y + l3.x * g3.x + l3.y * g3.y;
+    }
 #pragma unroll
     for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(half_mask, s, m);
     if (sub == 0) {
@@ -685,9 +692,9 @@ static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, 
     long long blocks = (groups * 16 + 255) / 256;
     const long long cap = (long long)yf_num_sms() * 8;
     if (blocks > cap) blocks = cap;
-    attn_delta_kernel<<<(int)blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(out),
-                                                  reinterpret_cast<const __nv_bfloat16*>(dout), delta, dq_accum, B, S, Hq,
-                                                  o_stride, do_stride);
+    const auto pre = mods.out_lo != nullptr ? attn_delta_kernel<true> : attn_delta_kernel<false>;
+    pre<<<(int)blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(out), mods.out_lo, reinterpret_cast<const __nv_bfloat16*>(dout), delta, dq_accum,
+                                     B, S, Hq, o_stride, do_stride);
   }
   BwdArgs a;
   a.lse = lse;
@@ -767,14 +774,17 @@ extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, co
   return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, rope, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
                       o_stride, do_stride, dq_stride, dkv_stride, scale, causal, 0, AttnMods{}, stream);
 }
-// Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal).
-extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta,
+// Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal); out_lo as the forward pass left it, or null.
+extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse, float* delta,
                                 float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S,
                                 int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
                                 long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding,
                                 void* stream) {
-  if (!(softcap >= 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7)) return -1;
-  const AttnMods m = attn_mods(scale, softcap, slopes, key_spans, padding);
+  if (!(softcap >= 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7) ||
+      (reinterpret_cast<uintptr_t>(out_lo) & 15))
+    return -1;
+  AttnMods m = attn_mods(scale, softcap, slopes, key_spans, padding);
+  m.out_lo = reinterpret_cast<__nv_bfloat16*>(const_cast<void*>(out_lo));
   const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
   return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, nullptr, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
                       o_stride, do_stride, dq_stride, dkv_stride, scale, 1, mods, m, stream);

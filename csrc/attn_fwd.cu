@@ -385,6 +385,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         uint4* dst = reinterpret_cast<uint4*>(args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD);
 #pragma unroll
         for (int v = 0; v < HD / 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
+        if (args.mods.out_lo != nullptr) {
+          uint4* lo = reinterpret_cast<uint4*>(args.mods.out_lo) + (dst - reinterpret_cast<uint4*>(args.out));
+#pragma unroll
+          for (int v = 0; v < HD / 8; ++v) lo[v] = make_uint4(0u, 0u, 0u, 0u);
+        }
         args.lse[((long long)b * args.Hq + h) * args.S + qrow] = -INFINITY;
       }
     } else
@@ -394,6 +399,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       const float l = l_run[0] + l_run[1];
       const float inv = (l > 0.f) ? 1.f / l : 0.f;
       __nv_bfloat16* dst = args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD;
+      __nv_bfloat16* dst_lo = MODS == 0 ? nullptr : args.mods.out_lo + (dst - args.out);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t r[32];
@@ -403,6 +409,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             uint4 w;
+            if (MODS != 0 && args.mods.out_lo != nullptr) {
+              uint32_t lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = __uint_as_float(r[8 * v + 2 * e]) * inv, y = __uint_as_float(r[8 * v + 2 * e + 1]) * inv;
+                const float2 hi = unpack_bf16x2(pack_bf16x2(x, y));
+                lo[e] = pack_bf16x2(x - hi.x, y - hi.y);
+              }
+              reinterpret_cast<uint4*>(dst_lo + c * 32)[v] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
             w.x = pack_bf16x2(__uint_as_float(r[8 * v + 0]) * inv, __uint_as_float(r[8 * v + 1]) * inv);
             w.y = pack_bf16x2(__uint_as_float(r[8 * v + 2]) * inv, __uint_as_float(r[8 * v + 3]) * inv);
             w.z = pack_bf16x2(__uint_as_float(r[8 * v + 4]) * inv, __uint_as_float(r[8 * v + 5]) * inv);
@@ -483,12 +499,16 @@ extern "C" int yf_attn_fwd(const void* q, const void* k, const void* v, void* ou
 }
 
 // The general form: scores capped at +-softcap (0: not) and less slopes[h] * distance (null: not), keys by `spans` and `padding` as
-// yf_document_mask gives them (both null: causal).  Rows without a key: zeros, lse -inf.
-extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq, int Hkv,
+// yf_document_mask gives them (both null: causal).  Rows without a key: zeros, lse -inf.  out_lo (may be null): what the rounding of `out`
+// left over, for the backward pass.
+extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int S, int Hq, int Hkv,
                                 long long q_stride, long long kv_stride, long long out_stride, float scale, float softcap, const float* slopes,
                                 const int* spans, const int* padding, void* stream) {
-  if (!(softcap >= 0.f) || (spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(spans) & 7) || B > 65535) return -1;
-  const AttnMods m = attn_mods(scale, softcap, slopes, spans, padding);
+  if (!(softcap >= 0.f) || (spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(spans) & 7) || B > 65535 ||
+      (reinterpret_cast<uintptr_t>(out_lo) & 15))
+    return -1;
+  AttnMods m = attn_mods(scale, softcap, slopes, spans, padding);
+  m.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
   const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
   return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, kv_stride, out_stride, scale, 1, mods, m, stream);
 }

@@ -263,11 +263,11 @@ def test_attention_shared_key_tiles(hq, hkv):
     q, k, v = (t.detach().reshape(b * s, -1) for t in _qkv(b, s, hq, hkv))
     slopes = torch.rand(hq, device=DEV)
     for cap, sl in ((0.0, None), (9.0, None), (0.0, slopes), (9.0, slopes)):
-        out, lse = kernels.attn_fwd_mods(q, k, v, b, s, hq, hkv, 0.1, cap, sl, m.spans, m.padding)
+        out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, b, s, hq, hkv, 0.1, cap, sl, m.spans, m.padding)
         dout, got = torch.randn_like(out), []
         for parts in [p for p in range(1, hq // hkv + 1) if (hq // hkv) % p == 0]:
             g = [torch.full(t.shape, math.nan, device=DEV, dtype=torch.bfloat16) for t in (q, k, v)]
-            kernels.attn_bwd_mods(q, k, v, out, dout, lse, *g, b, s, hq, hkv, 0.1, cap, sl, m.key_spans, m.padding, head_parts=parts)
+            kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *g, b, s, hq, hkv, 0.1, cap, sl, m.key_spans, m.padding, head_parts=parts)
             got.append(g)
         _done()
         for g in got[1:]:

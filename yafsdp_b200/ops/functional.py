@@ -591,31 +591,27 @@ class AttentionFn(torch.autograd.Function):
         q2, k2, v2 = _rows(q), _rows(k), _rows(v)
         if k2.stride(0) != v2.stride(0):
             k2, v2 = k2.contiguous(), v2.contiguous()
-        plain = mask is None and softcap == 0 and slopes is None
+        out_lo = None
         if q2.numel() == 0:
             out, lse = torch.empty_like(q2, memory_format=torch.contiguous_format), q2.new_empty((b, hq, s), dtype=torch.float32)
-        elif plain:
+        elif not keep and mask is None and softcap == 0 and slopes is None:
             out, lse = kernels.attn_fwd(q2, k2, v2, b, s, hq, hkv, scale)
         else:
             spans, padding = (None, None) if mask is None else (mask.spans, mask.padding)
-            out, lse = kernels.attn_fwd_mods(q2, k2, v2, b, s, hq, hkv, scale, softcap, slopes, spans, padding)
+            out, out_lo, lse = kernels.attn_fwd_mods(q2, k2, v2, b, s, hq, hkv, scale, softcap, slopes, spans, padding, keep)
         if keep:
-            ctx.save_for_backward(q2, k2, v2, out, lse, slopes, *((None, None) if mask is None else (mask.key_spans, mask.padding)))
-            ctx.args = (b, s, hq, hkv, scale, softcap, plain)
+            ctx.save_for_backward(q2, k2, v2, out, out_lo, lse, slopes, *((None, None) if mask is None else (mask.key_spans, mask.padding)))
+            ctx.args = (b, s, hq, hkv, scale, softcap)
         return out.view(q.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
-        q, k, v, out, lse, slopes, key_spans, padding = ctx.saved_tensors
-        b, s, hq, hkv, scale, softcap, plain = ctx.args
+        q, k, v, out, out_lo, lse, slopes, key_spans, padding = ctx.saved_tensors
+        b, s, hq, hkv, scale, softcap = ctx.args
         dq, dk, dv = torch.empty_like(out), *(torch.empty((b * s, hkv * 128), device=k.device, dtype=k.dtype) for _ in range(2))
         if out.numel() > 0:
-            g = _rows(dout)
-            if plain:
-                kernels.attn_bwd(q, k, v, out, g, lse, dq, dk, dv, b, s, hq, hkv, scale)
-            else:
-                kernels.attn_bwd_mods(q, k, v, out, g, lse, dq, dk, dv, b, s, hq, hkv, scale, softcap, slopes, key_spans, padding)
+            kernels.attn_bwd_mods(q, k, v, out, out_lo, _rows(dout), lse, dq, dk, dv, b, s, hq, hkv, scale, softcap, slopes, key_spans, padding)
         return dq.view(b, s, hq, 128), dk.view(b, s, hkv, 128), dv.view(b, s, hkv, 128), None, None, None, None, None
 
 
@@ -624,7 +620,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
     """Attention of ``q [B, S, Hq, D]`` over ``k``, ``v [B, S, Hkv, D]`` (query head ``h`` reads key head ``h // (Hq // Hkv)``), causal or under
     ``mask``; the result has the shape of ``q``, zeros where a token sees nothing.  The score of query ``i`` and key ``j`` is ``t = scale *
     q.k`` (``scale``: ``D ** -0.5``), ``softcap * tanh(t / softcap)`` with a ``softcap``, less ``slopes[h] * |i - j|`` with ``slopes [Hq]``
-    (constants: they get no gradient).  On CUDA: bf16, ``D`` = 128.  Tensors whose heads lie side by side in rows at a pitch of
+    (constants: they get no gradient).  On CUDA: bf16, ``D`` = 128; for the backward pass the output is kept in twice its bits.  Tensors whose heads lie side by side in rows at a pitch of
     16 bytes are read in place (parts of a fused projection), others are copied first.  What padding holds does not matter; any other
     value is taken to be finite: an infinity or NaN of one document may reach the documents that share a tile of 128 tokens with it."""
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
@@ -653,7 +649,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
             return attention(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes)
     if slopes is not None:
         slopes = _c(slopes.float())
-    return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes, torch.is_grad_enabled())  # type: ignore[no-any-return]
+    return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes, torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))  # type: ignore[no-any-return]
 
 
 def _attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,
@@ -776,7 +772,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)
-    return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps, torch.is_grad_enabled())  # type: ignore[no-any-return]
+    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, post_weight, gate))
+    return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps, keep)  # type: ignore[no-any-return]
 
 
 def _residual_norm_ref(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, scale: float,

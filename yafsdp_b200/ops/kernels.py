@@ -482,21 +482,24 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
 
 
 def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float,
-                  softcap: float, slopes: torch.Tensor | None, spans: torch.Tensor | None, padding: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
-    """:func:`attn_fwd` with scores capped by ``softcap * tanh(score / softcap)`` (0: not), less ``slopes[h] * distance`` (fp32 ``[Hq]``), under
-    the key ranges of :func:`document_mask` (``None``: causal)."""
+                  softcap: float, slopes: torch.Tensor | None, spans: torch.Tensor | None, padding: torch.Tensor | None,
+                  keep: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """``(out, out_lo, lse)``: :func:`attn_fwd` with scores capped by ``softcap * tanh(score / softcap)`` (0: not), less ``slopes[h] * distance`` (fp32 ``[Hq]``), under
+    the key ranges of :func:`document_mask` (``None``: causal).  ``out_lo`` (with ``keep``): what rounding ``out`` to bf16 left over, for the backward
+    pass."""
     t = batch * seq
     assert q.shape == (t, n_heads * 128) and k.shape == (t, n_kv_heads * 128) and v.shape == k.shape
     assert q.stride(1) == 1 and k.stride(1) == 1 and v.stride(1) == 1 and k.stride(0) == v.stride(0)
     out = torch.empty((t, n_heads * 128), device=q.device, dtype=torch.bfloat16)
     lse = torch.empty((batch, n_heads, seq), device=q.device, dtype=torch.float32)
-    _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, seq, n_heads, n_kv_heads,
+    out_lo = torch.empty_like(out) if keep else None
+    _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), lse.data_ptr(), batch, seq, n_heads, n_kv_heads,
                                           q.stride(0), k.stride(0), out.stride(0), scale, softcap, _ptr(slopes), _ptr(spans), _ptr(padding), _stream()),
            "yf_attn_fwd_mods")
-    return out, lse
+    return out, out_lo, lse
 
 
-def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor, lse: torch.Tensor, dq: torch.Tensor,
+def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, out_lo: torch.Tensor | None, dout: torch.Tensor, lse: torch.Tensor, dq: torch.Tensor,
                   dk: torch.Tensor, dv: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float, softcap: float,
                   slopes: torch.Tensor | None, key_spans: torch.Tensor | None, padding: torch.Tensor | None, head_parts: int = 0) -> None:
     """Backward of :func:`attn_fwd_mods` into the given views, as :func:`attn_bwd`."""
@@ -507,7 +510,7 @@ def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     parts = _attn_bwd_head_parts(batch, seq, n_heads, n_kv_heads, q.device.index) if head_parts == 0 else head_parts
     dkv_parts = torch.empty((parts, 2, batch, (seq + 127) // 128 * 128, n_kv_heads * 128), device=q.device, dtype=torch.float32) if parts > 1 else None
     global _launches
-    _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+    _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(),
                                           dq_acc.data_ptr(), _ptr(dkv_parts), 0 if dkv_parts is None else dkv_parts.numel(), parts, dq.data_ptr(),
                                           dk.data_ptr(), dv.data_ptr(), batch, seq, n_heads, n_kv_heads, q.stride(0), k.stride(0), out.stride(0),
                                           dout.stride(0), dq.stride(0), dk.stride(0), scale, softcap, _ptr(slopes), _ptr(key_spans), _ptr(padding),
