@@ -741,12 +741,12 @@ extern "C" int yf_attn_bwd_head_parts(int B, int S, int Hq, int Hkv) {
 }
 static int attn_bwd_any(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                                  float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, const float* rope, void* dq, void* dk, void* dv, int B,
-                                 int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
+                                 int S, int Hq, int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride,
                                  long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, int which, const AttnMods& mods, void* stream) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
   if (head_parts < 1 || (Hq / Hkv) % head_parts || (head_parts > 1) != (dkv_parts != nullptr)) return -1;
   if (dkv_parts != nullptr && dkv_floats < 4 * part_tile(head_parts, B, 0, (S + BKV - 1) / BKV, 0, Hkv, 0, 0)) return -1;
-  if ((q_stride % 8) || (kv_stride % 8) || (o_stride % 8) || (do_stride % 8) || (dq_stride % 8) || (dkv_stride % 8)) return -1;
+  if ((q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (o_stride % 8) || (do_stride % 8) || (dq_stride % 8) || (dkv_stride % 8)) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
        reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(dq_accum) |
@@ -754,8 +754,8 @@ static int attn_bwd_any(const void* q, const void* k, const void* v, const void*
     return -1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
-  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
-  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
   const CUtensorMap* md = yf_tensor_map_3d(dout, (uint64_t)Hq * HD, S, B, do_stride, (uint64_t)S * do_stride, 64, BQ, 1, 2, 1);
   const CUtensorMap* mdq = yf_tensor_map_3d(dq_accum, (uint64_t)Hq * HD, S, B, (uint64_t)Hq * HD, (uint64_t)S * Hq * HD, 32, BQ, 1, 4, 0);
   if (!mq || !mk || !mv || !md || !mdq) return -2;
@@ -772,13 +772,13 @@ extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, co
                                  int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
                                  long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, void* stream) {
   return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, rope, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
-                      o_stride, do_stride, dq_stride, dkv_stride, scale, causal, 0, AttnMods{}, stream);
+                      kv_stride, o_stride, do_stride, dq_stride, dkv_stride, scale, causal, 0, AttnMods{}, stream);
 }
 // Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal); out_lo as the forward pass left it, or null.
 extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse, float* delta,
                                 float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S,
-                                int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
-                                long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding,
+                                int Hq, int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride, long long do_stride,
+                                long long dq_stride, long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding,
                                 void* stream) {
   if (!(softcap >= 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7) ||
       (reinterpret_cast<uintptr_t>(out_lo) & 15))
@@ -786,8 +786,8 @@ extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, con
   AttnMods m = attn_mods(scale, softcap, slopes, key_spans, padding);
   m.out_lo = reinterpret_cast<__nv_bfloat16*>(const_cast<void*>(out_lo));
   const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
-  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, nullptr, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
-                      o_stride, do_stride, dq_stride, dkv_stride, scale, 1, mods, m, stream);
+  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, nullptr, dq, dk, dv, B, S, Hq, Hkv, q_stride, k_stride,
+                      v_stride, o_stride, do_stride, dq_stride, dkv_stride, scale, 1, mods, m, stream);
 }
 extern "C" int yf_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                            float* delta, float* dq_accum, void* dq, void* dk, void* dv, int B, int S, int Hq, int Hkv,

@@ -460,14 +460,14 @@ static int attn_fwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const C
 }
 
 static int attn_fwd_any(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq, int Hkv, long long q_stride,
-                        long long kv_stride, long long out_stride, float scale, int causal, int mods, const AttnMods& m, void* stream) {
-  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv) || (q_stride % 8) || (kv_stride % 8) || (out_stride % 8)) return -1;
+                        long long k_stride, long long v_stride, long long out_stride, float scale, int causal, int mods, const AttnMods& m, void* stream) {
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv) || (q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (out_stride % 8)) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out)) & 15)
     return -1;
   const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
-  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
-  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
   if (!mq || !mk || !mv) return -2;
   FwdArgs a;
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
@@ -495,14 +495,14 @@ static int attn_fwd_any(const void* q, const void* k, const void* v, void* out, 
 extern "C" int yf_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq,
                            int Hkv, long long q_stride, long long kv_stride, long long out_stride, float scale, int causal,
                            void* stream) {
-  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, kv_stride, out_stride, scale, causal, 0, AttnMods{}, stream);
+  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, kv_stride, kv_stride, out_stride, scale, causal, 0, AttnMods{}, stream);
 }
 
 // The general form: scores capped at +-softcap (0: not) and less slopes[h] * distance (null: not), keys by `spans` and `padding` as
 // yf_document_mask gives them (both null: causal).  Rows without a key: zeros, lse -inf.  out_lo (may be null): what the rounding of `out`
 // left over, for the backward pass.
 extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int S, int Hq, int Hkv,
-                                long long q_stride, long long kv_stride, long long out_stride, float scale, float softcap, const float* slopes,
+                                long long q_stride, long long k_stride, long long v_stride, long long out_stride, float scale, float softcap, const float* slopes,
                                 const int* spans, const int* padding, void* stream) {
   if (!(softcap >= 0.f) || (spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(spans) & 7) || B > 65535 ||
       (reinterpret_cast<uintptr_t>(out_lo) & 15))
@@ -510,5 +510,5 @@ extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, voi
   AttnMods m = attn_mods(scale, softcap, slopes, spans, padding);
   m.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
   const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
-  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, kv_stride, out_stride, scale, 1, mods, m, stream);
+  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, k_stride, v_stride, out_stride, scale, 1, mods, m, stream);
 }

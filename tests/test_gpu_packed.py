@@ -260,15 +260,13 @@ def test_attention_shared_key_tiles(hq, hkv):
     ids = _ids(b, s, 60, True)
     ids[0, 100:300] = -1
     m = Fn.document_mask(ids.to(DEV))
-    q, k, v = (t.detach().reshape(b * s, -1) for t in _qkv(b, s, hq, hkv))
+    q, k, v = (t.detach() for t in _qkv(b, s, hq, hkv))
     slopes = torch.rand(hq, device=DEV)
     for cap, sl in ((0.0, None), (9.0, None), (0.0, slopes), (9.0, slopes)):
-        out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, b, s, hq, hkv, 0.1, cap, sl, m.spans, m.padding)
+        out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, 0.1, cap, sl, m.spans, m.padding)
         dout, got = torch.randn_like(out), []
         for parts in [p for p in range(1, hq // hkv + 1) if (hq // hkv) % p == 0]:
-            g = [torch.full(t.shape, math.nan, device=DEV, dtype=torch.bfloat16) for t in (q, k, v)]
-            kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *g, b, s, hq, hkv, 0.1, cap, sl, m.key_spans, m.padding, head_parts=parts)
-            got.append(g)
+            got.append(kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, 0.1, cap, sl, m.key_spans, m.padding, head_parts=parts))
         _done()
         for g in got[1:]:
             for a, z in zip(g, got[0]):
@@ -411,10 +409,13 @@ def test_refusals():
         Fn.residual_norm(*[torch.ones(2, 16392, device=DEV)] * 2, torch.ones(16392, device=DEV))
     with pytest.raises(ValueError):
         Fn.residual_norm(torch.ones(2, 16, device=DEV), torch.ones(2, 16), torch.ones(16, device=DEV))
-    # the C entries refuse what the host can see: misaligned rows, a head group that does not divide, sizes of zero
+    # the C entries refuse what the host can see
     with pytest.raises(RuntimeError):
-        kernels.attn_fwd_mods(*(t.reshape(4, -1)[:, 4:] .contiguous().as_strided(t.reshape(4, -1).shape, (t.shape[2] * 128 - 4, 1)) for t in (q, k, v)), 1, 4, 2, 1, 0.1, 0.0,
-                              None, None, None)
+        kernels.attn_fwd_mods(q, k, v, 0.1, -1.0, None, None, None)
+    with pytest.raises(RuntimeError):
+        kernels.attn_fwd_mods(q, k, v, 0.1, 0.0, None, torch.zeros(1, 4, 2, device=DEV, dtype=torch.int32), None)
+    with pytest.raises(RuntimeError):
+        kernels.attn_fwd_mods(q, k.expand(1, 4, 3, 128), v.expand(1, 4, 3, 128), 0.1, 0.0, None, None, None)
     with pytest.raises(RuntimeError):
         kernels.residual_norm_fwd(torch.ones(3, 8, device=DEV), torch.ones(3, 8, device=DEV), torch.ones(8, device=DEV), None, torch.ones(2, 8, device=DEV), 2, 1.0, 1e-5)
 

@@ -403,14 +403,13 @@ def head_logits(h: torch.Tensor, w_norm: torch.Tensor, w_head: torch.Tensor, eps
 
 
 # ------------------------------------------------------------------------------------- packed documents
-def _elsewhere(t: torch.Tensor) -> bool:
-    return t.is_cuda and t.device.index != torch._C._cuda_getDevice()
-
-
-def _one_device(what: str, *ts: torch.Tensor | None) -> None:
-    devices = {t.device for t in ts if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{what}: tensors on different devices: {sorted(map(str, devices))}")
+def _device_of(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> bool:
+    """Whether the tensors, which must share a device, are on the current CUDA device (then kernels can be launched) or on the CPU."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and on {t.device}")
+    return dev.type != "cuda" or dev.index == torch._C._cuda_getDevice()
 
 
 @dataclass(frozen=True)
@@ -437,10 +436,10 @@ def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None
         raise ValueError(f"document_mask: window must be at least 0 and below 2^31, got {window}")
     if document_ids.shape[1] > 1 << 30:
         raise ValueError(f"document_mask: rows of at most 2^30 tokens, got {document_ids.shape[1]}")
-    _one_device("document_mask", document_ids, prefix)
+    here = _device_of("document_mask", document_ids, prefix)
     if not document_ids.is_cuda:
         return _document_mask_ref(document_ids, prefix, window)
-    if _elsewhere(document_ids):
+    if not here:
         with torch.cuda.device(document_ids.device):
             return document_mask(document_ids, prefix, window)
     ids, flags = (t if t is None or t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous() for t in (document_ids, prefix))
@@ -510,36 +509,19 @@ class RotaryAxes:
         return t
 
 
-def _tokens(t: torch.Tensor) -> torch.Tensor:
-    """``[B, S, H, D]`` as ``[B*S, H, D]`` that the kernels can read in place, or a copy that they can."""
-    t = t.detach().reshape(-1, t.shape[2], t.shape[3])
-    step = 16 // t.element_size()
-    good = (t.stride(2) == 1 and (t.shape[0] <= 1 or t.stride(0) % step == 0) and (t.shape[1] <= 1 or t.stride(1) % step == 0) and t.data_ptr() % 16 == 0)
-    if not good:
-        t = t.clone(memory_format=torch.contiguous_format)
-    if t.shape[0] > 1 and t.shape[1] > 1:
-        return t
-    # strides of axes that have one element may be anything
-    return t.as_strided(t.shape, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2], t.stride(1) if t.shape[1] > 1 else t.shape[2], 1))
-
-
 class RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor) -> Any:  # type: ignore[override]
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, table)
-        q2, k2 = kernels.rotary(_tokens(q), _tokens(k), positions, table)
-        assert q2 is not None and k2 is not None
-        return q2.view(q.shape), k2.view(k.shape)
+        return kernels.rotary(q, k, positions, table)
 
     @staticmethod
     @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dq: torch.Tensor | None, dk: torch.Tensor | None) -> Any:  # type: ignore[override]
-        positions, table = ctx.saved_tensors
         if dq is None and dk is None:
             return None, None, None, None
-        gq, gk = kernels.rotary(None if dq is None else _tokens(dq), None if dk is None else _tokens(dk), positions, table, backward=True)
-        return None if dq is None else gq.view(dq.shape), None if dk is None else gk.view(dk.shape), None, None
+        return *kernels.rotary(dq, dk, *ctx.saved_tensors, backward=True), None, None
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> tuple[torch.Tensor, torch.Tensor]:
@@ -552,16 +534,16 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: Rota
     n, tokens = len(axes.sections), q.shape[:2]
     if positions.dtype not in (torch.int32, torch.int64) or (positions.shape != (n, *tokens) and not (n == 1 and positions.shape == tokens)):
         raise ValueError(f"rotary: positions must be int32 or int64 {[n, *tokens]}, got {list(positions.shape)} {positions.dtype}")
-    _one_device("rotary", q, k, positions)
+    here = _device_of("rotary", q, k, positions)
     if not q.is_cuda:
         return _rotary_ref(q, positions, axes), _rotary_ref(k, positions, axes)
-    if _elsewhere(q):
+    if not here:
         with torch.cuda.device(q.device):
             return rotary(q, k, positions, axes)
-    pos = positions.reshape(n, -1)
-    if pos.shape[1] > 1 and pos.stride(1) != 1:
-        pos = pos.contiguous()
-    return RotaryFn.apply(q, k, pos, axes.table(q.device))  # type: ignore[no-any-return]
+    positions, table = positions.contiguous(), axes.table(q.device)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return RotaryFn.apply(q, k, positions, table)  # type: ignore[no-any-return]
+    return kernels.rotary(q, k, positions, table)  # type: ignore[return-value]
 
 
 def _rotary_ref(t: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
@@ -573,46 +555,21 @@ def _rotary_ref(t: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> t
 
 
 # ------------------------------------------------------------------------------------- attention with masks, capped scores and a distance bias
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``[B, S, H, 128]`` as ``[B*S, H*128]`` rows that the kernels can read in place, or a copy that they can."""
-    width = t.shape[2] * t.shape[3]
-    r = t.detach().reshape(t.shape[0] * t.shape[1], width)
-    if r.data_ptr() % 16 or r.stride(1) != 1 or (r.shape[0] > 1 and (r.stride(0) % 8 or r.stride(0) < width)):
-        r = r.clone(memory_format=torch.contiguous_format)
-    return r if r.shape[0] > 1 else r.as_strided(r.shape, (width, 1))  # the stride of an axis with one element may be anything
-
-
 class AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,  # type: ignore[override]
-                slopes: torch.Tensor | None, keep: bool) -> torch.Tensor:
-        b, s, hq, _ = q.shape
-        hkv = k.shape[2]
-        q2, k2, v2 = _rows(q), _rows(k), _rows(v)
-        if k2.stride(0) != v2.stride(0):
-            k2, v2 = k2.contiguous(), v2.contiguous()
-        out_lo = None
-        if q2.numel() == 0:
-            out, lse = torch.empty_like(q2, memory_format=torch.contiguous_format), q2.new_empty((b, hq, s), dtype=torch.float32)
-        elif not keep and mask is None and softcap == 0 and slopes is None:
-            out, lse = kernels.attn_fwd(q2, k2, v2, b, s, hq, hkv, scale)
-        else:
-            spans, padding = (None, None) if mask is None else (mask.spans, mask.padding)
-            out, out_lo, lse = kernels.attn_fwd_mods(q2, k2, v2, b, s, hq, hkv, scale, softcap, slopes, spans, padding, keep)
-        if keep:
-            ctx.save_for_backward(q2, k2, v2, out, out_lo, lse, slopes, *((None, None) if mask is None else (mask.key_spans, mask.padding)))
-            ctx.args = (b, s, hq, hkv, scale, softcap)
-        return out.view(q.shape)
+                slopes: torch.Tensor | None) -> torch.Tensor:
+        spans, key_spans, padding = (None, None, None) if mask is None else (mask.spans, mask.key_spans, mask.padding)
+        out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, scale, softcap, slopes, spans, padding)
+        ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes, key_spans, padding)
+        ctx.args = (scale, softcap)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
         q, k, v, out, out_lo, lse, slopes, key_spans, padding = ctx.saved_tensors
-        b, s, hq, hkv, scale, softcap = ctx.args
-        dq, dk, dv = torch.empty_like(out), *(torch.empty((b * s, hkv * 128), device=k.device, dtype=k.dtype) for _ in range(2))
-        if out.numel() > 0:
-            kernels.attn_bwd_mods(q, k, v, out, out_lo, _rows(dout), lse, dq, dk, dv, b, s, hq, hkv, scale, softcap, slopes, key_spans, padding)
-        return dq.view(b, s, hq, 128), dk.view(b, s, hkv, 128), dv.view(b, s, hkv, 128), None, None, None, None, None
+        return *kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *ctx.args, slopes, key_spans, padding), None, None, None, None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None = None, *, scale: float | None = None, softcap: float = 0.0,
@@ -639,17 +596,20 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
         raise ValueError(f"attention: slopes must have one value for each of {q.shape[2]} query heads, got {list(slopes.shape)}")
     if slopes is not None and slopes.requires_grad:
         raise ValueError("attention: slopes get no gradient; pass slopes.detach()")
-    _one_device("attention", q, k, v, slopes, None if mask is None else mask.spans)
+    here = _device_of("attention", q, k, v, slopes, None if mask is None else mask.spans)
     if not q.is_cuda:
         return _attention_ref(q, k, v, mask, scale, softcap, slopes)
     if q.dtype != torch.bfloat16 or q.shape[3] != 128:
         raise TypeError(f"attention: the CUDA kernels take bf16 heads of 128, got {q.dtype} heads of {q.shape[3]}")
-    if _elsewhere(q):
+    if not here:
         with torch.cuda.device(q.device):
             return attention(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes)
     if slopes is not None:
         slopes = _c(slopes.float())
-    return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes, torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))  # type: ignore[no-any-return]
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes)  # type: ignore[no-any-return]
+    spans, padding = (None, None) if mask is None else (mask.spans, mask.padding)
+    return kernels.attn_fwd_mods(q, k, v, scale, softcap, slopes, spans, padding, keep=False)[0]
 
 
 def _attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,
@@ -675,21 +635,14 @@ def _attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Docu
 class ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None,  # type: ignore[override]
-                gate_rows: int, scale: float, eps: float, keep: bool) -> Any:
+                gate_rows: int, scale: float, eps: float) -> Any:
         ctx.set_materialize_grads(False)
-        d = x.shape[-1]
-        x2, y2, w = _aligned(x).view(-1, d), _aligned(y).view(-1, d), _aligned(weight)
-        p, g = None if post is None else _aligned(post), None if gate is None else _aligned(gate)
-        if x2.shape[0] > 0:
-            h, n, rstd = kernels.residual_norm_fwd(x2, y2, w, p, g, gate_rows, scale, eps, keep)
-        else:
-            h, n, rstd = torch.empty_like(x2), torch.empty_like(x2), None
-        if keep:
-            # the inputs themselves, as torch's own layers do: the values of a sharded parameter are gathered anew for the backward pass
-            ctx.save_for_backward(x, y, weight, post, gate, rstd)
-            ctx.params = (weight, post)  # as parameters of a group they know where their gradients go
-            ctx.args = (gate_rows, scale)
-        return h.view(x.shape), n.view(x.shape)
+        h, n, rstd = kernels.residual_norm_fwd(x, y, weight, post, gate, gate_rows, scale, eps)
+        # the inputs themselves, as torch's own layers do: the values of a sharded parameter are gathered anew for the backward pass
+        ctx.save_for_backward(x, y, weight, post, gate, rstd)
+        ctx.params = (weight, post)  # as parameters of a group they know where their gradients go
+        ctx.args = (gate_rows, scale)
+        return h, n
 
     @staticmethod
     @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
@@ -697,25 +650,22 @@ class ResidualNormFn(torch.autograd.Function):
         x, y, w, p, g, rstd = ctx.saved_tensors
         gate_rows, scale = ctx.args
         if x.numel() == 0:
-            return *(None if t is None else torch.zeros_like(t) for t in (x, y, w, p, g)), None, None, None, None
-        shape, gate_shape = x.shape, None if g is None else g.shape
-        x, y, w, p, g = (None if t is None else _aligned(t) for t in (x, y, w, p, g))
-        x, y = x.view(-1, shape[-1]), y.view(-1, shape[-1])
-        outs = [None if t is None else _ParamGrad(t, x.dtype) for t in ctx.params]
-        a, b = outs[0], outs[1]
-        assert a is not None
-        dx, dy, dgate = kernels.residual_norm_bwd(
-            x, y, w, p, g, gate_rows, rstd, *(None if t is None else _aligned(t).view(x.shape) for t in (dh, dn)), scale, a.out, None if b is None else b.out,
-            add_dw=a.add, add_dpost=b is not None and b.add, dw_sumsq=a.sumsq, dpost_sumsq=None if b is None else b.sumsq)
-        return (dx.view(shape), dy.view(shape), a.result(), None if b is None else b.result(), None if dgate is None else dgate.view(gate_shape),
-                None, None, None, None)
+            return *(None if t is None else torch.zeros_like(t) for t in (x, y, w, p, g)), None, None, None
+        a = _ParamGrad(ctx.params[0])
+        b = None if p is None else _ParamGrad(ctx.params[1])
+        if b is None:
+            dx, dy, dgate = kernels.residual_norm_bwd(x, y, w, None, g, gate_rows, rstd, dh, dn, scale, a.out, None, add_dw=a.add, dw_sumsq=a.sumsq)
+        else:
+            dx, dy, dgate = kernels.residual_norm_bwd(x, y, w, p, g, gate_rows, rstd, dh, dn, scale, a.out, b.out, add_dw=a.add, add_dpost=b.add,
+                                                      dw_sumsq=a.sumsq, dpost_sumsq=b.sumsq)
+        return dx, dy, a.result(), None if b is None else b.result(), dgate, None, None, None
 
 
 class _ParamGrad:
     """Where a kernel that finishes a whole norm weight gradient in one go writes it: the parameter's fp32 sink when it has one, else a tensor of
     the parameter's type."""
 
-    def __init__(self, p: torch.Tensor, dtype: torch.dtype):
+    def __init__(self, p: torch.Tensor):
         self.sink, self.add, self.sumsq = _sink(p), False, None
         self.pushed = self.sink is not None and self.sink.pushes()
         self.sunk = self.sink is not None and not self.pushed and self.sink.local_ok
@@ -723,17 +673,12 @@ class _ParamGrad:
             self.out, self.add = self.sink.begin()
             self.sumsq = self.sink.norm_target(self.add)
         else:
-            self.out = torch.empty(p.shape, device=p.device, dtype=torch.float32 if self.pushed else dtype)
+            self.out = torch.empty(p.shape, device=p.device, dtype=torch.float32 if self.pushed else p.dtype)
 
     def result(self) -> torch.Tensor | None:
         if self.pushed:
             self.sink.push_from(self.out)
         return None if self.pushed or self.sunk else self.out
-
-
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    t = _c(t.detach())
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
@@ -764,16 +709,17 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     if not math.isfinite(scale) or not 0.0 < eps < math.inf:
         raise ValueError(f"residual_norm: scale must be finite and eps positive, got {scale} and {eps}")
     rows = 0 if gate is None else _gate_rows(gate, x)
-    _one_device("residual_norm", x, y, weight, post_weight, gate)
+    here = _device_of("residual_norm", x, y, weight, post_weight, gate)
     if not x.is_cuda:
         return _residual_norm_ref(x, y, weight, post_weight, gate, scale, eps)
     if x.shape[-1] % 8 or not 0 < x.shape[-1] <= 16384:
         raise ValueError(f"residual_norm: the CUDA kernels take widths that are multiples of 8 up to 16384, got {x.shape[-1]}")
-    if _elsewhere(x):
+    if not here:
         with torch.cuda.device(x.device):
             return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, post_weight, gate))
-    return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps, keep)  # type: ignore[no-any-return]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, post_weight, gate)):
+        return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps)  # type: ignore[no-any-return]
+    return kernels.residual_norm_fwd(x, y, weight, post_weight, gate, rows, scale, eps, keep=False)[:2]
 
 
 def _residual_norm_ref(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, scale: float,

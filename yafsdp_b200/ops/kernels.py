@@ -481,41 +481,59 @@ def attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tenso
     _launches += 2  # delta pre-pass and dq conversion post-pass
 
 
-def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float,
-                  softcap: float, slopes: torch.Tensor | None, spans: torch.Tensor | None, padding: torch.Tensor | None,
-                  keep: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
-    """``(out, out_lo, lse)``: :func:`attn_fwd` with scores capped by ``softcap * tanh(score / softcap)`` (0: not), less ``slopes[h] * distance`` (fp32 ``[Hq]``), under
-    the key ranges of :func:`document_mask` (``None``: causal).  ``out_lo`` (with ``keep``): what rounding ``out`` to bf16 left over, for the backward
-    pass."""
-    t = batch * seq
-    assert q.shape == (t, n_heads * 128) and k.shape == (t, n_kv_heads * 128) and v.shape == k.shape
-    assert q.stride(1) == 1 and k.stride(1) == 1 and v.stride(1) == 1 and k.stride(0) == v.stride(0)
-    out = torch.empty((t, n_heads * 128), device=q.device, dtype=torch.bfloat16)
-    lse = torch.empty((batch, n_heads, seq), device=q.device, dtype=torch.float32)
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [B, S, H, D]`` and the elements between its tokens, heads side by side and tokens at one pitch of a multiple of 16 bytes; a copy where
+    it is laid out otherwise.  (Host time counts here: no views are made.)"""
+    b, s, h, d = t.shape
+    sb, ss, sh, sd = t.stride()
+    row = ss if s > 1 else sb if b > 1 else h * d  # the stride of an axis with one element may be anything
+    if (sd == 1 and (h == 1 or sh == d) and (s == 1 or b == 1 or sb == s * ss) and row >= h * d and row * t.element_size() % 16 == 0
+            and t.data_ptr() % 16 == 0):
+        return t, row
+    return t.clone(memory_format=torch.contiguous_format), h * d
+
+
+def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, softcap: float, slopes: torch.Tensor | None,
+                  spans: torch.Tensor | None, padding: torch.Tensor | None, keep: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """``(out, out_lo, lse)``: flash attention forward of ``q [B,S,Hq,128]`` over ``k``, ``v [B,S,Hkv,128]`` (read in place where :func:`_rows` can)
+    with scores capped by ``softcap * tanh(score / softcap)`` (0: not), less ``slopes[h] * distance`` (fp32 ``[Hq]``), under the key
+    ranges of :func:`document_mask` (``None``: causal).  ``out_lo`` (with ``keep``): what rounding ``out`` to bf16 left over, for the
+    backward pass."""
+    b, s, hq, _ = q.shape
+    hkv = k.shape[2]
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    out = torch.empty((b, s, hq, 128), device=q.device, dtype=torch.bfloat16)
     out_lo = torch.empty_like(out) if keep else None
-    _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), lse.data_ptr(), batch, seq, n_heads, n_kv_heads,
-                                          q.stride(0), k.stride(0), out.stride(0), scale, softcap, _ptr(slopes), _ptr(spans), _ptr(padding), _stream()),
-           "yf_attn_fwd_mods")
+    lse = torch.empty((b, hq, s), device=q.device, dtype=torch.float32)
+    if b * s > 0:
+        _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), lse.data_ptr(), b, s, hq, hkv,
+                                              qs, ks, vs, hq * 128, scale, softcap, _ptr(slopes), _ptr(spans), _ptr(padding), _stream()), "yf_attn_fwd_mods")
     return out, out_lo, lse
 
 
-def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, out_lo: torch.Tensor | None, dout: torch.Tensor, lse: torch.Tensor, dq: torch.Tensor,
-                  dk: torch.Tensor, dv: torch.Tensor, batch: int, seq: int, n_heads: int, n_kv_heads: int, scale: float, softcap: float,
-                  slopes: torch.Tensor | None, key_spans: torch.Tensor | None, padding: torch.Tensor | None, head_parts: int = 0) -> None:
-    """Backward of :func:`attn_fwd_mods` into the given views, as :func:`attn_bwd`."""
-    assert dout.stride(1) == 1 and out.stride(1) == 1 and dq.stride(1) == 1 and dk.stride(1) == 1 and dv.stride(1) == 1
-    assert dk.stride(0) == dv.stride(0)
-    delta = torch.empty((batch, n_heads, seq), device=q.device, dtype=torch.float32)
-    dq_acc = torch.empty((batch * seq, n_heads * 128), device=q.device, dtype=torch.float32)
-    parts = _attn_bwd_head_parts(batch, seq, n_heads, n_kv_heads, q.device.index) if head_parts == 0 else head_parts
-    dkv_parts = torch.empty((parts, 2, batch, (seq + 127) // 128 * 128, n_kv_heads * 128), device=q.device, dtype=torch.float32) if parts > 1 else None
+def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, out_lo: torch.Tensor | None, dout: torch.Tensor,
+                  lse: torch.Tensor, scale: float, softcap: float, slopes: torch.Tensor | None, key_spans: torch.Tensor | None,
+                  padding: torch.Tensor | None, head_parts: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(dq, dk, dv)`` of :func:`attn_fwd_mods`, whose results ``out``, ``out_lo`` and ``lse`` are.  ``head_parts``: as in :func:`attn_bwd`."""
+    b, s, hq, _ = q.shape
+    hkv, dev = k.shape[2], q.device
+    dq, dk, dv = (torch.empty((b, s, h, 128), device=dev, dtype=torch.bfloat16) for h in (hq, hkv, hkv))
+    if b * s == 0:
+        return dq, dk, dv
+    (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q), _rows(k), _rows(v), _rows(dout)
+    parts = _attn_bwd_head_parts(b, s, hq, hkv, dev.index) if head_parts == 0 else head_parts
+    # scratch: the dQ accumulator, the parts' dK and dV, and D
+    n_dq, n_delta = b * s * hq * 128, b * hq * s
+    n_parts = parts * 2 * b * ((s + 127) // 128 * 128) * hkv * 128 if parts > 1 else 0
+    ws = torch.empty(n_dq + n_parts + n_delta, device=dev, dtype=torch.float32)
+    at = ws.data_ptr()
     global _launches
-    _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                                          dq_acc.data_ptr(), _ptr(dkv_parts), 0 if dkv_parts is None else dkv_parts.numel(), parts, dq.data_ptr(),
-                                          dk.data_ptr(), dv.data_ptr(), batch, seq, n_heads, n_kv_heads, q.stride(0), k.stride(0), out.stride(0),
-                                          dout.stride(0), dq.stride(0), dk.stride(0), scale, softcap, _ptr(slopes), _ptr(key_spans), _ptr(padding),
-                                          _stream()), "yf_attn_bwd_mods")
+    _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), dout.data_ptr(), lse.data_ptr(),
+                                          at + 4 * (n_dq + n_parts), at, at + 4 * n_dq if n_parts else None, n_parts, parts, dq.data_ptr(), dk.data_ptr(),
+                                          dv.data_ptr(), b, s, hq, hkv, qs, ks, vs, hq * 128, gs, hq * 128, hkv * 128, scale, softcap, _ptr(slopes),
+                                          _ptr(key_spans), _ptr(padding), _stream()), "yf_attn_bwd_mods")
     _launches += 2  # delta pre-pass and dq conversion post-pass
+    return dq, dk, dv
 
 
 # --------------------------------------------------------------------------------------- packed batches
@@ -528,45 +546,69 @@ def document_mask(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -
     b, s = ids.shape
     assert ids.dtype in (torch.int32, torch.int64) and (prefix is None or prefix.dtype == torch.bool)
     assert all(t is None or s < 2 or t.stride(1) == 1 for t in (ids, prefix))
-    spans = torch.empty((2, b, s, 2), device=ids.device, dtype=torch.int32)
-    positions = torch.empty((b, s), device=ids.device, dtype=torch.int32)
-    padding = torch.empty((b, (s + 127) // 128), device=ids.device, dtype=torch.int32)
+    dev = ids.device
+    spans, key_spans = torch.empty((2, b, s, 2), device=dev, dtype=torch.int32).unbind(0)
+    positions = torch.empty((b, s), device=dev, dtype=torch.int32)
+    padding = torch.empty((b, (s + 127) // 128), device=dev, dtype=torch.int32)
     if b * s > 0:
-        _check(_native.lib().yf_document_mask(ids.data_ptr(), int(ids.dtype == torch.int64), _ptr(prefix), spans.data_ptr(),
-                                              spans.data_ptr() + 8 * b * s, positions.data_ptr(), padding.data_ptr(), b, s, ids.stride(0),
-                                              0 if prefix is None else prefix.stride(0), window, _stream()), "yf_document_mask")
-    return spans[0], spans[1], positions, padding
+        _check(_native.lib().yf_document_mask(ids.data_ptr(), int(ids.dtype == torch.int64), _ptr(prefix), spans.data_ptr(), key_spans.data_ptr(),
+                                              positions.data_ptr(), padding.data_ptr(), b, s, ids.stride(0), 0 if prefix is None else prefix.stride(0),
+                                              window, _stream()), "yf_document_mask")
+    return spans, key_spans, positions, padding
+
+
+def _tokens(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``t [B, S, H, D]`` and the elements between its tokens and between its heads, both multiples of 16 bytes; a copy where it is laid out
+    otherwise."""
+    b, s, h, d = t.shape
+    sb, ss, sh, sd = t.stride()
+    token = ss if s > 1 else sb if b > 1 else h * d
+    head = sh if h > 1 else d
+    if sd == 1 and (s == 1 or b == 1 or sb == s * ss) and (token | head) * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        return t, token, head
+    return t.clone(memory_format=torch.contiguous_format), h * d, d
 
 
 def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
            backward: bool = False) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    """``q [T,Hq,D]`` and ``k [T,Hk,D]`` (either may be ``None``) turned by ``positions [axes,T]``; ``table [D/2,2]`` int64: a pair's frequency
-    (2^64 a whole turn) and its axis.  ``backward``: turned back.  Heads and tokens may lie apart by multiples of 16 bytes."""
+    """``q [B,S,Hq,D]`` and ``k [B,S,Hk,D]`` (either may be ``None``) turned by ``positions`` (``[axes,B,S]`` without gaps); ``table [D/2,2]`` int64: a
+    pair's frequency (2^64 a whole turn) and its axis.  ``backward``: turned back.  Read in place where :func:`_tokens` can."""
     some = q if q is not None else k
-    assert some is not None and positions.dtype in (torch.int32, torch.int64) and table.dtype == torch.int64
-    (t, _, d), dev, dtype = some.shape, some.device, some.dtype
-    assert positions.shape[1] == t and (t < 2 or positions.stride(1) == 1)
-    assert all(x is None or (x.shape[0] == t and x.shape[2] == d and x.stride(2) == 1 and x.dtype == dtype) for x in (q, k))
-    outs = [None if x is None else torch.empty(x.shape, device=dev, dtype=dtype) for x in (q, k)]
-    heads = [0 if x is None else x.shape[1] for x in (q, k)]
-    if t * sum(heads) > 0:
-        strides = [0 if x is None else x.stride(i) for x in (q, k) for i in (0, 1)]
-        _check(_native.lib().yf_rotary(_ptr(q), _ptr(k), _ptr(outs[0]), _ptr(outs[1]), positions.data_ptr(), int(positions.dtype == torch.int64),
-                                       positions.stride(0), table.data_ptr(), t, heads[0], heads[1], d, *strides, heads[0] * d, heads[1] * d,
-                                       _DTYPES[dtype], -1 if backward else 1, _stream()), "yf_rotary")
-    return outs[0], outs[1]
+    assert some is not None and positions.is_contiguous() and table.is_contiguous() and table.dtype == torch.int64
+    b, s, _, d = some.shape
+    t, dtype = b * s, some.dtype
+    q_out, k_out = (None if x is None else torch.empty(x.shape, device=x.device, dtype=dtype) for x in (q, k))
+    q, q_token, q_head = (None, 0, 0) if q is None else _tokens(q)
+    k, k_token, k_head = (None, 0, 0) if k is None else _tokens(k)
+    hq, hk = 0 if q is None else q.shape[2], 0 if k is None else k.shape[2]
+    if t * (hq + hk) > 0:
+        _check(_native.lib().yf_rotary(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), positions.data_ptr(), int(positions.dtype == torch.int64), t,
+                                       table.data_ptr(), t, hq, hk, d, q_token, q_head, k_token, k_head, hq * d, hk * d, _DTYPES[dtype],
+                                       -1 if backward else 1, _stream()), "yf_rotary")
+    return q_out, k_out
 
 
 # --------------------------------------------------------------------------------------- the residual step between two blocks
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """``t`` without gaps from a 16-byte boundary on; a copy where it is laid out otherwise."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def residual_norm_fwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, post: torch.Tensor | None, gate: torch.Tensor | None, gate_rows: int,
                       scale: float, eps: float, keep: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """``h = x + scale * gate * norm(y) * post``, ``n = norm(h) * weight`` of ``[T,D]`` tensors of one type, and the norms' factors ``[T,2]`` (with
-    ``keep``).  ``gate``: ``gate_rows`` rows of ``D``, each for as many tokens in a row."""
-    t, d = x.shape
+    """``h = x + scale * gate * norm(y) * post``, ``n = norm(h) * weight`` of ``[..., D]`` tensors of one type, and the norms' factors ``[T, 2]``
+    (with ``keep``).  ``gate``: ``gate_rows`` rows of ``D``, each for as many tokens in a row."""
+    d = x.shape[-1]
+    t = x.numel() // d
+    x, y, weight = _flat(x), _flat(y), _flat(weight)
+    post, gate = None if post is None else _flat(post), None if gate is None else _flat(gate)
     h, n = torch.empty_like(x), torch.empty_like(x)
     rstd = torch.empty((t, 2), device=x.device, dtype=torch.float32) if keep else None
-    _check(_native.lib().yf_residual_norm_fwd(x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, h.data_ptr(), n.data_ptr(),
-                                              _ptr(rstd), t, d, scale, eps, _DTYPES[x.dtype], _stream()), "yf_residual_norm_fwd")
+    if t > 0:
+        _check(_native.lib().yf_residual_norm_fwd(x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, h.data_ptr(),
+                                                  n.data_ptr(), _ptr(rstd), t, d, scale, eps, _DTYPES[x.dtype], _stream()), "yf_residual_norm_fwd")
     return h, n, rstd
 
 
@@ -582,20 +624,24 @@ def residual_norm_bwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, po
                       rstd: torch.Tensor, dh: torch.Tensor | None, dn: torch.Tensor | None, scale: float, dw: torch.Tensor, dpost: torch.Tensor | None,
                       *, add_dw: bool = False, add_dpost: bool = False, dw_sumsq: torch.Tensor | None = None,
                       dpost_sumsq: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """``(dx, dy, dgate)``; ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the weights' gradients and
-    ``*_sumsq`` the squares of them."""
-    t, d = x.shape
+    """``(dx, dy, dgate)`` for at least one token; ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the
+    weights' gradients and ``*_sumsq`` the squares of them."""
+    d = x.shape[-1]
+    t = x.numel() // d
+    x, y, weight = _flat(x), _flat(y), _flat(weight)
+    post, gate, dh, dn = (None if o is None else _flat(o) for o in (post, gate, dh, dn))
     dx, dy = torch.empty_like(x), torch.empty_like(x)
-    dgate = None if gate is None else torch.empty((gate_rows, d), device=x.device, dtype=x.dtype)
+    dgate = None if gate is None else torch.empty_like(gate)
     rows = _residual_norm_parts(t, d, gate_rows, x.device.index)
     two = post is not None or (gate is not None and gate_rows != t)
-    parts = torch.empty((2 if two else 1) * rows * d, device=x.device, dtype=torch.float32)
+    floats = (2 if two else 1) * rows * d
+    parts = torch.empty(floats, device=x.device, dtype=torch.float32)
     kinds = [0 if o is None or o.dtype == x.dtype and not add else 2 if add else 1 for o, add in ((dw, add_dw), (dpost, add_dpost))]
     assert all(o is None or (o.is_contiguous() and o.numel() == d and (kind == 0 or o.dtype == torch.float32)) for o, kind in zip((dw, dpost), kinds))
     _check(_native.lib().yf_residual_norm_bwd(
         x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, rstd.data_ptr(), _ptr(dh), _ptr(dn), dx.data_ptr(),
-        dy.data_ptr(), dw.data_ptr(), kinds[0], _ptr(dw_sumsq), _ptr(dpost), kinds[1], _ptr(dpost_sumsq), _ptr(dgate), parts.data_ptr(), parts.numel(),
-        t, d, scale, _DTYPES[x.dtype], _stream()), "yf_residual_norm_bwd")
+        dy.data_ptr(), dw.data_ptr(), kinds[0], _ptr(dw_sumsq), _ptr(dpost), kinds[1], _ptr(dpost_sumsq), _ptr(dgate), parts.data_ptr(), floats, t, d,
+        scale, _DTYPES[x.dtype], _stream()), "yf_residual_norm_bwd")
     global _launches
     _launches += 1  # the parameters' sums
     return dx, dy, dgate
