@@ -4,11 +4,11 @@
 // tile where the whole problem then still fits the GPU at once).  Roles:
 //   warp 0      TMA producer: Q once, then K/V tiles of 128 keys through a 2-stage ring
 //   warp 1      MMA issuer:   S_i = Q_i K^T and O_i += P_i V for the tiles i = 0, 1
-//   warps 2-5   softmax of tile 0, warps 6-9 of tile 1: one thread per query row (TMEM lane == row)
+//   warps 2-9   softmax of tile 0, warps 10-17 of tile 1: two threads per query row (TMEM lane == row), one for each half of the keys
 // While one tile's softmax runs, the tensor cores work for the other one.  TMEM (512 columns): S_0, S_1, O_0, O_1, 128
-// columns of fp32 each; P_i (bf16, 64 columns) takes the place of S_i, whose row its thread has read into registers, and is
-// the MMA's A operand from there, so the probabilities never go through shared memory.  A row belongs to one thread: the
-// softmax threads exchange nothing but one bit per block, at a barrier of the tile's four warps (below).
+// columns of fp32 each; P_i (bf16, 64 columns) takes the place of S_i, whose row its threads have read into registers, and is
+// the MMA's A operand from there, so the probabilities never go through shared memory.  The softmax threads exchange one bit per block, at
+// a barrier of the tile's eight warps, and a row's maximum where that bit says that it moves (below).
 // The output accumulates in TMEM over all key blocks (O += P V).  The exponent's reference maximum is only moved when
 // some row of a tile has grown by more than 2^8 since it was set (then its warps rescale their rows of O in TMEM and their
 // sums); otherwise P is taken relative to the older maximum (values up to 2^8, harmless in bf16 / fp32), and the final
@@ -33,8 +33,8 @@ constexpr int BQ = 128;        // query rows per tile
 constexpr int BKV = 128;       // keys per tile
 constexpr int ATOM = 16384;    // bytes of one [128 rows x 64 bf16] swizzled block
 constexpr int TILE = 2 * ATOM; // one 128x128 bf16 tile
-constexpr int FWD_THREADS = 320;  // producer warp, MMA warp, eight softmax warps
-constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 256;
+constexpr int FWD_THREADS = 576;  // producer warp, MMA warp, sixteen softmax warps
+constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
 
 struct FwdArgs {
   __nv_bfloat16* out;
@@ -56,7 +56,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                   // tile i at + i * TILE
   uint8_t* sKV = sQ + 2 * TILE;         // stage s: K at sKV + s*2*TILE, V at + TILE
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * TILE);
+  float* sRow = reinterpret_cast<float*>(sKV + 4 * TILE);  // [tile][half of the keys][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 2 * BQ);
   uint64_t* q_full = bars;              // [2] per tile
   uint64_t* k_full = bars + 2;          // [2] per stage
   uint64_t* v_full = bars + 4;          // [2]
@@ -111,7 +112,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], 4);  // one arrival per softmax warp of the tile
+      mbar_init(&p_ready[s], 8);  // one arrival per softmax warp of the tile
       mbar_init(&o_full[s], 1);
       dead[s] = 0;
     }
@@ -262,14 +263,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       }
     }
   } else {
-    const int i = (warp - 2) >> 2;           // tile
+    const int i = (warp - 2) >> 3;           // tile
+    const int half = ((warp - 2) >> 2) & 1;  // of a block's keys, of the columns of O
     const int n = i == 0 ? n_kv0 : n_kv1, first = i == 0 ? first0 : first1;
     const int q = warp & 3;                  // a warp may only touch TMEM lanes [32*(warp%4), +32)
     const int qrow = q0 + i * BQ + q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t tS = tmem_base + lane_off + i * 128, tO = tmem_base + lane_off + 256 + i * 128;
+    const uint32_t tS = tmem_base + lane_off + i * 128, tO = tmem_base + lane_off + 256 + i * 128 + half * 64;
+    float* mine = sRow + (i * 2 + half) * BQ + q * 32 + lane;
+    float* theirs = sRow + (i * 2 + (half ^ 1)) * BQ + q * 32 + lane;
     float m_run = -INFINITY;                 // reference maximum of the exponent
-    float l_run[2] = {0.f, 0.f};             // row sums of the even and the odd 64 keys of all blocks, each in the order of the keys
+    float l_run = 0.f;                       // sum of the row over this half of all blocks, in the order of the keys
     const float sl2 = args.scale_log2;
     constexpr float RESCALE_LOG2 = 8.f;      // move the reference maximum when a row's maximum exceeds it by 2^8
     // keys allowed for this row: col <= limit
@@ -281,15 +285,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const float to_log2 = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
     bool alive = true;
     for (int j = first; j < n; ++j) {
-      // a bounded wait that runs out ends the work of the tile's four warps: they meet at the barrier below, so the one that gives up
+      // a bounded wait that runs out ends the work of the tile's eight warps: they meet at the barrier below, so the one that gives up
       // says so there (the lanes of a warp decide together: TMEM accesses are warp-wide)
       alive = alive && __all_sync(0xffffffffu, mbar_wait(&s_full[i], (j - first) & 1, 120 + i));
-      const int kv0 = j * BKV;
-      uint32_t sc[4][32];
+      const int kv0 = j * BKV + half * 64;
+      uint32_t sc[2][32];
       if (alive) {
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sc[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld32(tS + half * 64 + c * 32, sc[c]);
         tmem_ld_wait();
       } else {
         dead[i] = j + 1;
@@ -297,7 +301,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (MODS & (MOD_CAP | MOD_BIAS)) {
         const float far = (float)(kv0 - qrow);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           if (MODS & MOD_CAP) cap_scores(sc[c], args.mods);
           if (MODS & MOD_BIAS) {
 #pragma unroll
@@ -309,18 +313,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         }
       }
       if (MODS != 0) {
-        if (kv0 < span.x || kv0 + BKV > span.y) {  // the ends of a row's range
+        if (kv0 < span.x || kv0 + 64 > span.y) {  // the ends of a row's range
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             const uint32_t seen = bit_range(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
 #pragma unroll
             for (int t = 0; t < 32; ++t)
               if (!((seen >> t) & 1u)) sc[c][t] = 0xff800000u;  // -inf
           }
         }
-      } else if (kv0 + BKV - 1 > limit) {  // only the blocks on the diagonal and the last one have masked keys
+      } else if (kv0 + 63 > limit) {  // only the blocks on the diagonal and the last one have masked keys
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int t = 0; t < 32; ++t)
             if (kv0 + c * 32 + t > limit) sc[c][t] = 0xff800000u;  // -inf
@@ -328,53 +332,55 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       float mx4[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx4[c] = __uint_as_float(sc[c][0]);
+        mx4[c] = __uint_as_float(sc[c >> 1][(c & 1) * 16]);
 #pragma unroll
-        for (int t = 1; t < 32; ++t) mx4[c] = fmaxf(mx4[c], __uint_as_float(sc[c][t]));
+        for (int t = 1; t < 16; ++t) mx4[c] = fmaxf(mx4[c], __uint_as_float(sc[c >> 1][(c & 1) * 16 + t]));
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       const bool grew = !alive || j == first || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * to_log2 > RESCALE_LOG2));
-      // The four warps of a tile move their rows' maxima together: a row's bits then depend on its tile alone and repeat those of
-      // kernels that deal the rows to warps in another way.  The barrier costs 4 % at 2048 tokens x 32 heads (49 -> 51 us) and 8 % at
-      // 8192 x 32/8 (570 -> 615 us), less than 0.2 % of a layer's forward and backward.
-      if (i == 0 ? named_bar_or(1, 128, grew) : named_bar_or(2, 128, grew)) {
+      // The warps of a tile move their rows' maxima together: a row's bits then depend on its tile alone and repeat those of
+      // kernels that deal the rows to warps in another way.  Behind this barrier both threads of a row have read their halves of S, so P may
+      // take its place.
+      if (i == 0 ? named_bar_or(1, 256, grew) : named_bar_or(2, 256, grew)) {
         if (dead[i] == j + 1) { alive = false; break; }  // not a later block's: who gives up there waits for this warp there
-        const float m_new = fmaxf(m_run, mx);
+        *mine = mx;
+        if (i == 0) named_bar_sync(3, 256);
+        else named_bar_sync(4, 256);
+        const float m_new = fmaxf(m_run, fmaxf(mx, *theirs));
         if (j > first) {
-          // O holds sums relative to the old maximum: wait for the last P V to land, then scale this warp's rows
+          // O holds sums relative to the old maximum: wait for the last P V to land, then scale this warp's part of the rows
           alive = __all_sync(0xffffffffu, mbar_wait(&o_full[i], (j - 1 - first) & 1, 122 + i));
           if (!alive) continue;  // to the next barrier, where the others learn of it
           tc_fence_after();
           const float alpha = (m_run == -INFINITY) ? 0.f : fast_exp2((m_run - m_new) * to_log2);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t r[32];
-            tmem_ld32(tO + c * 32, r);
+            uint32_t r[16];
+            tmem_ld16(tO + c * 16, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int t = 0; t < 32; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
-            tmem_st32(tO + c * 32, r);
+            for (int t = 0; t < 16; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
+            tmem_st16(tO + c * 16, r);
           }
-          l_run[0] *= alpha;
-          l_run[1] *= alpha;
+          l_run *= alpha;
         }
         m_run = m_new;
       }
       const float neg_ms = (m_run == -INFINITY) ? 0.f : -m_run * to_log2;
+      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {  // 64 keys: 32 TMEM columns of packed bf16 pairs
-        uint32_t packed[32];
-        float sum = 0.f;
+      for (int c = 0; c < 2; ++c) {  // 32 keys: 16 TMEM columns of packed bf16 pairs
+        uint32_t packed[16];
 #pragma unroll
-        for (int t = 0; t < 32; ++t) {
-          const float p0 = fast_exp2(fmaf(__uint_as_float(sc[2 * c + (t >> 4)][(2 * t) & 31]), to_log2, neg_ms));
-          const float p1 = fast_exp2(fmaf(__uint_as_float(sc[2 * c + (t >> 4)][(2 * t + 1) & 31]), to_log2, neg_ms));
+        for (int t = 0; t < 16; ++t) {
+          const float p0 = fast_exp2(fmaf(__uint_as_float(sc[c][2 * t]), to_log2, neg_ms));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(sc[c][2 * t + 1]), to_log2, neg_ms));
           sum += p0 + p1;  // one chain: an addition takes less than the two exponentials next to it
           packed[t] = pack_bf16x2(p0, p1);
         }
-        tmem_st32(tS + c * 32, packed);
-        l_run[c] += sum;
+        tmem_st16(tS + half * 32 + c * 16, packed);
       }
+      l_run += sum;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -382,26 +388,30 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     }
     if (MODS != 0 && n == first) {  // nothing but padding: zeros
       if (qrow < args.S && (i == 0 || args.tiles == 2)) {
-        uint4* dst = reinterpret_cast<uint4*>(args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD);
+        uint4* dst = reinterpret_cast<uint4*>(args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64);
 #pragma unroll
-        for (int v = 0; v < HD / 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
+        for (int v = 0; v < 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
         if (args.mods.out_lo != nullptr) {
           uint4* lo = reinterpret_cast<uint4*>(args.mods.out_lo) + (dst - reinterpret_cast<uint4*>(args.out));
 #pragma unroll
-          for (int v = 0; v < HD / 8; ++v) lo[v] = make_uint4(0u, 0u, 0u, 0u);
+          for (int v = 0; v < 8; ++v) lo[v] = make_uint4(0u, 0u, 0u, 0u);
         }
-        args.lse[((long long)b * args.Hq + h) * args.S + qrow] = -INFINITY;
+        if (half == 0) args.lse[((long long)b * args.Hq + h) * args.S + qrow] = -INFINITY;
       }
-    } else
-    // the output of the last block
-    if (n > 0 && alive && __all_sync(0xffffffffu, mbar_wait(&o_full[i], (n - 1 - first) & 1, 124 + i))) {
+    } else if (n > first) {
+      // the output of the last block, and the sum over both halves of the keys
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_full[i], (n - 1 - first) & 1, 124 + i));
+      *mine = l_run;
+      if (i == 0 ? named_bar_or(1, 256, !alive) : named_bar_or(2, 256, !alive)) alive = false;
+    }
+    if (n > first && alive) {
       tc_fence_after();
-      const float l = l_run[0] + l_run[1];
+      const float l = half == 0 ? l_run + *theirs : *theirs + l_run;
       const float inv = (l > 0.f) ? 1.f / l : 0.f;
-      __nv_bfloat16* dst = args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD;
+      __nv_bfloat16* dst = args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64;
       __nv_bfloat16* dst_lo = MODS == 0 ? nullptr : args.mods.out_lo + (dst - args.out);
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t r[32];
         tmem_ld32(tO + c * 32, r);
         tmem_ld_wait();
@@ -427,7 +437,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           }
         }
       }
-      if (qrow < args.S)
+      if (half == 0 && qrow < args.S)
         args.lse[((long long)b * args.Hq + h) * args.S + qrow] = (l > 0.f) ? (m_run * ((MODS & (MOD_CAP | MOD_BIAS)) ? 0.6931471805599453f : args.scale) + logf(l)) : -INFINITY;
     }
     tc_fence_before();
