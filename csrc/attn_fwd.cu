@@ -4,11 +4,11 @@
 // tile where the whole problem then still fits the GPU at once).  Roles:
 //   warp 0      TMA producer: Q once, then K/V tiles of 128 keys through a 2-stage ring
 //   warp 1      MMA issuer:   S_i = Q_i K^T and O_i += P_i V for the tiles i = 0, 1
-//   warps 2-9   softmax of tile 0, warps 10-17 of tile 1: two threads per query row (TMEM lane == row), one for each half of the keys
+//   warps 2-5   softmax of tile 0, warps 6-9 of tile 1: one thread per query row (TMEM lane == row)
 // While one tile's softmax runs, the tensor cores work for the other one.  TMEM (512 columns): S_0, S_1, O_0, O_1, 128
-// columns of fp32 each; P_i (bf16, 64 columns) takes the place of S_i, whose row its threads have read into registers, and is
-// the MMA's A operand from there, so the probabilities never go through shared memory.  The softmax threads exchange one bit per block, at
-// a barrier of the tile's eight warps, and a row's maximum where that bit says that it moves (below).
+// columns of fp32 each; P_i (bf16, 64 columns) takes the place of S_i, whose row its thread has read into registers, and is
+// the MMA's A operand from there, so the probabilities never go through shared memory.  A row belongs to one thread: the
+// softmax threads exchange nothing but one bit per block, at a barrier of the tile's four warps (below).
 // The output accumulates in TMEM over all key blocks (O += P V).  The exponent's reference maximum is only moved when
 // some row of a tile has grown by more than 2^8 since it was set (then its warps rescale their rows of O in TMEM and their
 // sums); otherwise P is taken relative to the older maximum (values up to 2^8, harmless in bf16 / fp32), and the final
@@ -17,10 +17,6 @@
 // different pipes.
 // Inputs are read in place from the fused QKV projection output ([tokens, (Hq+2Hkv)*128], row pitch
 // given), so no head transposes are materialised.  Writes O (bf16) and the log-sum-exp per row (fp32).
-//
-// Instantiations beyond plain causal attention (attn_mods.cuh) cap the scores, subtract a distance bias, and take every query's range of
-// keys from memory; a tile then walks over the key blocks between its first row's first key and its last row's last one.
-#include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
 
@@ -33,8 +29,8 @@ constexpr int BQ = 128;        // query rows per tile
 constexpr int BKV = 128;       // keys per tile
 constexpr int ATOM = 16384;    // bytes of one [128 rows x 64 bf16] swizzled block
 constexpr int TILE = 2 * ATOM; // one 128x128 bf16 tile
-constexpr int FWD_THREADS = 576;  // producer warp, MMA warp, sixteen softmax warps
-constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
+constexpr int FWD_THREADS = 320;  // producer warp, MMA warp, eight softmax warps
+constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 256;
 
 struct FwdArgs {
   __nv_bfloat16* out;
@@ -45,10 +41,8 @@ struct FwdArgs {
   float scale;
   int causal;
   int tiles;             // query tiles per CTA: two, or one where even so every CTA finds an SM of its own
-  AttnMods mods;
 };
 
-template <int MODS>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                 const __grid_constant__ CUtensorMap tma_v, FwdArgs args) {
@@ -56,8 +50,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;                   // tile i at + i * TILE
   uint8_t* sKV = sQ + 2 * TILE;         // stage s: K at sKV + s*2*TILE, V at + TILE
-  float* sRow = reinterpret_cast<float*>(sKV + 4 * TILE);  // [tile][half of the keys][row]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 2 * BQ);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + 4 * TILE);
   uint64_t* q_full = bars;              // [2] per tile
   uint64_t* k_full = bars + 2;          // [2] per stage
   uint64_t* v_full = bars + 4;          // [2]
@@ -66,8 +59,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   uint64_t* s_full = bars + 10;         // [2] per tile
   uint64_t* p_ready = bars + 12;        // [2] per tile
   uint64_t* o_full = bars + 14;         // [2] per tile
-  uint64_t* v_land = bars + 16;         // a V tile with padded rows has landed, to be cleared before it counts as full
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [2] per tile: 1 + the block at which one of its warps has given up
 
   const int warp = threadIdx.x >> 5;
@@ -79,26 +71,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   const int hkv = h / (args.Hq / args.Hkv);
   const int q0 = qt * args.tiles * BQ;
   const int n_kv_total = (args.S + BKV - 1) / BKV;
-  // key blocks [first, end) of the two tiles (the second one has none when the sequence ends in the first, or a CTA has one tile)
-  int first0 = 0, first1 = 0;
-  int n_kv0 = args.causal ? min(q0 / BKV + 1, n_kv_total) : n_kv_total;
-  int n_kv1 = args.tiles < 2 || q0 + BQ >= args.S ? 0 : (args.causal ? min(q0 / BKV + 2, n_kv_total) : n_kv_total);
-  const int2* spans = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
-  const int* padding = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * n_kv_total;
-  if (MODS != 0 && spans != nullptr) {
-    auto blocks = [&](int row0, int& first, int& end) {
-      const int rows = min(BQ, args.S - row0);
-      if (__ldg(padding + row0 / BQ) >= rows) { first = end = 0; return; }
-      first = max(__ldg(spans + row0).x, 0) / BKV;
-      end = min((__ldg(spans + row0 + rows - 1).y + BKV - 1) / BKV, n_kv_total);
-    };
-    blocks(q0, first0, n_kv0);
-    if (n_kv1 > 0) blocks(q0 + BQ, first1, n_kv1);
-    if (first0 >= n_kv0) first0 = n_kv0 = 0;
-    if (first1 >= n_kv1) first1 = n_kv1 = 0;
-  }
-  const bool has0 = MODS == 0 || n_kv0 > 0;  // tile 0 may hold nothing but padding
-  const int j_first = MODS == 0 ? 0 : has0 ? (n_kv1 > 0 ? min(first0, first1) : first0) : first1;
+  // key blocks of the two tiles (the second one has none when the sequence ends in the first, or a CTA has one tile)
+  const int n_kv0 = args.causal ? min(q0 / BKV + 1, n_kv_total) : n_kv_total;
+  const int n_kv1 = args.tiles < 2 || q0 + BQ >= args.S ? 0 : (args.causal ? min(q0 / BKV + 2, n_kv_total) : n_kv_total);
   const int n_kv = max(n_kv0, n_kv1);
 
   if (threadIdx.x == 0) {
@@ -112,11 +87,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       mbar_init(&k_empty[s], 1);
       mbar_init(&v_empty[s], 1);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_ready[s], 8);  // one arrival per softmax warp of the tile
+      mbar_init(&p_ready[s], 4);  // one arrival per softmax warp of the tile
       mbar_init(&o_full[s], 1);
       dead[s] = 0;
     }
-    if (MODS != 0) mbar_init(v_land, 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -128,52 +102,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (MODS != 0 && warp == 0) {
-    // the whole warp, since it clears the padded rows of the V tiles that have some
-    if (lane == 0 && has0) {
-      mbar_expect_tx(&q_full[0], TILE);
-      tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
-      tma_load_3d(sQ + ATOM, &tma_q, &q_full[0], h * HD + 64, q0, b);
-    }
-    int dead_rows = padding != nullptr && j_first < n_kv ? __ldg(padding + j_first) : 0, landed = 0;
-    for (int j = j_first; j < n_kv; ++j) {
-      const int s = (j - j_first) & 1, ph = (((j - j_first) >> 1) & 1) ^ 1;
-      uint8_t* sK = sKV + s * 2 * TILE;
-      uint8_t* sV = sK + TILE;
-      const bool clear = dead_rows > 0;
-      if (padding != nullptr && j + 1 < n_kv) dead_rows = __ldg(padding + j + 1);
-      bool ok = true;
-      if (lane == 0) {
-        ok = mbar_wait(&k_empty[s], ph, 100);
-        if (ok) {
-          mbar_expect_tx(&k_full[s], TILE);
-          tma_load_3d(sK, &tma_k, &k_full[s], hkv * HD, j * BKV, b);
-          tma_load_3d(sK + ATOM, &tma_k, &k_full[s], hkv * HD + 64, j * BKV, b);
-          if (j == j_first && n_kv1 > 0) {
-            mbar_expect_tx(&q_full[1], TILE);
-            tma_load_3d(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ, b);
-            tma_load_3d(sQ + TILE + ATOM, &tma_q, &q_full[1], h * HD + 64, q0 + BQ, b);
-          }
-          ok = mbar_wait(&v_empty[s], ph, 101);
-        }
-        if (ok) {
-          uint64_t* bar = clear ? v_land : &v_full[s];
-          mbar_expect_tx(bar, TILE);
-          tma_load_3d(sV, &tma_v, bar, hkv * HD, j * BKV, b);
-          tma_load_3d(sV + ATOM, &tma_v, bar, hkv * HD + 64, j * BKV, b);
-        }
-      }
-      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
-      if (clear) {
-        if (!__all_sync(0xffffffffu, mbar_wait(v_land, landed & 1, 102))) break;
-        ++landed;
-        zero_padded_rows(sV, ATOM, BKV, j * BKV, args.S, spans);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[s]);
-      }
-    }
-  } else if (MODS == 0 && warp == 0) {
+  if (warp == 0) {
     if (elect_one()) {
       mbar_expect_tx(&q_full[0], TILE);
       tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
@@ -206,7 +135,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       const uint64_t dV = umma_smem_desc_sw128(smem_u32(sKV) + TILE, ATOM, 1024);
       // descriptor addresses advance in units of 16 bytes
       auto issue_s = [&](int i, int j) {
-        const uint64_t q = dQ + i * (TILE >> 4), k = dK + ((j - j_first) & 1) * (2 * TILE >> 4);
+        const uint64_t q = dQ + i * (TILE >> 4), k = dK + (j & 1) * (2 * TILE >> 4);
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) {
           const uint32_t off = ((e >> 2) * ATOM + (e & 3) * 32) >> 4;
@@ -215,45 +144,37 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tc_commit(&s_full[i]);
       };
       auto issue_o = [&](int i, int j) {
-        const uint64_t v = dV + ((j - j_first) & 1) * (2 * TILE >> 4);
-        const int first = i == 0 ? first0 : first1;
+        const uint64_t v = dV + (j & 1) * (2 * TILE >> 4);
 #pragma unroll
         for (int e = 0; e < BKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
-          tc_mma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + e * 8, v + e * (2048 >> 4), idesc_o, ((j - first) | e) != 0);
+          tc_mma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + e * 8, v + e * (2048 >> 4), idesc_o, (j | e) != 0);
         tc_commit(&o_full[i]);
       };
-      bool alive = (MODS == 0 || n_kv > 0) && mbar_wait(&k_full[0], 0, 110) && (!has0 || mbar_wait(&q_full[0], 0, 111));
+      bool alive = mbar_wait(&k_full[0], 0, 110) && mbar_wait(&q_full[0], 0, 111);
       if (alive) {
         tc_fence_after();
-        if (has0 && first0 == j_first) issue_s(0, j_first);
+        issue_s(0, 0);
         if (n_kv1 > 0 && (alive = mbar_wait(&q_full[1], 0, 112))) {
           tc_fence_after();
-          if (first1 == j_first) issue_s(1, j_first);
+          issue_s(1, 0);
         }
         tc_commit(&k_empty[0]);
       }
-      for (int j = j_first; j < n_kv && alive; ++j) {
-        const int s = (j - j_first) & 1;
-        if (j + 1 < n_kv && !mbar_wait(&k_full[s ^ 1], ((j + 1 - j_first) >> 1) & 1, 113)) break;
-        if (!mbar_wait(&v_full[s], ((j - j_first) >> 1) & 1, 114)) break;
+      for (int j = 0; j < n_kv && alive; ++j) {
+        const int s = j & 1;
+        if (j + 1 < n_kv && !mbar_wait(&k_full[s ^ 1], ((j + 1) >> 1) & 1, 113)) break;
+        if (!mbar_wait(&v_full[s], (j >> 1) & 1, 114)) break;
         // P_i(j) V, then S_i(j+1) into the columns that P_i(j) held: the order of MMAs with different accumulators is not
         // promised, so the product is waited for (about 200 cycles; the other tile's softmax is running meanwhile)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int n = i == 0 ? n_kv0 : n_kv1, first = i == 0 ? first0 : first1;
+          const int n = i == 0 ? n_kv0 : n_kv1;
           if (j >= n) continue;
-          if (MODS != 0 && j < first) {  // the tile's range starts later: its first product, when the block before it is through
-            if (j + 1 == first) {
-              tc_fence_after();
-              issue_s(i, first);
-            }
-            continue;
-          }
-          if (!mbar_wait(&p_ready[i], (j - first) & 1, 115 + i)) { alive = false; break; }
+          if (!mbar_wait(&p_ready[i], j & 1, 115 + i)) { alive = false; break; }
           tc_fence_after();
           issue_o(i, j);
           if (j + 1 < n) {
-            if (!mbar_wait(&o_full[i], (j - first) & 1, 117 + i)) { alive = false; break; }
+            if (!mbar_wait(&o_full[i], j & 1, 117 + i)) { alive = false; break; }
             tc_fence_after();
             issue_s(i, j + 1);
           }
@@ -263,68 +184,36 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       }
     }
   } else {
-    const int i = (warp - 2) >> 3;           // tile
-    const int half = ((warp - 2) >> 2) & 1;  // of a block's keys, of the columns of O
-    const int n = i == 0 ? n_kv0 : n_kv1, first = i == 0 ? first0 : first1;
+    const int i = (warp - 2) >> 2;           // tile
+    const int n = i == 0 ? n_kv0 : n_kv1;
     const int q = warp & 3;                  // a warp may only touch TMEM lanes [32*(warp%4), +32)
     const int qrow = q0 + i * BQ + q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t tS = tmem_base + lane_off + i * 128, tO = tmem_base + lane_off + 256 + i * 128 + half * 64;
-    float* mine = sRow + (i * 2 + half) * BQ + q * 32 + lane;
-    float* theirs = sRow + (i * 2 + (half ^ 1)) * BQ + q * 32 + lane;
+    const uint32_t tS = tmem_base + lane_off + i * 128, tO = tmem_base + lane_off + 256 + i * 128;
     float m_run = -INFINITY;                 // reference maximum of the exponent
-    float l_run = 0.f;                       // sum of the row over this half of all blocks, in the order of the keys
+    float l_run[2] = {0.f, 0.f};             // row sums of the even and the odd 64 keys of all blocks, each in the order of the keys
     const float sl2 = args.scale_log2;
     constexpr float RESCALE_LOG2 = 8.f;      // move the reference maximum when a row's maximum exceeds it by 2^8
     // keys allowed for this row: col <= limit
     const int limit = args.causal ? min(qrow, args.S - 1) : (args.S - 1);
-    int2 span = make_int2(0, qrow + 1);      // keys [x, y) with MODS
-    if (MODS != 0 && (spans != nullptr || qrow >= args.S)) span = qrow < args.S ? __ldg(spans + qrow) : make_int2(0, 0);
-    const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[h] * 1.4426950408889634f : 0.f;
-    // scores that were transformed are in units of log2 already
-    const float to_log2 = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
     bool alive = true;
-    for (int j = first; j < n; ++j) {
-      // a bounded wait that runs out ends the work of the tile's eight warps: they meet at the barrier below, so the one that gives up
+    for (int j = 0; j < n; ++j) {
+      // a bounded wait that runs out ends the work of the tile's four warps: they meet at the barrier below, so the one that gives up
       // says so there (the lanes of a warp decide together: TMEM accesses are warp-wide)
-      alive = alive && __all_sync(0xffffffffu, mbar_wait(&s_full[i], (j - first) & 1, 120 + i));
-      const int kv0 = j * BKV + half * 64;
-      uint32_t sc[2][32];
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, 120 + i));
+      const int kv0 = j * BKV;
+      uint32_t sc[4][32];
       if (alive) {
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld32(tS + half * 64 + c * 32, sc[c]);
+        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sc[c]);
         tmem_ld_wait();
       } else {
         dead[i] = j + 1;
       }
-      if (MODS & (MOD_CAP | MOD_BIAS)) {
-        const float far = (float)(kv0 - qrow);
+      if (kv0 + BKV - 1 > limit) {  // only the blocks on the diagonal and the last one have masked keys
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (MODS & MOD_CAP) cap_scores(sc[c], args.mods);
-          if (MODS & MOD_BIAS) {
-#pragma unroll
-            for (int t = 0; t < 32; ++t) {
-              const float x = __uint_as_float(sc[c][t]);
-              sc[c][t] = __float_as_uint(fmaf(-slope, fabsf(far + (float)(c * 32 + t)), (MODS & MOD_CAP) ? x : x * sl2));
-            }
-          }
-        }
-      }
-      if (MODS != 0) {
-        if (kv0 < span.x || kv0 + 64 > span.y) {  // the ends of a row's range
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t seen = bit_range(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
-#pragma unroll
-            for (int t = 0; t < 32; ++t)
-              if (!((seen >> t) & 1u)) sc[c][t] = 0xff800000u;  // -inf
-          }
-        }
-      } else if (kv0 + 63 > limit) {  // only the blocks on the diagonal and the last one have masked keys
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int t = 0; t < 32; ++t)
             if (kv0 + c * 32 + t > limit) sc[c][t] = 0xff800000u;  // -inf
@@ -332,86 +221,66 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       float mx4[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx4[c] = __uint_as_float(sc[c >> 1][(c & 1) * 16]);
+        mx4[c] = __uint_as_float(sc[c][0]);
 #pragma unroll
-        for (int t = 1; t < 16; ++t) mx4[c] = fmaxf(mx4[c], __uint_as_float(sc[c >> 1][(c & 1) * 16 + t]));
+        for (int t = 1; t < 32; ++t) mx4[c] = fmaxf(mx4[c], __uint_as_float(sc[c][t]));
       }
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      const bool grew = !alive || j == first || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * to_log2 > RESCALE_LOG2));
-      // The warps of a tile move their rows' maxima together: a row's bits then depend on its tile alone and repeat those of
-      // kernels that deal the rows to warps in another way.  Behind this barrier both threads of a row have read their halves of S, so P may
-      // take its place.
-      if (i == 0 ? named_bar_or(1, 256, grew) : named_bar_or(2, 256, grew)) {
+      const bool grew = !alive || j == 0 || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * sl2 > RESCALE_LOG2));
+      // The four warps of a tile move their rows' maxima together: a row's bits then depend on its tile alone and repeat those of
+      // kernels that deal the rows to warps in another way.  The barrier costs 4 % at 2048 tokens x 32 heads (49 -> 51 us) and 8 % at
+      // 8192 x 32/8 (570 -> 615 us), less than 0.2 % of a layer's forward and backward.
+      if (i == 0 ? named_bar_or(1, 128, grew) : named_bar_or(2, 128, grew)) {
         if (dead[i] == j + 1) { alive = false; break; }  // not a later block's: who gives up there waits for this warp there
-        *mine = mx;
-        if (i == 0) named_bar_sync(3, 256);
-        else named_bar_sync(4, 256);
-        const float m_new = fmaxf(m_run, fmaxf(mx, *theirs));
-        if (j > first) {
-          // O holds sums relative to the old maximum: wait for the last P V to land, then scale this warp's part of the rows
-          alive = __all_sync(0xffffffffu, mbar_wait(&o_full[i], (j - 1 - first) & 1, 122 + i));
+        const float m_new = fmaxf(m_run, mx);
+        if (j > 0) {
+          // O holds sums relative to the old maximum: wait for the last P V to land, then scale this warp's rows
+          alive = __all_sync(0xffffffffu, mbar_wait(&o_full[i], (j - 1) & 1, 122 + i));
           if (!alive) continue;  // to the next barrier, where the others learn of it
           tc_fence_after();
-          const float alpha = (m_run == -INFINITY) ? 0.f : fast_exp2((m_run - m_new) * to_log2);
+          const float alpha = (m_run == -INFINITY) ? 0.f : fast_exp2((m_run - m_new) * sl2);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
-            uint32_t r[16];
-            tmem_ld16(tO + c * 16, r);
+            uint32_t r[32];
+            tmem_ld32(tO + c * 32, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int t = 0; t < 16; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
-            tmem_st16(tO + c * 16, r);
+            for (int t = 0; t < 32; ++t) r[t] = __float_as_uint(__uint_as_float(r[t]) * alpha);
+            tmem_st32(tO + c * 32, r);
           }
-          l_run *= alpha;
+          l_run[0] *= alpha;
+          l_run[1] *= alpha;
         }
         m_run = m_new;
       }
-      const float neg_ms = (m_run == -INFINITY) ? 0.f : -m_run * to_log2;
-      float sum = 0.f;
+      const float neg_ms = (m_run == -INFINITY) ? 0.f : -m_run * sl2;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {  // 32 keys: 16 TMEM columns of packed bf16 pairs
-        uint32_t packed[16];
+      for (int c = 0; c < 2; ++c) {  // 64 keys: 32 TMEM columns of packed bf16 pairs
+        uint32_t packed[32];
+        float sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-          const float p0 = fast_exp2(fmaf(__uint_as_float(sc[c][2 * t]), to_log2, neg_ms));
-          const float p1 = fast_exp2(fmaf(__uint_as_float(sc[c][2 * t + 1]), to_log2, neg_ms));
+        for (int t = 0; t < 32; ++t) {
+          const float p0 = fast_exp2(fmaf(__uint_as_float(sc[2 * c + (t >> 4)][(2 * t) & 31]), sl2, neg_ms));
+          const float p1 = fast_exp2(fmaf(__uint_as_float(sc[2 * c + (t >> 4)][(2 * t + 1) & 31]), sl2, neg_ms));
           sum += p0 + p1;  // one chain: an addition takes less than the two exponentials next to it
           packed[t] = pack_bf16x2(p0, p1);
         }
-        tmem_st16(tS + half * 32 + c * 16, packed);
+        tmem_st32(tS + c * 32, packed);
+        l_run[c] += sum;
       }
-      l_run += sum;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_ready[i]);
     }
-    if (MODS != 0 && n == first) {  // nothing but padding: zeros
-      if (qrow < args.S && (i == 0 || args.tiles == 2)) {
-        uint4* dst = reinterpret_cast<uint4*>(args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64);
-#pragma unroll
-        for (int v = 0; v < 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
-        if (args.mods.out_lo != nullptr) {
-          uint4* lo = reinterpret_cast<uint4*>(args.mods.out_lo) + (dst - reinterpret_cast<uint4*>(args.out));
-#pragma unroll
-          for (int v = 0; v < 8; ++v) lo[v] = make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (half == 0) args.lse[((long long)b * args.Hq + h) * args.S + qrow] = -INFINITY;
-      }
-    } else if (n > first) {
-      // the output of the last block, and the sum over both halves of the keys
-      alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_full[i], (n - 1 - first) & 1, 124 + i));
-      *mine = l_run;
-      if (i == 0 ? named_bar_or(1, 256, !alive) : named_bar_or(2, 256, !alive)) alive = false;
-    }
-    if (n > first && alive) {
+    // the output of the last block
+    if (n > 0 && alive && __all_sync(0xffffffffu, mbar_wait(&o_full[i], (n - 1) & 1, 124 + i))) {
       tc_fence_after();
-      const float l = half == 0 ? l_run + *theirs : *theirs + l_run;
+      const float l = l_run[0] + l_run[1];
       const float inv = (l > 0.f) ? 1.f / l : 0.f;
-      __nv_bfloat16* dst = args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64;
-      __nv_bfloat16* dst_lo = MODS == 0 ? nullptr : args.mods.out_lo + (dst - args.out);
+      __nv_bfloat16* dst = args.out + ((long long)b * args.S + qrow) * args.out_stride + h * HD;
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) {
         uint32_t r[32];
         tmem_ld32(tO + c * 32, r);
         tmem_ld_wait();
@@ -419,16 +288,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             uint4 w;
-            if (MODS != 0 && args.mods.out_lo != nullptr) {
-              uint32_t lo[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = __uint_as_float(r[8 * v + 2 * e]) * inv, y = __uint_as_float(r[8 * v + 2 * e + 1]) * inv;
-                const float2 hi = unpack_bf16x2(pack_bf16x2(x, y));
-                lo[e] = pack_bf16x2(x - hi.x, y - hi.y);
-              }
-              reinterpret_cast<uint4*>(dst_lo + c * 32)[v] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
             w.x = pack_bf16x2(__uint_as_float(r[8 * v + 0]) * inv, __uint_as_float(r[8 * v + 1]) * inv);
             w.y = pack_bf16x2(__uint_as_float(r[8 * v + 2]) * inv, __uint_as_float(r[8 * v + 3]) * inv);
             w.z = pack_bf16x2(__uint_as_float(r[8 * v + 4]) * inv, __uint_as_float(r[8 * v + 5]) * inv);
@@ -437,8 +296,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
           }
         }
       }
-      if (half == 0 && qrow < args.S)
-        args.lse[((long long)b * args.Hq + h) * args.S + qrow] = (l > 0.f) ? (m_run * ((MODS & (MOD_CAP | MOD_BIAS)) ? 0.6931471805599453f : args.scale) + logf(l)) : -INFINITY;
+      if (qrow < args.S)
+        args.lse[((long long)b * args.Hq + h) * args.S + qrow] = (l > 0.f) ? (m_run * args.scale + logf(l)) : -INFINITY;
     }
     tc_fence_before();
   }
@@ -453,32 +312,29 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
 
 }  // namespace
 
-template <int MODS>
-static int attn_fwd_launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdArgs& a, cudaStream_t st) {
-  static bool optin[64] = {};  // the shared-memory opt-in is a per-device attribute
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
-  if (!optin[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel<MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM);
-    if (e != cudaSuccess) return -(int)e;
-    optin[dev] = true;
-  }
-  if (int rc = yf_tu_bind_status()) return rc;
-  dim3 grid(a.Hq, a.B, (a.S + a.tiles * BQ - 1) / (a.tiles * BQ));
-  attn_fwd_kernel<MODS><<<grid, FWD_THREADS, FWD_SMEM, st>>>(mq, mk, mv, a);
-  return -(int)cudaGetLastError();
-}
-
-static int attn_fwd_any(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq, int Hkv, long long q_stride,
-                        long long k_stride, long long v_stride, long long out_stride, float scale, int causal, int mods, const AttnMods& m, void* stream) {
-  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv) || (q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (out_stride % 8)) return -1;
+// q, k, v: bf16 pointers to the first head's first column; token rows are q_stride / kv_stride elements
+// apart (the three may alias one fused projection output).  Tokens are ordered [batch, seq].
+// out: [B*S, out_stride] bf16 (head h at columns h*128), lse: [B, Hq, S] fp32.
+extern "C" int yf_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq,
+                           int Hkv, long long q_stride, long long kv_stride, long long out_stride, float scale, int causal,
+                           void* stream) {
+  if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv) || (q_stride % 8) || (kv_stride % 8) || (out_stride % 8)) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out)) & 15)
     return -1;
   const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
-  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
-  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
   if (!mq || !mk || !mv) return -2;
+  static bool optin[64] = {};  // the shared-memory opt-in is a per-device attribute
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!optin[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(attn_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM);
+    if (e != cudaSuccess) return -(int)e;
+    optin[dev] = true;
+  }
+  if (int rc = yf_tu_bind_status()) return rc;
   FwdArgs a;
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.lse = lse;
@@ -488,37 +344,7 @@ static int attn_fwd_any(const void* q, const void* k, const void* v, void* out, 
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal ? 1 : 0;
   a.tiles = (long long)((S + BQ - 1) / BQ) * Hq * B <= yf_num_sms() ? 1 : 2;
-  a.mods = m;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (mods) {
-    case 0: return attn_fwd_launch<0>(*mq, *mk, *mv, a, st);
-    case MOD_SPANS: return attn_fwd_launch<MOD_SPANS>(*mq, *mk, *mv, a, st);
-    case MOD_SPANS | MOD_CAP: return attn_fwd_launch<MOD_SPANS | MOD_CAP>(*mq, *mk, *mv, a, st);
-    case MOD_SPANS | MOD_BIAS: return attn_fwd_launch<MOD_SPANS | MOD_BIAS>(*mq, *mk, *mv, a, st);
-    default: return attn_fwd_launch<MOD_SPANS | MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, a, st);
-  }
-}
-
-// q, k, v: bf16 pointers to the first head's first column; token rows are q_stride / kv_stride elements
-// apart (the three may alias one fused projection output).  Tokens are ordered [batch, seq].
-// out: [B*S, out_stride] bf16 (head h at columns h*128), lse: [B, Hq, S] fp32.
-extern "C" int yf_attn_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int B, int S, int Hq,
-                           int Hkv, long long q_stride, long long kv_stride, long long out_stride, float scale, int causal,
-                           void* stream) {
-  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, kv_stride, kv_stride, out_stride, scale, causal, 0, AttnMods{}, stream);
-}
-
-// The general form: scores capped at +-softcap (0: not) and less slopes[h] * distance (null: not), keys by `spans` and `padding` as
-// yf_document_mask gives them (both null: causal).  Rows without a key: zeros, lse -inf.  out_lo (may be null): what the rounding of `out`
-// left over, for the backward pass.
-extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int S, int Hq, int Hkv,
-                                long long q_stride, long long k_stride, long long v_stride, long long out_stride, float scale, float softcap, const float* slopes,
-                                const int* spans, const int* padding, void* stream) {
-  if (!(softcap >= 0.f) || (spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(spans) & 7) || B > 65535 ||
-      (reinterpret_cast<uintptr_t>(out_lo) & 15))
-    return -1;
-  AttnMods m = attn_mods(scale, softcap, slopes, spans, padding);
-  m.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
-  const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
-  return attn_fwd_any(q, k, v, out, lse, B, S, Hq, Hkv, q_stride, k_stride, v_stride, out_stride, scale, 1, mods, m, stream);
+  dim3 grid(Hq, B, (S + a.tiles * BQ - 1) / (a.tiles * BQ));
+  attn_fwd_kernel<<<grid, FWD_THREADS, FWD_SMEM, reinterpret_cast<cudaStream_t>(stream)>>>(*mq, *mk, *mv, a);
+  return -(int)cudaGetLastError();
 }

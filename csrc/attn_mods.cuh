@@ -57,8 +57,15 @@ YF_DEVINL void cap_scores(uint32_t (&s)[32], const AttnMods& m) {
 #pragma unroll
   for (int t = 0; t < 32; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
   if (far <= m.poly_max) {
+    const uint64_t p0 = f32x2(m.poly[0], m.poly[0]), p1 = f32x2(m.poly[1], m.poly[1]), p2 = f32x2(m.poly[2], m.poly[2]),
+                   p3 = f32x2(m.poly[3], m.poly[3]), p4 = f32x2(m.poly[4], m.poly[4]);
 #pragma unroll
-    for (int t = 0; t < 32; ++t) s[t] = __float_as_uint(capped_small(__uint_as_float(s[t]), m));
+    for (int t = 0; t < 32; t += 2) {  // capped_small, two at a time
+      const uint64_t x = f32x2(__uint_as_float(s[t]), __uint_as_float(s[t + 1])), z = mul_f32x2(x, x);
+      const float2 y = f32x2_split(mul_f32x2(x, fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(p4, z, p3), z, p2), z, p1), z, p0)));
+      s[t] = __float_as_uint(y.x);
+      s[t + 1] = __float_as_uint(y.y);
+    }
   } else {
 #pragma unroll
     for (int t = 0; t < 32; ++t) s[t] = __float_as_uint(capped_any(__uint_as_float(s[t]), m));

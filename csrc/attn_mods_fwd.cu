@@ -1,0 +1,474 @@
+// Flash-attention forward for head_dim 128 on sm_100a (MHA and GQA) with ranges of keys for every query, capped scores and a distance
+// bias (attn_mods.cuh).
+//
+// One CTA per (256 query rows, query head, sequence), as two tiles of 128 rows (one tile where the whole problem then still fits the
+// GPU at once).  A tile walks over the half blocks of 64 keys between its first row's first key and its last row's last one.  Roles:
+//   warp 0       TMA producer: Q once, then K/V tiles of 128 keys through a 2-stage ring; clears the padded rows of V tiles that have some
+//   warp 1       MMA issuer:   S = Q K^T and O += P V, half block by half block
+//   warps 2-9    softmax of tile 0, warps 10-17 of tile 1: two threads per query row (TMEM lane == row), 32 keys of a half block each
+// TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  S_i has two halves of 64 columns, one for each half of a block;
+// P (bf16, 32 columns) takes the place of its half of S, whose row its two threads have read into registers, and is the MMA's A
+// operand from there.  While the softmax of one half runs, the tensor cores take the other half's P V and then its next S, so the softmax
+// warps have work all the time (with whole blocks, S(j+1) waited for P(j) V and both for each other: 555 instead of ISITNOW us at 8192 x 32).
+// The exponent's reference maximum is only moved when some row of a warp has grown by more than 2^8 since it was set (then its pair of
+// warps rescales its rows of O in TMEM and their sums); the final division by the row sum makes the result exact again.  A row's bits depend
+// on the 32 rows that share its warps.
+// Bound: per 128 x 128 block S takes 768 cycles of the tensor cores (N = 64 is limited by shared memory: 48 instead of 32 cycles per
+// instruction), P V 512, the exponentials 1024 of the special-function units.
+#include "attn_mods.cuh"
+#include "common.cuh"
+#include "yafsdp_b200.h"
+
+YF_TU_STATUS()
+
+namespace {
+
+constexpr int HD = 128;        // head dim
+constexpr int BQ = 128;        // query rows per tile
+constexpr int BKV = 128;       // keys per tile of K and V
+constexpr int HKV = 64;        // keys per half block
+constexpr int ATOM = 16384;    // bytes of one [128 rows x 64 bf16] swizzled block
+constexpr int TILE = 2 * ATOM; // one 128x128 bf16 tile
+constexpr int FWD_THREADS = 576;  // producer warp, MMA warp, sixteen softmax warps
+constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct FwdArgs {
+  __nv_bfloat16* out;
+  float* lse;
+  long long out_stride;  // elements between token rows of out
+  int S, B, Hq, Hkv;
+  float scale_log2;      // softmax scale * log2(e)
+  float scale;
+  int tiles;             // query tiles per CTA: two, or one where even so every CTA finds an SM of its own
+  AttnMods mods;
+};
+
+template <int MODS>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
+                     const __grid_constant__ CUtensorMap tma_v, FwdArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                   // tile i at + i * TILE
+  uint8_t* sKV = sQ + 2 * TILE;         // stage s: K at sKV + s*2*TILE, V at + TILE
+  float* sRow = reinterpret_cast<float*>(sKV + 4 * TILE);  // [tile][thread of the row][row]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 2 * BQ);
+  uint64_t* q_full = bars;              // [2] per tile
+  uint64_t* k_full = bars + 2;          // [2] per stage
+  uint64_t* v_full = bars + 4;          // [2]
+  uint64_t* k_empty = bars + 6;         // [2]
+  uint64_t* v_empty = bars + 8;         // [2]
+  uint64_t* s_full = bars + 10;         // [2][2] per tile and half, as the next two
+  uint64_t* p_ready = bars + 14;
+  uint64_t* o_done = bars + 18;
+  uint64_t* v_land = bars + 22;         // a V tile with padded rows has landed, to be cleared before it counts as full
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [2][4] per tile and pair of warps: 1 + the half block at which one of them has given up
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  // the query position is the slowest index: under the causal mask the long rows of all heads start first
+  const int qt = (int)(gridDim.z - 1 - blockIdx.z);
+  const int h = blockIdx.x;
+  const int b = blockIdx.y;
+  const int hkv = h / (args.Hq / args.Hkv);
+  const int q0 = qt * args.tiles * BQ;
+  const int n_tiles_kv = (args.S + BKV - 1) / BKV;
+  const int2* spans = args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
+  const int* padding = args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * n_tiles_kv;
+  // half blocks [from, to) of the two tiles; none when the sequence ends before, for nothing but padding, or without a second tile
+  int from[2], to[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int row0 = q0 + i * BQ, rows = min(BQ, args.S - row0);
+    from[i] = to[i] = 0;
+    if (i >= args.tiles || rows <= 0) continue;
+    if (spans == nullptr) {
+      to[i] = (row0 + rows + HKV - 1) / HKV;
+    } else if (__ldg(padding + row0 / BQ) < rows) {
+      from[i] = max(__ldg(spans + row0).x, 0) / HKV;
+      to[i] = min(__ldg(spans + row0 + rows - 1).y, args.S);
+      to[i] = max((to[i] + HKV - 1) / HKV, from[i]);
+    }
+    if (from[i] >= to[i]) from[i] = to[i] = 0;
+  }
+  const bool has0 = to[0] > 0, has1 = to[1] > 0;
+  const int j_first = (has0 && has1 ? min(from[0], from[1]) : has0 ? from[0] : from[1]) >> 1;
+  const int j_end = (max(to[0], to[1]) + 1) >> 1;
+  // phase of the barriers of half u of tile i at block j: how often that half has been used before
+  auto phase = [&](int i, int j, int u) { return (j - (((i == 0 ? from[0] : from[1]) - u + 1) >> 1)) & 1; };
+  auto active = [&](int i, int j, int u) { return 2 * j + u >= (i == 0 ? from[0] : from[1]) && 2 * j + u < (i == 0 ? to[0] : to[1]); };
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tma_q);
+    tma_prefetch_desc(&tma_k);
+    tma_prefetch_desc(&tma_v);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&k_full[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_ready[s], 8);  // one arrival per softmax warp of the tile
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(v_land, 1);
+    for (int s = 0; s < 8; ++s) dead[s] = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // the whole warp, since it clears the padded rows of the V tiles that have some
+    if (lane == 0 && has0) {
+      mbar_expect_tx(&q_full[0], TILE);
+      tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
+      tma_load_3d(sQ + ATOM, &tma_q, &q_full[0], h * HD + 64, q0, b);
+    }
+    int dead_rows = padding != nullptr && j_first < j_end ? __ldg(padding + j_first) : 0, landed = 0;
+    for (int j = j_first; j < j_end; ++j) {
+      const int s = (j - j_first) & 1, ph = (((j - j_first) >> 1) & 1) ^ 1;
+      uint8_t* sK = sKV + s * 2 * TILE;
+      uint8_t* sV = sK + TILE;
+      const bool clear = dead_rows > 0;
+      if (padding != nullptr && j + 1 < j_end) dead_rows = __ldg(padding + j + 1);
+      bool ok = true;
+      if (lane == 0) {
+        ok = mbar_wait(&k_empty[s], ph, 400);
+        if (ok) {
+          mbar_expect_tx(&k_full[s], TILE);
+          tma_load_3d(sK, &tma_k, &k_full[s], hkv * HD, j * BKV, b);
+          tma_load_3d(sK + ATOM, &tma_k, &k_full[s], hkv * HD + 64, j * BKV, b);
+          if (j == j_first && has1) {
+            mbar_expect_tx(&q_full[1], TILE);
+            tma_load_3d(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ, b);
+            tma_load_3d(sQ + TILE + ATOM, &tma_q, &q_full[1], h * HD + 64, q0 + BQ, b);
+          }
+          ok = mbar_wait(&v_empty[s], ph, 401);
+        }
+        if (ok) {
+          uint64_t* bar = clear ? v_land : &v_full[s];
+          mbar_expect_tx(bar, TILE);
+          tma_load_3d(sV, &tma_v, bar, hkv * HD, j * BKV, b);
+          tma_load_3d(sV + ATOM, &tma_v, bar, hkv * HD + 64, j * BKV, b);
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+      if (clear) {
+        if (!__all_sync(0xffffffffu, mbar_wait(v_land, landed & 1, 402))) break;
+        ++landed;
+        zero_padded_rows(sV, ATOM, BKV, j * BKV, args.S, spans);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[s]);
+      }
+    }
+  } else if (warp == 1) {
+    if (j_first < j_end && elect_one()) {
+      const uint32_t idesc_s = umma_idesc_bf16(BQ, HKV, 0, 0);   // Q, K both K-major (K = head dim)
+      const uint32_t idesc_o = umma_idesc_bf16(BQ, HD, 0, 1);    // P from TMEM (K = keys), V MN-major
+      const uint64_t dQ = umma_smem_desc_sw128(smem_u32(sQ), 0, 1024);
+      const uint64_t dK = umma_smem_desc_sw128(smem_u32(sKV), 0, 1024);
+      const uint64_t dV = umma_smem_desc_sw128(smem_u32(sKV) + TILE, ATOM, 1024);
+      // descriptor addresses advance in units of 16 bytes; half a tile of K is 64 rows of 128 bytes further on in either column block
+      auto issue_s = [&](int i, int j, int u) {
+        const uint64_t q = dQ + i * (TILE >> 4), k = dK + ((((j - j_first) & 1) * 2 * TILE + u * HKV * 128) >> 4);
+        const uint32_t t = tmem_base + i * 128 + u * HKV;
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) {
+          const uint32_t off = ((e >> 2) * ATOM + (e & 3) * 32) >> 4;
+          tc_mma_bf16(t, q + off, k + off, idesc_s, e != 0);
+        }
+        tc_commit(&s_full[i * 2 + u]);
+      };
+      auto issue_o = [&](int i, int j, int u) {
+        const uint64_t v = dV + ((((j - j_first) & 1) * 2 * TILE + u * HKV * 128) >> 4);
+        const uint32_t t = tmem_base + i * 128 + u * HKV;
+#pragma unroll
+        for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
+          tc_mma_bf16_ts(tmem_base + 256 + i * 128, t + e * 8, v + e * (2048 >> 4), idesc_o, 2 * j + u != (i == 0 ? from[0] : from[1]) || e != 0);
+        tc_commit(&o_done[i * 2 + u]);
+      };
+      // The next S of a half goes into the columns that its P holds, and the order of MMAs with different accumulators is not promised: P V
+      // is waited for, but only after the next half's P V has been issued too.
+      int p_i = -1, p_j = 0, p_u = 0;  // the half whose P V was issued last
+      bool p_last = false;             // of its block
+      auto follow = [&]() -> bool {
+        if (p_i < 0) return true;
+        const int i = p_i;
+        p_i = -1;
+        if (active(i, p_j + 1, p_u)) {
+          if (!mbar_wait(&o_done[i * 2 + p_u], phase(i, p_j, p_u), 410 + i)) return false;
+          tc_fence_after();
+          issue_s(i, p_j + 1, p_u);
+        }
+        if (p_last && p_j + 1 < j_end) tc_commit(&k_empty[(p_j + 1 - j_first) & 1]);
+        return true;
+      };
+      // the first S of a half that a tile has not used yet
+      auto begin = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (active(i, j, u) && !active(i, j - 1, u)) issue_s(i, j, u);
+      };
+      bool alive = (!has0 || mbar_wait(&q_full[0], 0, 412)) && (!has1 || mbar_wait(&q_full[1], 0, 413)) && mbar_wait(&k_full[0], 0, 414);
+      if (alive) {
+        tc_fence_after();
+        begin(j_first);
+        tc_commit(&k_empty[0]);
+      }
+      for (int j = j_first; j < j_end && alive; ++j) {
+        const int s = (j - j_first) & 1;
+        if (j + 1 < j_end) {
+          if (!mbar_wait(&k_full[s ^ 1], ((j + 1 - j_first) >> 1) & 1, 415)) break;
+          tc_fence_after();
+          begin(j + 1);
+        }
+        if (!mbar_wait(&v_full[s], ((j - j_first) >> 1) & 1, 416)) break;
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (!alive || !active(i, j, u)) continue;
+            if (!mbar_wait(&p_ready[i * 2 + u], phase(i, j, u), 417 + i)) { alive = false; continue; }
+            tc_fence_after();
+            issue_o(i, j, u);
+            alive = follow();
+            p_i = i; p_j = j; p_u = u;
+            p_last = false;
+            any = true;
+          }
+        p_last = true;
+        tc_commit(&v_empty[s]);
+        if (!any) {  // a block between the tiles' ranges
+          alive = alive && follow();
+          if (j + 1 < j_end) tc_commit(&k_empty[s ^ 1]);
+        }
+      }
+    }
+  } else {
+    const int i = (warp - 2) >> 3;           // tile
+    const int half = ((warp - 2) >> 2) & 1;  // of a half block's keys, of the columns of O
+    const int lo = i == 0 ? from[0] : from[1], hi = i == 0 ? to[0] : to[1];
+    const int q = warp & 3;                  // a warp may only touch TMEM lanes [32*(warp%4), +32)
+    const int bar = 1 + i * 4 + q;           // barrier of the two warps that share 32 rows
+    const int qrow = q0 + i * BQ + q * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off + i * 128, tO = tmem_base + lane_off + 256 + i * 128 + half * 64;
+    float* mine = sRow + (i * 2 + half) * BQ + q * 32 + lane;
+    float* theirs = sRow + (i * 2 + (half ^ 1)) * BQ + q * 32 + lane;
+    volatile int* gone = dead + i * 4 + q;
+    float m_run = -INFINITY;                 // reference maximum of the exponent
+    float l_run = 0.f;                       // sum over this thread's keys
+    const float sl2 = args.scale_log2;
+    constexpr float RESCALE_LOG2 = 8.f;      // move the reference maximum when a row's maximum exceeds it by 2^8
+    int2 span = make_int2(0, qrow + 1);      // keys [x, y) of this row
+    if (spans != nullptr || qrow >= args.S) span = qrow < args.S ? __ldg(spans + qrow) : make_int2(0, 0);
+    const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[h] * LOG2E : 0.f;
+    // scores that were transformed are in units of log2 already
+    const float to_log2 = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
+    const uint64_t to_log2_2 = f32x2(to_log2, to_log2);
+    bool alive = true;
+    for (int t = lo; t < hi; ++t) {
+      const int u = t & 1, j = t >> 1;
+      const int ph = (j - ((lo - u + 1) >> 1)) & 1;
+      // a bounded wait that runs out ends the work of the two warps: they meet at the barrier below, so the one that gives up says so there
+      // (the lanes of a warp decide together: TMEM accesses are warp-wide)
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(&s_full[i * 2 + u], ph, 420 + i));
+      const int kv0 = t * HKV + half * 32;
+      uint32_t sc[32];
+      if (alive) {
+        tc_fence_after();
+        tmem_ld32(tS + u * HKV + half * 32, sc);
+        tmem_ld_wait();
+      } else {
+        *gone = t + 1;
+      }
+      if (MODS & MOD_CAP) cap_scores(sc, args.mods);
+      if (MODS & MOD_BIAS) {
+        const float far = (float)(kv0 - qrow);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = __uint_as_float(sc[e]);
+          sc[e] = __float_as_uint(fmaf(-slope, fabsf(far + (float)e), (MODS & MOD_CAP) ? x : x * sl2));
+        }
+      }
+      if (kv0 < span.x || kv0 + 32 > span.y) {  // the ends of a row's range
+        const uint32_t seen = bit_range(span.x - kv0, span.y - kv0);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!((seen >> e) & 1u)) sc[e] = 0xff800000u;  // -inf
+      }
+      float mx4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx4[c] = __uint_as_float(sc[c * 8]);
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx4[c] = fmaxf(mx4[c], __uint_as_float(sc[c * 8 + e]));
+      }
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      const bool grew = !alive || t == lo || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * to_log2 > RESCALE_LOG2));
+      // Behind this barrier both threads of a row have read their parts of S, so P may take its place.
+      if (named_bar_or(bar, 64, grew)) {
+        if (*gone == t + 1) { alive = false; break; }  // not a later half block's: who gives up there waits for this warp there
+        *mine = mx;
+        named_bar_sync(bar, 64);
+        const float m_new = fmaxf(m_run, fmaxf(mx, *theirs));
+        if (t > lo) {
+          // O holds sums relative to the old maximum: wait for the last P V to land, then scale this warp's part of the rows
+          const int up = u ^ 1, jp = (t - 1) >> 1;
+          alive = __all_sync(0xffffffffu, mbar_wait(&o_done[i * 2 + up], (jp - ((lo - up + 1) >> 1)) & 1, 422 + i));
+          if (!alive) continue;  // to the next barrier, where the other warp learns of it
+          tc_fence_after();
+          const float alpha = (m_run == -INFINITY) ? 0.f : fast_exp2((m_run - m_new) * to_log2);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[16];
+            tmem_ld16(tO + c * 16, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * alpha);
+            tmem_st16(tO + c * 16, r);
+          }
+          l_run *= alpha;
+        }
+        m_run = m_new;
+      }
+      const float neg_ms = (m_run == -INFINITY) ? 0.f : -m_run * to_log2;
+      const uint64_t neg_ms_2 = f32x2(neg_ms, neg_ms);
+      uint64_t sum = f32x2(0.f, 0.f);
+      uint32_t packed[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), to_log2_2, neg_ms_2));
+        const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
+        sum = add_f32x2(sum, f32x2(p0, p1));
+        packed[e] = pack_bf16x2(p0, p1);
+      }
+      tmem_st16(tS + u * HKV + half * 16, packed);
+      const float2 two = f32x2_split(sum);
+      l_run += two.x + two.y;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[i * 2 + u]);
+    }
+    if (lo == hi) {  // nothing but padding, or no tile here: zeros
+      if (qrow < args.S && i < args.tiles) {
+        const long long at = ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+          reinterpret_cast<uint4*>(args.out + at)[v] = make_uint4(0u, 0u, 0u, 0u);
+          if (args.mods.out_lo != nullptr) reinterpret_cast<uint4*>(args.mods.out_lo + at)[v] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (half == 0) args.lse[((long long)b * args.Hq + h) * args.S + qrow] = -INFINITY;
+      }
+    } else {
+      // the output of the last half block, and the sum of both threads
+      const int u = (hi - 1) & 1, j = (hi - 1) >> 1;
+      alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[i * 2 + u], (j - ((lo - u + 1) >> 1)) & 1, 424 + i));
+      *mine = l_run;
+      if (named_bar_or(bar, 64, !alive)) alive = false;
+    }
+    if (lo < hi && alive) {
+      tc_fence_after();
+      const float l = half == 0 ? l_run + *theirs : *theirs + l_run;
+      const float inv = (l > 0.f) ? 1.f / l : 0.f;
+      const long long at = ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld32(tO + c * 32, r);
+        tmem_ld_wait();
+        if (qrow < args.S) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint32_t w[4], lw[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = __uint_as_float(r[8 * v + 2 * e]) * inv, y = __uint_as_float(r[8 * v + 2 * e + 1]) * inv;
+              w[e] = pack_bf16x2(x, y);
+              const float2 z = unpack_bf16x2(w[e]);
+              lw[e] = pack_bf16x2(x - z.x, y - z.y);
+            }
+            reinterpret_cast<uint4*>(args.out + at + c * 32)[v] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (args.mods.out_lo != nullptr) reinterpret_cast<uint4*>(args.mods.out_lo + at + c * 32)[v] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+          }
+        }
+      }
+      if (half == 0 && qrow < args.S)
+        args.lse[((long long)b * args.Hq + h) * args.S + qrow] =
+            (l > 0.f) ? (m_run * ((MODS & (MOD_CAP | MOD_BIAS)) ? 0.6931471805599453f : args.scale) + logf(l)) : -INFINITY;
+    }
+    tc_fence_before();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int MODS>
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdArgs& a, cudaStream_t st) {
+  static bool optin[64] = {};  // the shared-memory opt-in is a per-device attribute
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!optin[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(attn_mods_fwd_kernel<MODS>, cudaFuncAttributeMaxDynamicSharedMemorySize, FWD_SMEM);
+    if (e != cudaSuccess) return -(int)e;
+    optin[dev] = true;
+  }
+  if (int rc = yf_tu_bind_status()) return rc;
+  dim3 grid(a.Hq, a.B, (a.S + a.tiles * BQ - 1) / (a.tiles * BQ));
+  attn_mods_fwd_kernel<MODS><<<grid, FWD_THREADS, FWD_SMEM, st>>>(mq, mk, mv, a);
+  return -(int)cudaGetLastError();
+}
+
+}  // namespace
+
+// As yf_attn_fwd, with row pitches of their own for k and v, scores capped at +-softcap (0: not) and less slopes[h] * distance (null: not), keys
+// by `spans` and `padding` as yf_document_mask gives them (both null: causal).  Rows without a key: zeros, lse -inf.  out_lo (may be null):
+// what the rounding of `out` left over, for the backward pass.
+extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int S, int Hq, int Hkv,
+                                long long q_stride, long long k_stride, long long v_stride, long long out_stride, float scale, float softcap,
+                                const float* slopes, const int* spans, const int* padding, void* stream) {
+  if (B <= 0 || B > 65535 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv) || (q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (out_stride % 8)) return -1;
+  if (!(softcap >= 0.f) || !(scale > 0.f) || (spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(spans) & 7)) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15)
+    return -1;
+  const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
+  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
+  if (!mq || !mk || !mv) return -2;
+  FwdArgs a;
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.out_stride = out_stride;
+  a.S = S; a.B = B; a.Hq = Hq; a.Hkv = Hkv;
+  a.scale = scale;
+  a.scale_log2 = scale * LOG2E;
+  a.tiles = (long long)((S + BQ - 1) / BQ) * Hq * B <= yf_num_sms() ? 1 : 2;
+  a.mods = attn_mods(scale, softcap, slopes, spans, padding);
+  a.mods.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (softcap > 0.f) return slopes != nullptr ? launch<MOD_SPANS | MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, a, st) : launch<MOD_SPANS | MOD_CAP>(*mq, *mk, *mv, a, st);
+  return slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS>(*mq, *mk, *mv, a, st) : launch<MOD_SPANS>(*mq, *mk, *mv, a, st);
+}
