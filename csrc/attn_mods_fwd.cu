@@ -3,18 +3,19 @@
 //
 // One CTA per (256 query rows, query head, sequence), as two tiles of 128 rows (one tile where the whole problem then still fits the
 // GPU at once).  A tile walks over the half blocks of 64 keys between its first row's first key and its last row's last one.  Roles:
-//   warp 0       TMA producer: Q once, then K/V tiles of 128 keys through a 2-stage ring; clears the padded rows of V tiles that have some
-//   warp 1       MMA issuer:   S = Q K^T and O += P V, half block by half block
+//   warps 18, 0  TMA producers: Q once and K, and V, in tiles of 128 keys through rings of three and two stages; the latter clears the padded
+//                rows of V tiles that have some
+//   warp 1       MMA issuer:   S = Q K^T block by block and O += P V half block by half block
 //   warps 2-9    softmax of tile 0, warps 10-17 of tile 1: two threads per query row (TMEM lane == row), 32 keys of a half block each
-// TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  S_i has two halves of 64 columns, one for each half of a block;
-// P (bf16, 32 columns) takes the place of its half of S, whose row its two threads have read into registers, and is the MMA's A
-// operand from there.  While the softmax of one half runs, the tensor cores take the other half's P V and then its next S, so the softmax
-// warps have work all the time (with whole blocks, S(j+1) waited for P(j) V and both for each other: 555 instead of ISITNOW us at 8192 x 32).
+// TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  The softmax takes S_i in halves of 64 keys; a half's P (bf16, 32
+// columns) takes the place of its part of S, whose row its two threads have read into registers, and is the MMA's A operand from
+// there, under the softmax of the other half.  The next S has to wait for the whole P, so one tile's products run under the other one's softmax.
+// (S itself in halves, each with columns of its own, would uncouple them, but an MMA that reads 128 rows of A from shared memory takes 64 cycles at
+// N = 64 as at N = 128.)
 // The exponent's reference maximum is only moved when some row of a warp has grown by more than 2^8 since it was set (then its pair of
 // warps rescales its rows of O in TMEM and their sums); the final division by the row sum makes the result exact again.  A row's bits depend
 // on the 32 rows that share its warps.
-// Bound: per 128 x 128 block S takes 768 cycles of the tensor cores (N = 64 is limited by shared memory: 48 instead of 32 cycles per
-// instruction), P V 512, the exponentials 1024 of the special-function units.
+// Bound: per 128 x 128 block the two MMAs take 1024 cycles and the exponentials as long, on different pipes.
 #include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
@@ -29,8 +30,10 @@ constexpr int BKV = 128;       // keys per tile of K and V
 constexpr int HKV = 64;        // keys per half block
 constexpr int ATOM = 16384;    // bytes of one [128 rows x 64 bf16] swizzled block
 constexpr int TILE = 2 * ATOM; // one 128x128 bf16 tile
-constexpr int FWD_THREADS = 576;  // producer warp, MMA warp, sixteen softmax warps
-constexpr int FWD_SMEM = 1024 + 2 * TILE /*Q*/ + 2 * 2 * TILE /*K,V x2 stages*/ + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
+constexpr int FWD_THREADS = 640;  // producer warps of V and K, two MMA warps, sixteen softmax warps
+constexpr int KST = 3, VST = 2;   // stages of K and V
+constexpr int FWD_SMEM = 2 * TILE /*Q*/ + (KST + VST) * TILE + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
+static_assert(FWD_SMEM <= 232448, "shared memory of one CTA");
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct FwdArgs {
@@ -48,23 +51,28 @@ template <int MODS>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                      const __grid_constant__ CUtensorMap tma_v, FwdArgs args) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                   // tile i at + i * TILE
-  uint8_t* sKV = sQ + 2 * TILE;         // stage s: K at sKV + s*2*TILE, V at + TILE
-  float* sRow = reinterpret_cast<float*>(sKV + 4 * TILE);  // [tile][thread of the row][row]
+  uint8_t* sK = sQ + 2 * TILE;          // stage s at + s * TILE
+  uint8_t* sV = sK + KST * TILE;
+  float* sRow = reinterpret_cast<float*>(sV + VST * TILE);  // [tile][thread of the row][row]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + 2 * 2 * BQ);
   uint64_t* q_full = bars;              // [2] per tile
-  uint64_t* k_full = bars + 2;          // [2] per stage
-  uint64_t* v_full = bars + 4;          // [2]
-  uint64_t* k_empty = bars + 6;         // [2]
-  uint64_t* v_empty = bars + 8;         // [2]
-  uint64_t* s_full = bars + 10;         // [2][2] per tile and half, as the next two
-  uint64_t* p_ready = bars + 14;
-  uint64_t* o_done = bars + 18;
-  uint64_t* v_land = bars + 22;         // a V tile with padded rows has landed, to be cleared before it counts as full
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
+  uint64_t* k_full = bars + 2;          // [KST] per stage
+  uint64_t* k_empty = k_full + KST;
+  uint64_t* v_full = k_empty + KST;     // [VST]
+  uint64_t* v_empty = v_full + VST;
+  uint64_t* s_full = v_empty + VST;     // [2][2] per tile and half, as the next two
+  uint64_t* p_ready = s_full + 4;
+  uint64_t* o_done = p_ready + 4;
+  uint64_t* v_land = o_done + 4;        // a V tile with padded rows has landed, to be cleared before it counts as full
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_land + 1);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);  // [2][4] per tile and pair of warps: 1 + the half block at which one of them has given up
+  // nothing but this array is in shared memory, so it starts on the boundary that the swizzled tiles need
+  if ((smem_u32(smem) & 1023) != 0) {
+    if (threadIdx.x == 0) yf_raise(YF_ERR_BAD_ARGUMENT, 430);
+    return;
+  }
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -96,20 +104,21 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
   const bool has0 = to[0] > 0, has1 = to[1] > 0;
   const int j_first = (has0 && has1 ? min(from[0], from[1]) : has0 ? from[0] : from[1]) >> 1;
   const int j_end = (max(to[0], to[1]) + 1) >> 1;
-  // phase of the barriers of half u of tile i at block j: how often that half has been used before
-  auto phase = [&](int i, int j, int u) { return (j - (((i == 0 ? from[0] : from[1]) - u + 1) >> 1)) & 1; };
-  auto active = [&](int i, int j, int u) { return 2 * j + u >= (i == 0 ? from[0] : from[1]) && 2 * j + u < (i == 0 ? to[0] : to[1]); };
-
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tma_q);
     tma_prefetch_desc(&tma_k);
     tma_prefetch_desc(&tma_v);
+    const int n_tiles = max(1, (has0 ? 1 : 0) + (has1 ? 1 : 0));  // one arrival each for a stage that is free again
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], n_tiles);
+    }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], n_tiles);
+    }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&k_full[s], 1);
-      mbar_init(&v_full[s], 1);
-      mbar_init(&k_empty[s], 1);
-      mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
@@ -129,136 +138,116 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // the whole warp, since it clears the padded rows of the V tiles that have some
-    if (lane == 0 && has0) {
-      mbar_expect_tx(&q_full[0], TILE);
-      tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
-      tma_load_3d(sQ + ATOM, &tma_q, &q_full[0], h * HD + 64, q0, b);
+  if (warp == 18) {
+    if (j_first < j_end && elect_one()) {
+      for (int j = j_first, s = 0, ph = 1; j < j_end; ++j) {
+        if (!mbar_wait(&k_empty[s], ph, 400)) break;
+        if (j == j_first && has0) {
+          mbar_expect_tx(&q_full[0], TILE);
+          tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
+          tma_load_3d(sQ + ATOM, &tma_q, &q_full[0], h * HD + 64, q0, b);
+        }
+        mbar_expect_tx(&k_full[s], TILE);
+        tma_load_3d(sK + s * TILE, &tma_k, &k_full[s], hkv * HD, j * BKV, b);
+        tma_load_3d(sK + s * TILE + ATOM, &tma_k, &k_full[s], hkv * HD + 64, j * BKV, b);
+        if (j == j_first && has1) {
+          mbar_expect_tx(&q_full[1], TILE);
+          tma_load_3d(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ, b);
+          tma_load_3d(sQ + TILE + ATOM, &tma_q, &q_full[1], h * HD + 64, q0 + BQ, b);
+        }
+        if (++s == KST) { s = 0; ph ^= 1; }
+      }
     }
+  } else if (warp == 0) {
+    // V: the whole warp, since it clears the padded rows of the tiles that have some
     int dead_rows = padding != nullptr && j_first < j_end ? __ldg(padding + j_first) : 0, landed = 0;
-    for (int j = j_first; j < j_end; ++j) {
-      const int s = (j - j_first) & 1, ph = (((j - j_first) >> 1) & 1) ^ 1;
-      uint8_t* sK = sKV + s * 2 * TILE;
-      uint8_t* sV = sK + TILE;
+    for (int j = j_first, s = 0, ph = 1; j < j_end; ++j) {
       const bool clear = dead_rows > 0;
       if (padding != nullptr && j + 1 < j_end) dead_rows = __ldg(padding + j + 1);
-      bool ok = true;
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[s], ph, 401))) break;
       if (lane == 0) {
-        ok = mbar_wait(&k_empty[s], ph, 400);
-        if (ok) {
-          mbar_expect_tx(&k_full[s], TILE);
-          tma_load_3d(sK, &tma_k, &k_full[s], hkv * HD, j * BKV, b);
-          tma_load_3d(sK + ATOM, &tma_k, &k_full[s], hkv * HD + 64, j * BKV, b);
-          if (j == j_first && has1) {
-            mbar_expect_tx(&q_full[1], TILE);
-            tma_load_3d(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ, b);
-            tma_load_3d(sQ + TILE + ATOM, &tma_q, &q_full[1], h * HD + 64, q0 + BQ, b);
-          }
-          ok = mbar_wait(&v_empty[s], ph, 401);
-        }
-        if (ok) {
-          uint64_t* bar = clear ? v_land : &v_full[s];
-          mbar_expect_tx(bar, TILE);
-          tma_load_3d(sV, &tma_v, bar, hkv * HD, j * BKV, b);
-          tma_load_3d(sV + ATOM, &tma_v, bar, hkv * HD + 64, j * BKV, b);
-        }
+        uint64_t* bar = clear ? v_land : &v_full[s];
+        mbar_expect_tx(bar, TILE);
+        tma_load_3d(sV + s * TILE, &tma_v, bar, hkv * HD, j * BKV, b);
+        tma_load_3d(sV + s * TILE + ATOM, &tma_v, bar, hkv * HD + 64, j * BKV, b);
       }
-      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
       if (clear) {
         if (!__all_sync(0xffffffffu, mbar_wait(v_land, landed & 1, 402))) break;
         ++landed;
-        zero_padded_rows(sV, ATOM, BKV, j * BKV, args.S, spans);
+        zero_padded_rows(sV + s * TILE, ATOM, BKV, j * BKV, args.S, spans);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&v_full[s]);
       }
+      if (++s == VST) { s = 0; ph ^= 1; }
     }
-  } else if (warp == 1) {
-    if (j_first < j_end && elect_one()) {
+  } else if (warp == 1 || warp == 19) {
+    // One issuer for each tile, both in the same few instructions: an issuer comes by too seldom for its code to stay in the cache, and was the
+    // bound when one thread went through all four halves of both tiles.
+    const int i = warp == 1 ? 0 : 1;
+    const int lo = i == 0 ? from[0] : from[1], hi = i == 0 ? to[0] : to[1];
+    if (lo < hi && elect_one()) {
       const uint32_t idesc_s = umma_idesc_bf16(BQ, HKV, 0, 0);   // Q, K both K-major (K = head dim)
       const uint32_t idesc_o = umma_idesc_bf16(BQ, HD, 0, 1);    // P from TMEM (K = keys), V MN-major
-      const uint64_t dQ = umma_smem_desc_sw128(smem_u32(sQ), 0, 1024);
-      const uint64_t dK = umma_smem_desc_sw128(smem_u32(sKV), 0, 1024);
-      const uint64_t dV = umma_smem_desc_sw128(smem_u32(sKV) + TILE, ATOM, 1024);
+      const uint64_t dQ = umma_smem_desc_sw128(smem_u32(sQ) + i * TILE, 0, 1024);
+      const uint64_t dK = umma_smem_desc_sw128(smem_u32(sK), 0, 1024);
+      const uint64_t dV = umma_smem_desc_sw128(smem_u32(sV), ATOM, 1024);
+      const uint32_t tS = tmem_base + i * 128, tO = tmem_base + 256 + i * 128;
       // descriptor addresses advance in units of 16 bytes; half a tile of K is 64 rows of 128 bytes further on in either column block
-      auto issue_s = [&](int i, int j, int u) {
-        const uint64_t q = dQ + i * (TILE >> 4), k = dK + ((((j - j_first) & 1) * 2 * TILE + u * HKV * 128) >> 4);
-        const uint32_t t = tmem_base + i * 128 + u * HKV;
+      auto issue_s = [&](int stage, int u) {
+        const uint64_t k = dK + (uint32_t)(stage * (TILE >> 4) + u * (HKV * 128 >> 4));
 #pragma unroll
         for (int e = 0; e < HD / 16; ++e) {
           const uint32_t off = ((e >> 2) * ATOM + (e & 3) * 32) >> 4;
-          tc_mma_bf16(t, q + off, k + off, idesc_s, e != 0);
+          tc_mma_bf16(tS + u * HKV, dQ + off, k + off, idesc_s, e != 0);
         }
         tc_commit(&s_full[i * 2 + u]);
       };
-      auto issue_o = [&](int i, int j, int u) {
-        const uint64_t v = dV + ((((j - j_first) & 1) * 2 * TILE + u * HKV * 128) >> 4);
-        const uint32_t t = tmem_base + i * 128 + u * HKV;
-#pragma unroll
-        for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
-          tc_mma_bf16_ts(tmem_base + 256 + i * 128, t + e * 8, v + e * (2048 >> 4), idesc_o, 2 * j + u != (i == 0 ? from[0] : from[1]) || e != 0);
-        tc_commit(&o_done[i * 2 + u]);
+      // blocks that only the other tile walks over: passed on as soon as they are there
+      int kj = j_first, ks = 0, kp = 0;  // the block whose K comes next, its stage and phase
+      auto next_k = [&]() {
+        ++kj;
+        if (++ks == KST) { ks = 0; kp ^= 1; }
       };
-      // The next S of a half goes into the columns that its P holds, and the order of MMAs with different accumulators is not promised: P V
-      // is waited for, but only after the next half's P V has been issued too.
-      int p_i = -1, p_j = 0, p_u = 0;  // the half whose P V was issued last
-      bool p_last = false;             // of its block
-      auto follow = [&]() -> bool {
-        if (p_i < 0) return true;
-        const int i = p_i;
-        p_i = -1;
-        if (active(i, p_j + 1, p_u)) {
-          if (!mbar_wait(&o_done[i * 2 + p_u], phase(i, p_j, p_u), 410 + i)) return false;
-          tc_fence_after();
-          issue_s(i, p_j + 1, p_u);
+      auto pass = [&](int until) {
+        for (int j = kj; j < until; ++j) {
+          const int vs = (j - j_first) & 1;
+          if (!mbar_wait(&k_full[ks], kp, 410 + i)) return false;
+          mbar_arrive(&k_empty[ks]);
+          next_k();
+          if (!mbar_wait(&v_full[vs], ((j - j_first) >> 1) & 1, 412 + i)) return false;
+          mbar_arrive(&v_empty[vs]);
         }
-        if (p_last && p_j + 1 < j_end) tc_commit(&k_empty[(p_j + 1 - j_first) & 1]);
         return true;
       };
-      // the first S of a half that a tile has not used yet
-      auto begin = [&](int j) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (active(i, j, u) && !active(i, j - 1, u)) issue_s(i, j, u);
-      };
-      bool alive = (!has0 || mbar_wait(&q_full[0], 0, 412)) && (!has1 || mbar_wait(&q_full[1], 0, 413)) && mbar_wait(&k_full[0], 0, 414);
-      if (alive) {
-        tc_fence_after();
-        begin(j_first);
-        tc_commit(&k_empty[0]);
-      }
-      for (int j = j_first; j < j_end && alive; ++j) {
-        const int s = (j - j_first) & 1;
-        if (j + 1 < j_end) {
-          if (!mbar_wait(&k_full[s ^ 1], ((j + 1 - j_first) >> 1) & 1, 415)) break;
+      bool alive = mbar_wait(&q_full[i], 0, 414 + i) && pass(lo >> 1);
+      // S of half block t goes into the columns that P of t - 2 held: P V of t - 2 has been waited for, the order of MMAs with different
+      // accumulators is not promised
+      for (int t = lo - 2; t < hi && alive; ++t) {
+        const int u = t & 1, j = t >> 1;
+        if (t >= lo) {
+          const int vs = (j - j_first) & 1, ph = (j - ((lo - u + 1) >> 1)) & 1;
+          if (!mbar_wait(&v_full[vs], ((j - j_first) >> 1) & 1, 416 + i) || !mbar_wait(&p_ready[i * 2 + u], ph, 418 + i)) { alive = false; break; }
           tc_fence_after();
-          begin(j + 1);
+          const uint64_t v = dV + (uint32_t)(vs * (TILE >> 4) + u * (HKV * 128 >> 4));
+#pragma unroll
+          for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
+            tc_mma_bf16_ts(tO, tS + u * HKV + e * 8, v + e * (2048 >> 4), idesc_o, t != lo || e != 0);
+          tc_commit(&o_done[i * 2 + u]);
+          if (u == 1 || t == hi - 1) tc_commit(&v_empty[vs]);
+          if (t + 2 < hi && !mbar_wait(&o_done[i * 2 + u], ph, 420 + i)) { alive = false; break; }
         }
-        if (!mbar_wait(&v_full[s], ((j - j_first) >> 1) & 1, 416)) break;
-        bool any = false;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (!alive || !active(i, j, u)) continue;
-            if (!mbar_wait(&p_ready[i * 2 + u], phase(i, j, u), 417 + i)) { alive = false; continue; }
-            tc_fence_after();
-            issue_o(i, j, u);
-            alive = follow();
-            p_i = i; p_j = j; p_u = u;
-            p_last = false;
-            any = true;
+        if (t + 2 < hi) {
+          if (!mbar_wait(&k_full[ks], kp, 422 + i)) { alive = false; break; }
+          tc_fence_after();
+          issue_s(ks, u);
+          if (u == 1 || t + 2 == hi - 1) {  // the last S of its block
+            tc_commit(&k_empty[ks]);
+            next_k();
           }
-        p_last = true;
-        tc_commit(&v_empty[s]);
-        if (!any) {  // a block between the tiles' ranges
-          alive = alive && follow();
-          if (j + 1 < j_end) tc_commit(&k_empty[s ^ 1]);
         }
       }
+      alive = alive && pass(j_end);
     }
   } else {
     const int i = (warp - 2) >> 3;           // tile
