@@ -30,7 +30,7 @@ constexpr int BKV = 128;       // keys per tile of K and V
 constexpr int HKV = 64;        // keys per half block
 constexpr int ATOM = 16384;    // bytes of one [128 rows x 64 bf16] swizzled block
 constexpr int TILE = 2 * ATOM; // one 128x128 bf16 tile
-constexpr int FWD_THREADS = 640;  // producer warps of V and K, two MMA warps, sixteen softmax warps
+constexpr int FWD_THREADS = 640;  // producer warp, three MMA warps, sixteen softmax warps
 constexpr int KST = 3, VST = 2;   // stages of K and V
 constexpr int FWD_SMEM = 2 * TILE /*Q*/ + (KST + VST) * TILE + 2 * 2 * BQ * 4 /*between the threads of a row*/ + 256;
 static_assert(FWD_SMEM <= 232448, "shared memory of one CTA");
@@ -50,7 +50,8 @@ struct FwdArgs {
 template <int MODS>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
-                     const __grid_constant__ CUtensorMap tma_v, FwdArgs args) {
+                     const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ CUtensorMap tma_o,
+                     const __grid_constant__ CUtensorMap tma_lo, FwdArgs args) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem;                   // tile i at + i * TILE
   uint8_t* sK = sQ + 2 * TILE;          // stage s at + s * TILE
@@ -108,6 +109,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     tma_prefetch_desc(&tma_q);
     tma_prefetch_desc(&tma_k);
     tma_prefetch_desc(&tma_v);
+    tma_prefetch_desc(&tma_o);
     const int n_tiles = max(1, (has0 ? 1 : 0) + (has1 ? 1 : 0));  // one arrival each for a stage that is free again
     for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], 1);
@@ -115,7 +117,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     }
     for (int s = 0; s < VST; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], n_tiles);
+      mbar_init(&v_empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 1);
@@ -138,116 +140,108 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 18) {
-    if (j_first < j_end && elect_one()) {
-      for (int j = j_first, s = 0, ph = 1; j < j_end; ++j) {
-        if (!mbar_wait(&k_empty[s], ph, 400)) break;
-        if (j == j_first && has0) {
-          mbar_expect_tx(&q_full[0], TILE);
-          tma_load_3d(sQ, &tma_q, &q_full[0], h * HD, q0, b);
-          tma_load_3d(sQ + ATOM, &tma_q, &q_full[0], h * HD + 64, q0, b);
-        }
-        mbar_expect_tx(&k_full[s], TILE);
-        tma_load_3d(sK + s * TILE, &tma_k, &k_full[s], hkv * HD, j * BKV, b);
-        tma_load_3d(sK + s * TILE + ATOM, &tma_k, &k_full[s], hkv * HD + 64, j * BKV, b);
-        if (j == j_first && has1) {
-          mbar_expect_tx(&q_full[1], TILE);
-          tma_load_3d(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ, b);
-          tma_load_3d(sQ + TILE + ATOM, &tma_q, &q_full[1], h * HD + 64, q0 + BQ, b);
-        }
-        if (++s == KST) { s = 0; ph ^= 1; }
-      }
-    }
-  } else if (warp == 0) {
-    // V: the whole warp, since it clears the padded rows of the tiles that have some
+  if (warp == 0) {
+    // the whole warp, since it clears the padded rows of the V tiles that have some; K of a block comes before V of the block before
+    auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+      mbar_expect_tx(bar, TILE);
+      tma_load_3d(dst, map, bar, x, y, b);
+      tma_load_3d(dst + ATOM, map, bar, x + 64, y, b);
+    };
     int dead_rows = padding != nullptr && j_first < j_end ? __ldg(padding + j_first) : 0, landed = 0;
-    for (int j = j_first, s = 0, ph = 1; j < j_end; ++j) {
-      const bool clear = dead_rows > 0;
-      if (padding != nullptr && j + 1 < j_end) dead_rows = __ldg(padding + j + 1);
-      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[s], ph, 401))) break;
-      if (lane == 0) {
-        uint64_t* bar = clear ? v_land : &v_full[s];
-        mbar_expect_tx(bar, TILE);
-        tma_load_3d(sV + s * TILE, &tma_v, bar, hkv * HD, j * BKV, b);
-        tma_load_3d(sV + s * TILE + ATOM, &tma_v, bar, hkv * HD + 64, j * BKV, b);
+    int ks = 0, kp = 1, vs = 0, vp = 1;
+    for (int j = j_first; j <= j_end && j_first < j_end; ++j) {
+      bool ok = true;
+      if (lane == 0 && j < j_end) {
+        ok = mbar_wait(&k_empty[ks], kp, 400);
+        if (ok) {
+          if (j == j_first && has0) load(sQ, &tma_q, &q_full[0], h * HD, q0);
+          load(sK + ks * TILE, &tma_k, &k_full[ks], hkv * HD, j * BKV);
+          if (j == j_first && has1) load(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ);
+        }
+        if (++ks == KST) { ks = 0; kp ^= 1; }
       }
+      if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+      if (j == j_first) continue;
+      const bool clear = dead_rows > 0;
+      if (padding != nullptr && j < j_end) dead_rows = __ldg(padding + j);
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_empty[vs], vp, 401))) break;
+      if (lane == 0) load(sV + vs * TILE, &tma_v, clear ? v_land : &v_full[vs], hkv * HD, (j - 1) * BKV);
       if (clear) {
         if (!__all_sync(0xffffffffu, mbar_wait(v_land, landed & 1, 402))) break;
         ++landed;
-        zero_padded_rows(sV + s * TILE, ATOM, BKV, j * BKV, args.S, spans);
+        zero_padded_rows(sV + vs * TILE, ATOM, BKV, (j - 1) * BKV, args.S, spans);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[s]);
+        if (lane == 0) mbar_arrive(&v_full[vs]);
       }
-      if (++s == VST) { s = 0; ph ^= 1; }
+      if (++vs == VST) { vs = 0; vp ^= 1; }
     }
-  } else if (warp == 1 || warp == 19) {
-    // One issuer for each tile, both in the same few instructions: an issuer comes by too seldom for its code to stay in the cache, and was the
-    // bound when one thread went through all four halves of both tiles.
-    const int i = warp == 1 ? 0 : 1;
+  } else if (warp == 1) {
+    // O += P V, the tiles in turn
+    if (j_first < j_end && elect_one()) {
+      const uint32_t idesc_o = umma_idesc_bf16(BQ, HD, 0, 1);    // P from TMEM (K = keys), V MN-major
+      const uint64_t dV = umma_smem_desc_sw128(smem_u32(sV), ATOM, 1024);
+      bool alive = true;
+      for (int j = j_first; j < j_end && alive; ++j) {
+        const int vs = (j - j_first) & 1;
+        if (!mbar_wait(&v_full[vs], ((j - j_first) >> 1) & 1, 410)) break;
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          const int i = x & 1, u = x >> 1, t = 2 * j + u, lo = i == 0 ? from[0] : from[1], hi = i == 0 ? to[0] : to[1];
+          if (t < lo || t >= hi) continue;
+          if (!mbar_wait(&p_ready[i * 2 + u], (j - ((lo - u + 1) >> 1)) & 1, 411)) { alive = false; break; }
+          tc_fence_after();
+          const uint64_t v = dV + (uint32_t)(vs * (TILE >> 4) + u * (HKV * 128 >> 4));
+          const uint32_t p = tmem_base + i * 128 + u * HKV;
+#pragma unroll
+          for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
+            tc_mma_bf16_ts(tmem_base + 256 + i * 128, p + e * 8, v + e * (2048 >> 4), idesc_o, t != lo || e != 0);
+          tc_commit(&o_done[i * 2 + u]);
+        }
+        tc_commit(&v_empty[vs]);
+      }
+    }
+  } else if (warp >= 18) {
+    // S = Q K^T, one thread for each tile.  S of half block t goes into the columns that P of t - 2 held: P V of t - 2 is waited for, the order
+    // of MMAs with different accumulators is not promised.
+    const int i = warp - 18;
     const int lo = i == 0 ? from[0] : from[1], hi = i == 0 ? to[0] : to[1];
     if (lo < hi && elect_one()) {
       const uint32_t idesc_s = umma_idesc_bf16(BQ, HKV, 0, 0);   // Q, K both K-major (K = head dim)
-      const uint32_t idesc_o = umma_idesc_bf16(BQ, HD, 0, 1);    // P from TMEM (K = keys), V MN-major
       const uint64_t dQ = umma_smem_desc_sw128(smem_u32(sQ) + i * TILE, 0, 1024);
       const uint64_t dK = umma_smem_desc_sw128(smem_u32(sK), 0, 1024);
-      const uint64_t dV = umma_smem_desc_sw128(smem_u32(sV), ATOM, 1024);
-      const uint32_t tS = tmem_base + i * 128, tO = tmem_base + 256 + i * 128;
-      // descriptor addresses advance in units of 16 bytes; half a tile of K is 64 rows of 128 bytes further on in either column block
-      auto issue_s = [&](int stage, int u) {
-        const uint64_t k = dK + (uint32_t)(stage * (TILE >> 4) + u * (HKV * 128 >> 4));
-#pragma unroll
-        for (int e = 0; e < HD / 16; ++e) {
-          const uint32_t off = ((e >> 2) * ATOM + (e & 3) * 32) >> 4;
-          tc_mma_bf16(tS + u * HKV, dQ + off, k + off, idesc_s, e != 0);
-        }
-        tc_commit(&s_full[i * 2 + u]);
-      };
-      // blocks that only the other tile walks over: passed on as soon as they are there
-      int kj = j_first, ks = 0, kp = 0;  // the block whose K comes next, its stage and phase
+      int ks = 0, kp = 0;  // stage and phase of the block whose K comes next
       auto next_k = [&]() {
-        ++kj;
         if (++ks == KST) { ks = 0; kp ^= 1; }
       };
-      auto pass = [&](int until) {
-        for (int j = kj; j < until; ++j) {
-          const int vs = (j - j_first) & 1;
-          if (!mbar_wait(&k_full[ks], kp, 410 + i)) return false;
+      auto pass = [&](int blocks) {  // that only the other tile walks over: passed on as soon as they are there
+        for (; blocks > 0; --blocks) {
+          if (!mbar_wait(&k_full[ks], kp, 412 + i)) return false;
           mbar_arrive(&k_empty[ks]);
           next_k();
-          if (!mbar_wait(&v_full[vs], ((j - j_first) >> 1) & 1, 412 + i)) return false;
-          mbar_arrive(&v_empty[vs]);
         }
         return true;
       };
-      bool alive = mbar_wait(&q_full[i], 0, 414 + i) && pass(lo >> 1);
-      // S of half block t goes into the columns that P of t - 2 held: P V of t - 2 has been waited for, the order of MMAs with different
-      // accumulators is not promised
-      for (int t = lo - 2; t < hi && alive; ++t) {
-        const int u = t & 1, j = t >> 1;
-        if (t >= lo) {
-          const int vs = (j - j_first) & 1, ph = (j - ((lo - u + 1) >> 1)) & 1;
-          if (!mbar_wait(&v_full[vs], ((j - j_first) >> 1) & 1, 416 + i) || !mbar_wait(&p_ready[i * 2 + u], ph, 418 + i)) { alive = false; break; }
-          tc_fence_after();
-          const uint64_t v = dV + (uint32_t)(vs * (TILE >> 4) + u * (HKV * 128 >> 4));
+      bool alive = mbar_wait(&q_full[i], 0, 414 + i) && pass((lo >> 1) - j_first);
+      for (int t = lo; t < hi && alive; ++t) {
+        const int u = t & 1;
+        if ((u == 0 || t == lo) && !mbar_wait(&k_full[ks], kp, 416 + i)) break;
+        if (t >= lo + 2 && !mbar_wait(&o_done[i * 2 + u], ((t >> 1) - 1 - ((lo - u + 1) >> 1)) & 1, 418 + i)) break;
+        tc_fence_after();
+        // descriptor addresses advance in units of 16 bytes; half a tile of K is 64 rows of 128 bytes further on in either column block
+        const uint64_t k = dK + (uint32_t)(ks * (TILE >> 4) + u * (HKV * 128 >> 4));
 #pragma unroll
-          for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
-            tc_mma_bf16_ts(tO, tS + u * HKV + e * 8, v + e * (2048 >> 4), idesc_o, t != lo || e != 0);
-          tc_commit(&o_done[i * 2 + u]);
-          if (u == 1 || t == hi - 1) tc_commit(&v_empty[vs]);
-          if (t + 2 < hi && !mbar_wait(&o_done[i * 2 + u], ph, 420 + i)) { alive = false; break; }
+        for (int e = 0; e < HD / 16; ++e) {
+          const uint32_t off = ((e >> 2) * ATOM + (e & 3) * 32) >> 4;
+          tc_mma_bf16(tmem_base + i * 128 + u * HKV, dQ + off, k + off, idesc_s, e != 0);
         }
-        if (t + 2 < hi) {
-          if (!mbar_wait(&k_full[ks], kp, 422 + i)) { alive = false; break; }
-          tc_fence_after();
-          issue_s(ks, u);
-          if (u == 1 || t + 2 == hi - 1) {  // the last S of its block
-            tc_commit(&k_empty[ks]);
-            next_k();
-          }
+        tc_commit(&s_full[i * 2 + u]);
+        if (u == 1 || t == hi - 1) {  // the last S of its block
+          tc_commit(&k_empty[ks]);
+          next_k();
         }
       }
-      alive = alive && pass(j_end);
+      pass(j_end - ((hi + 1) >> 1));
     }
   } else {
     const int i = (warp - 2) >> 3;           // tile
@@ -377,28 +371,46 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       tc_fence_after();
       const float l = half == 0 ? l_run + *theirs : *theirs + l_run;
       const float inv = (l > 0.f) ? 1.f / l : 0.f;
-      const long long at = ((long long)b * args.S + qrow) * args.out_stride + h * HD + half * 64;
-#pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tO + c * 32, r);
-        tmem_ld_wait();
-        if (qrow < args.S) {
+      // The warp's 32 rows x 64 columns go out through the place of Q, which the tile's last product has read, and TMA (which leaves out the
+      // rows past the end): a thread's own 16 bytes at a time touch 32 lines with each instruction.
+      uint8_t* stage = sQ + i * TILE + half * ATOM + q * 32 * 128;
+      uint32_t r[2][32];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t w[4], lw[4];
+      for (int c = 0; c < 2; ++c) tmem_ld32(tO + c * 32, r[c]);
+      tmem_ld_wait();
+      uint32_t low[32];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = __uint_as_float(r[8 * v + 2 * e]) * inv, y = __uint_as_float(r[8 * v + 2 * e + 1]) * inv;
-              w[e] = pack_bf16x2(x, y);
-              const float2 z = unpack_bf16x2(w[e]);
-              lw[e] = pack_bf16x2(x - z.x, y - z.y);
-            }
-            reinterpret_cast<uint4*>(args.out + at + c * 32)[v] = make_uint4(w[0], w[1], w[2], w[3]);
-            if (args.mods.out_lo != nullptr) reinterpret_cast<uint4*>(args.mods.out_lo + at + c * 32)[v] = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-          }
+      for (int v = 0; v < 8; ++v) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __uint_as_float(r[v >> 2][8 * (v & 3) + 2 * e]) * inv, y = __uint_as_float(r[v >> 2][8 * (v & 3) + 2 * e + 1]) * inv;
+          w[e] = pack_bf16x2(x, y);
+          const float2 z = unpack_bf16x2(w[e]);
+          low[4 * v + e] = pack_bf16x2(x - z.x, y - z.y);
+        }
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&tma_o, stage, h * HD + half * 64, q0 + i * BQ + q * 32, b);
+        tma_store_commit();
+      }
+      if (args.mods.out_lo != nullptr) {
+        if (lane == 0) tma_store_wait_read0();
+        __syncwarp();
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(low[4 * v], low[4 * v + 1], low[4 * v + 2], low[4 * v + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&tma_lo, stage, h * HD + half * 64, q0 + i * BQ + q * 32, b);
+          tma_store_commit();
         }
       }
+      if (lane == 0) tma_store_wait0();
       if (half == 0 && qrow < args.S)
         args.lse[((long long)b * args.Hq + h) * args.S + qrow] =
             (l > 0.f) ? (m_run * ((MODS & (MOD_CAP | MOD_BIAS)) ? 0.6931471805599453f : args.scale) + logf(l)) : -INFINITY;
@@ -415,7 +427,8 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
 }
 
 template <int MODS>
-int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const FwdArgs& a, cudaStream_t st) {
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo, const CUtensorMap& ml, const FwdArgs& a,
+           cudaStream_t st) {
   static bool optin[64] = {};  // the shared-memory opt-in is a per-device attribute
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -426,7 +439,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, 
   }
   if (int rc = yf_tu_bind_status()) return rc;
   dim3 grid(a.Hq, a.B, (a.S + a.tiles * BQ - 1) / (a.tiles * BQ));
-  attn_mods_fwd_kernel<MODS><<<grid, FWD_THREADS, FWD_SMEM, st>>>(mq, mk, mv, a);
+  attn_mods_fwd_kernel<MODS><<<grid, FWD_THREADS, FWD_SMEM, st>>>(mq, mk, mv, mo, ml, a);
   return -(int)cudaGetLastError();
 }
 
@@ -446,7 +459,9 @@ extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, voi
   const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
   const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
   const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
-  if (!mq || !mk || !mv) return -2;
+  const CUtensorMap* mo = yf_tensor_map_3d(out, (uint64_t)Hq * HD, S, B, out_stride, (uint64_t)S * out_stride, 64, 32, 1, 2, 1);
+  const CUtensorMap* ml = out_lo == nullptr ? mo : yf_tensor_map_3d(out_lo, (uint64_t)Hq * HD, S, B, out_stride, (uint64_t)S * out_stride, 64, 32, 1, 2, 1);
+  if (!mq || !mk || !mv || !mo || !ml) return -2;
   FwdArgs a;
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.lse = lse;
@@ -458,6 +473,6 @@ extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, voi
   a.mods = attn_mods(scale, softcap, slopes, spans, padding);
   a.mods.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (softcap > 0.f) return slopes != nullptr ? launch<MOD_SPANS | MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, a, st) : launch<MOD_SPANS | MOD_CAP>(*mq, *mk, *mv, a, st);
-  return slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS>(*mq, *mk, *mv, a, st) : launch<MOD_SPANS>(*mq, *mk, *mv, a, st);
+  if (softcap > 0.f) return slopes != nullptr ? launch<MOD_SPANS | MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<MOD_SPANS | MOD_CAP>(*mq, *mk, *mv, *mo, *ml, a, st);
+  return slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<MOD_SPANS>(*mq, *mk, *mv, *mo, *ml, a, st);
 }

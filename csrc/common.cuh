@@ -149,6 +149,12 @@ YF_DEVINL void tma_store_2d(const CUtensorMap* m, const void* smem_src, int x, i
                "r"(smem_u32(smem_src)), "r"(x), "r"(y)
                : "memory");
 }
+YF_DEVINL void tma_store_3d(const CUtensorMap* m, const void* smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 YF_DEVINL void tma_reduce_add_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(m)),
