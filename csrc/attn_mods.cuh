@@ -18,10 +18,10 @@ struct AttnMods {
   float cap_log2;       // cap * log2(e)
   float cap_exp;        // 2 log2(e) scale / cap: tanh of a raw product s is 1 - 2 / (1 + 2^(s * cap_exp))
   float poly_max;       // |s| up to here: cap_log2 * tanh(s * scale / cap) = s * (poly[0] + poly[1] s^2 + ...)
-  float poly[5];
+  float poly[4];
 };
 
-// The host's part: tanh(x) / x as a polynomial in x^2, fitted for the least relative error (6e-7) on |x| <= 3/4, with the scale and
+// The host's part: tanh(x) / x as a polynomial in x^2, fitted for the least relative error (6e-7) on |x| <= 1/2, with the scale and
 // the cap multiplied in.  Caps so small that the factors would leave fp32 do without.
 inline AttnMods attn_mods(float scale, float softcap, const float* slopes, const int* spans, const int* padding) {
   AttnMods m = {};
@@ -29,13 +29,13 @@ inline AttnMods attn_mods(float scale, float softcap, const float* slopes, const
   m.padding = padding;
   m.slopes = slopes;
   if (softcap > 0.f) {
-    const double fit[5] = {0.999999435, -0.333282511, 0.132589789, -0.0500561567, 0.0129294833};
+    const double fit[4] = {0.999999456, -0.333263172, 0.131902872, -0.0444019209};
     const double x = (double)scale / (double)softcap, cap = 1.4426950408889634 * (double)softcap;
     m.cap_log2 = (float)cap;
     m.cap_exp = (float)(2.8853900817779268 * x);
-    m.poly_max = x < 1000. ? (float)(0.75 / x) : -1.f;
+    m.poly_max = x < 1000. ? (float)(0.5 / x) : -1.f;
     double power = cap * x;
-    for (int i = 0; i < 5; ++i, power *= x * x) m.poly[i] = x < 1000. ? (float)(fit[i] * power) : 0.f;
+    for (int i = 0; i < 4; ++i, power *= x * x) m.poly[i] = x < 1000. ? (float)(fit[i] * power) : 0.f;
   }
   return m;
 }
@@ -44,7 +44,7 @@ inline AttnMods attn_mods(float scale, float softcap, const float* slopes, const
 // about 2^-22 of the cap; the hardware's tanh is good to 2^-11 relative, 2 % of a probability at a cap of 50).  Both in one:
 YF_DEVINL float capped_small(float s, const AttnMods& m) {
   const float z = s * s;
-  return s * fmaf(fmaf(fmaf(fmaf(m.poly[4], z, m.poly[3]), z, m.poly[2]), z, m.poly[1]), z, m.poly[0]);
+  return s * fmaf(fmaf(fmaf(m.poly[3], z, m.poly[2]), z, m.poly[1]), z, m.poly[0]);
 }
 YF_DEVINL float capped_any(float s, const AttnMods& m) {
   float r;
@@ -58,11 +58,11 @@ YF_DEVINL void cap_scores(uint32_t (&s)[32], const AttnMods& m) {
   for (int t = 0; t < 32; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
   if (far <= m.poly_max) {
     const uint64_t p0 = f32x2(m.poly[0], m.poly[0]), p1 = f32x2(m.poly[1], m.poly[1]), p2 = f32x2(m.poly[2], m.poly[2]),
-                   p3 = f32x2(m.poly[3], m.poly[3]), p4 = f32x2(m.poly[4], m.poly[4]);
+                   p3 = f32x2(m.poly[3], m.poly[3]);
 #pragma unroll
     for (int t = 0; t < 32; t += 2) {  // capped_small, two at a time
       const uint64_t x = f32x2(__uint_as_float(s[t]), __uint_as_float(s[t + 1])), z = mul_f32x2(x, x);
-      const float2 y = f32x2_split(mul_f32x2(x, fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(p4, z, p3), z, p2), z, p1), z, p0)));
+      const float2 y = f32x2_split(mul_f32x2(x, fma_f32x2(fma_f32x2(fma_f32x2(p3, z, p2), z, p1), z, p0)));
       s[t] = __float_as_uint(y.x);
       s[t + 1] = __float_as_uint(y.y);
     }
