@@ -17,11 +17,9 @@
 // the MMAs of its neighbours.  Bound: about 1700 cycles of MMA per step (S^T, dP^T and dQ^T with N = 64 are limited by the
 // 128 bytes per cycle that shared memory delivers: 48 instead of 32 cycles per instruction).
 // D = rowsum(dO * O) comes from a small pre-pass; scale and bf16 of dQ are applied by a post-pass, of dK at the end.
-// Instantiations beyond plain causal attention (attn_mods.cuh): with t = tanh(scale s / cap), dS^T gets the factor 1 - t^2, and a key tile
-// walks over the queries between its first key's first query and its last key's last one.
 #include <stdio.h>
 
-#include "attn_mods.cuh"
+#include "attn_bwd_common.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
 
@@ -29,9 +27,6 @@ YF_TU_STATUS()
 
 namespace {
 
-constexpr int HD = 128;
-constexpr int BQ = 64;    // query rows per step
-constexpr int BKV = 128;  // keys per CTA
 constexpr int ATOM = 16384;        // [128 rows x 64 bf16], 128-byte swizzle
 constexpr int TILE = 2 * ATOM;     // K or V: [128 x 128] bf16
 constexpr int QATOM = 8192;        // [64 rows x 64 bf16]
@@ -57,44 +52,10 @@ struct BwdArgs {
   int head_parts;      // CTAs that share a key tile of a KV head, each with a part of its query heads
   float scale, scale_log2;
   int causal;
-  AttnMods mods;
 };
 
-YF_DEVINL void tma_reduce_add_3d(const CUtensorMap* m, const void* smem_src, int x, int y, int z) {
-  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(m)),
-               "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-
-// Where a CTA that shares its key tile leaves dK (is_v = 0) and dV: [head_parts][B][key tiles][Hkv][2] blocks of 32 groups of four head
-// dims x 128 keys, so that a warp, one key per lane, stores 512 contiguous bytes at a time (rows of 128 dims: 16 bytes in each of
-// 32 lines).
-constexpr int PART_TILE = BKV * HD / 4;  // float4s of a block
-__host__ __device__ inline long long part_tile(int part, int B, int b, int n_kt, int jt, int Hkv, int hk, int is_v) {
-  return (((((long long)part * B + b) * n_kt + jt) * Hkv + hk) * 2 + is_v) * PART_TILE;
-}
-
-// Order of the CTAs: heads are taken in groups, within a group key tile by key tile with the heads fastest, so that all heads'
-// long walks start first.  One group holds all heads unless the dQ accumulator outgrows the L2 and there are heads for three
-// groups; then a group has two CTAs per SM, whose sums stay in the L2.  It pays for many sequences or long ones: 8 x 2048 tokens x 32
-// heads 1449 us in one group, 1247 in groups of 19; 2 x 8192 x 32 3516 / 3438 in groups of five; 2 x 2304 x 32 393 / 380; 2 x 4096 x
-// 32 971 / 995 in groups of ten; 1 x 4096 x 64 984 / 1013.  1 x 8192 x 32/8 stays whole: 1543 us, 1572 in two groups.
-YF_DEVINL void head_group_order(int cta, int n_pos, int n_heads, int group, int& pos, int& head) {
-  const int per_group = n_pos * group;
-  const int g = cta / per_group;
-  const int r = cta - g * per_group;
-  const int size = min(group, n_heads - g * group);
-  pos = r / size;
-  head = g * group + r - pos * size;
-}
-int head_group_size(int n_pos, int n_heads, long long accum_bytes, int n_sms) {
-  const int group = (2 * n_sms + n_pos - 1) / n_pos;
-  return accum_bytes <= (64ll << 20) || group >= n_heads / 3 ? n_heads : group;
-}
-
 // SHARED: head_parts > 1 (an instantiation of its own: the parts' addresses cost the other one registers it does not have)
-template <bool SHARED, int MODS>
+template <bool SHARED>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                 const __grid_constant__ CUtensorMap tma_v, const __grid_constant__ CUtensorMap tma_do,
@@ -117,9 +78,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   uint64_t* vk_done = dq_full + 2;
   uint64_t* dq_read = vk_done + 2;
   uint64_t* all_done = dq_read + 2;         // every MMA of the walk (waiting two phases ahead on vk_done would not do)
-  uint64_t* kv_land = all_done + 1;         // MODS: bytes of K and V, and of a stage's Q and dO, before padded rows are cleared
-  uint64_t* q_land = kv_land + 1;           // [STAGES]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(MODS == 0 ? all_done + 1 : q_land + STAGES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -130,17 +89,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   const int heads = args.Hq / args.Hkv / head_parts;  // query heads of this CTA
   const int h0 = hk * (args.Hq / args.Hkv) + part * heads;
   const int kv0 = jt * BKV;
-  int i_start = args.causal ? kv0 / BQ : 0;          // first query tile
-  int per_head = (args.S + BQ - 1) / BQ - i_start;   // at least one: the tile that holds these keys' own rows
-  // ranges of queries by key, padded tokens by tile
-  const int2* spans = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
-  const int* padding = MODS == 0 || args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * ((args.S + BKV - 1) / BKV);
-  if (MODS != 0 && spans != nullptr) {
-    const int keys = min(BKV, args.S - kv0), n_qt = (args.S + BQ - 1) / BQ;
-    i_start = max(__ldg(spans + kv0).x, 0) / BQ;
-    per_head = min((__ldg(spans + kv0 + keys - 1).y + BQ - 1) / BQ, n_qt) - i_start;
-    if (__ldg(padding + jt) >= keys || per_head < 0) per_head = 0;  // nothing but padding
-  }
+  const int i_start = args.causal ? kv0 / BQ : 0;          // first query tile
+  const int per_head = (args.S + BQ - 1) / BQ - i_start;   // at least one: the tile that holds these keys' own rows
   const int n_it = per_head * heads;
 
   if (threadIdx.x == 0) {
@@ -151,12 +101,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     tma_prefetch_desc(&tma_dq);
     mbar_init(kv_full, 1);
     mbar_init(all_done, 1);
-    if (MODS != 0) {
-      mbar_init(kv_land, 1);
-      for (int i = 0; i < STAGES; ++i) mbar_init(&q_land[i], 1);
-    }
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&q_full[i], MODS == 0 ? 2 : 1);
+      mbar_init(&q_full[i], 2);
       mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -179,25 +125,23 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   const uint32_t tdV = tmem_base + 256, tdK = tmem_base + 384;  // set p of S^T | dP^T: tmem_base + 128 p, + 64
 
   if (warp == 12) {
-    if ((MODS == 0 || n_it > 0) && elect_one()) {
-      uint64_t* kv_bar = MODS == 0 ? kv_full : kv_land;
-      mbar_expect_tx(kv_bar, 2 * TILE);
-      tma_load_3d(sK, &tma_k, kv_bar, hk * HD, kv0, b);
-      tma_load_3d(sK + ATOM, &tma_k, kv_bar, hk * HD + 64, kv0, b);
-      tma_load_3d(sV, &tma_v, kv_bar, hk * HD, kv0, b);
-      tma_load_3d(sV + ATOM, &tma_v, kv_bar, hk * HD + 64, kv0, b);
+    if (elect_one()) {
+      mbar_expect_tx(kv_full, 2 * TILE);
+      tma_load_3d(sK, &tma_k, kv_full, hk * HD, kv0, b);
+      tma_load_3d(sK + ATOM, &tma_k, kv_full, hk * HD + 64, kv0, b);
+      tma_load_3d(sV, &tma_v, kv_full, hk * HD, kv0, b);
+      tma_load_3d(sV + ATOM, &tma_v, kv_full, hk * HD + 64, kv0, b);
       int h = h0, i = 0;
       for (int it = 0, st = 0, ph = 1; it < n_it; ++it) {
         if (!mbar_wait(&q_empty[st], ph, 200)) break;
         const int q0 = (i_start + i) * BQ;
         uint8_t* sQ = sRing + st * 2 * QTILE;
         uint8_t* sdO = sQ + QTILE;
-        uint64_t* q_bar = MODS == 0 ? &q_full[st] : &q_land[st];
-        mbar_expect_tx(q_bar, 2 * QTILE);
-        tma_load_3d(sQ, &tma_q, q_bar, h * HD, q0, b);
-        tma_load_3d(sQ + QATOM, &tma_q, q_bar, h * HD + 64, q0, b);
-        tma_load_3d(sdO, &tma_do, q_bar, h * HD, q0, b);
-        tma_load_3d(sdO + QATOM, &tma_do, q_bar, h * HD + 64, q0, b);
+        mbar_expect_tx(&q_full[st], 2 * QTILE);
+        tma_load_3d(sQ, &tma_q, &q_full[st], h * HD, q0, b);
+        tma_load_3d(sQ + QATOM, &tma_q, &q_full[st], h * HD + 64, q0, b);
+        tma_load_3d(sdO, &tma_do, &q_full[st], h * HD, q0, b);
+        tma_load_3d(sdO + QATOM, &tma_do, &q_full[st], h * HD + 64, q0, b);
         if (++i == per_head) { i = 0; ++h; }
         if (++st == STAGES) { st = 0; ph ^= 1; }
       }
@@ -217,15 +161,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         dl[e] = ok ? args.delta[at + r] : 0.f;
       }
     };
-    if (MODS == 0 || n_it > 0) fetch();
-    if (MODS != 0 && n_it > 0 && __all_sync(0xffffffffu, mbar_wait(kv_land, 0, 202))) {
-      if (padding != nullptr && __ldg(padding + jt) > 0) {  // dQ^T = K^T dS^T would multiply what padding holds by zeros
-        zero_padded_rows(sK, ATOM, BKV, kv0, args.S, spans);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) mbar_arrive(kv_full);
-    }
+    fetch();
     for (int it = 0, st = 0, ph = 1; it < n_it; ++it) {
       if (!__all_sync(0xffffffffu, mbar_wait(&q_empty[st], ph, 201))) break;
       float* stat = sStat + st * STAT_FLOATS;
@@ -234,16 +170,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         stat[lane + 32 * e] = nl[e];
         stat[BQ + lane + 32 * e] = dl[e];
       }
-      if (MODS != 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&q_land[st], ph ^ 1, 203))) break;
-        const int q0 = (i_start + i) * BQ;
-        if (padding != nullptr && __ldg(padding + q0 / BKV) > 0) {  // dK and dV: as above
-          uint8_t* sQ = sRing + st * 2 * QTILE;
-          zero_padded_rows(sQ, QATOM, BQ, q0, args.S, spans);
-          zero_padded_rows(sQ + QTILE, QATOM, BQ, q0, args.S, spans);
-          fence_proxy_async_smem();
-        }
-      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[st]);
       if (++i == per_head) { i = 0; ++h; }
@@ -251,7 +177,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (++st == STAGES) { st = 0; ph ^= 1; }
     }
   } else if (warp == 13) {
-    if ((MODS == 0 || n_it > 0) && elect_one()) {
+    if (elect_one()) {
       const uint32_t id_s = umma_idesc_bf16(128, BQ, 0, 0);    // S^T, dP^T: both operands K-major (K = head dim)
       const uint32_t id_g = umma_idesc_bf16(128, HD, 0, 1);    // dV, dK: A from TMEM (K = queries), dO / Q MN-major
       const uint32_t id_q = umma_idesc_bf16(128, BQ, 1, 1);    // dQ^T: K tile MN-major (M = head dim), dS^T MN-major
@@ -316,10 +242,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
     const float sl2 = args.scale_log2;
     uint8_t* ds_row = sdS + p * DS_BYTES + row * 128;
     bool alive = true;
-    int st = p, ph = 0, i = MODS != 0 && n_it == 0 ? 0 : p % per_head;  // ring stage and its parity, query tile of step p
-    int2 span = make_int2(key, args.S);       // queries [x, y) that see this key, with MODS
-    if (MODS != 0 && (spans != nullptr || key >= args.S)) span = key < args.S ? __ldg(spans + key) : make_int2(0, 0);
-    const float cap_inv = (MODS & MOD_CAP) ? 1.f / args.mods.cap_log2 : 0.f;
+    int st = p, ph = 0, i = p % per_head;     // ring stage and its parity, query tile of step p
     for (int it = p; it < n_it; it += 2) {
       const int q0 = (i_start + i) * BQ;
       // a bounded wait that runs out ends the warp's work (the lanes decide together: TMEM accesses are warp-wide)
@@ -328,9 +251,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       const float4* stat = reinterpret_cast<const float4*>(sStat + st * STAT_FLOATS);
       // queries [0, hidden) of the tile do not see this key: those in front of it, all when the key is past the end
       const int hidden = key >= args.S ? BQ : (args.causal ? key - q0 : 0);
-      const bool any_hidden = __any_sync(0xffffffffu, MODS == 0 ? hidden > 0 : (q0 < span.x || q0 + BQ > span.y));
-      const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h0 + it / per_head) * 1.4426950408889634f : 0.f;
-      const float far = (float)(q0 - key);
+      const bool any_hidden = __any_sync(0xffffffffu, hidden > 0);
       // 32 queries at a time: all but a few words (28 bytes, 52 with shared key tiles) stay in registers; a spill goes to the L2, as
       // shared memory leaves no L1
 #pragma unroll
@@ -339,40 +260,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
         tmem_ld32(t + c * 32, s);
         tmem_ld32(t + 64 + c * 32, dp);
         tmem_ld_wait();
-        if (MODS != 0) {
-          if (MODS & MOD_CAP) cap_scores(s, args.mods);
-          const uint32_t seen = bit_range(span.x - q0 - c * 32, span.y - q0 - c * 32);
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            const float4 nl4 = stat[c * 8 + v], dl4 = stat[BQ / 4 + c * 8 + v];
-            const float nl[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, dl[4] = {dl4.x, dl4.y, dl4.z, dl4.w};
-            float x[4], g[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float y = __uint_as_float(s[4 * v + e]);
-              g[e] = __uint_as_float(dp[4 * v + e]) - dl[e];
-              if (MODS & MOD_CAP) {
-                const float t = y * cap_inv;
-                g[e] *= fmaf(-t, t, 1.f);
-                y += nl[e];
-              } else {
-                y = fmaf(y, sl2, nl[e]);
-              }
-              if (MODS & MOD_BIAS) y = fmaf(-slope, fabsf(far + (float)(c * 32 + 4 * v + e)), y);
-              x[e] = fast_exp2(y);
-              g[e] *= x[e];
-            }
-            if (any_hidden) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!((seen >> (4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
-            }
-            pk[2 * v] = pack_bf16x2(x[0], x[1]);
-            pk[2 * v + 1] = pack_bf16x2(x[2], x[3]);
-            dk[2 * v] = pack_bf16x2(g[0], g[1]);
-            dk[2 * v + 1] = pack_bf16x2(g[2], g[3]);
-          }
-        } else
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
           const float4 nl = stat[c * 8 + v], dl = stat[BQ / 4 + c * 8 + v];
@@ -406,17 +293,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
       if (st >= STAGES) { st -= STAGES; ph ^= 1; }
     }
     // the results: the even steps' warps write dV, the odd steps' warps dK (TMEM lane == key)
-    if (MODS != 0 && n_it == 0) {  // nothing but padding: zeros
-      if (key < args.S) {
-        if (SHARED) {
-          float4* dst = args.dkv_parts + part_tile(part, args.B, b, (args.S + BKV - 1) / BKV, jt, args.Hkv, hk, p == 0 ? 1 : 0) + row;
-          for (int v = 0; v < HD / 4; ++v) dst[v * BKV] = make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>((p == 0 ? args.dv : args.dk) + ((long long)b * args.S + key) * args.dkv_stride + hk * HD);
-          for (int v = 0; v < HD / 8; ++v) dst[v] = make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    } else if (alive && __all_sync(0xffffffffu, mbar_wait(all_done, 0, 222))) {
+    if (alive && __all_sync(0xffffffffu, mbar_wait(all_done, 0, 222))) {
       tc_fence_after();
       const uint32_t src = (p == 0 ? tdV : tdK) + ((uint32_t)((warp & 3) * 32) << 16);
       const float f = p == 0 ? 1.f : args.scale;
@@ -519,162 +396,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   }
 }
 
-// delta[b,h,s] = sum_d dO * O, and the fp32 dQ accumulator of the same (token, head) cleared on the way (the main kernel
-// adds into it): sixteen lanes per (token, head), one 16-byte load of O and of dO and two 16-byte stores of zeros per lane.
-// LO: O is the sum of two bf16 tensors (attn_mods.cuh).
-template <bool LO>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o_lo, const __nv_bfloat16* __restrict__ d_o,
-                                                         float* __restrict__ delta, float* __restrict__ dq_zero, int B, int S, int Hq,
-                                                         long long o_stride, long long do_stride) {
-  const long long total = (long long)B * S * Hq;
-  const int sub = threadIdx.x & 15;
-  const unsigned half_mask = 0xffffu << (threadIdx.x & 16);  // the two halves of a warp may leave the loop at different times
-  for (long long w = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 4; w < total;
-       w += ((long long)gridDim.x * blockDim.x) >> 4) {
-    const int h = (int)(w % Hq);
-    const long long t = w / Hq;
-    const uint4 a = *reinterpret_cast<const uint4*>(o + t * o_stride + h * HD + sub * 8);
-    const uint4 g = *reinterpret_cast<const uint4*>(d_o + t * do_stride + h * HD + sub * 8);
-    if (dq_zero != nullptr) {
-      float4* z = reinterpret_cast<float4*>(dq_zero + (t * Hq + h) * HD + sub * 8);
-      z[0] = make_float4(0.f, 0.f, 0.f, 0.f);
-      z[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    const float2 a0 = unpack_bf16x2(a.x), a1 = unpack_bf16x2(a.y), a2 = unpack_bf16x2(a.z), a3 = unpack_bf16x2(a.w);
-    const float2 g0 = unpack_bf16x2(g.x), g1 = unpack_bf16x2(g.y), g2 = unpack_bf16x2(g.z), g3 = unpack_bf16x2(g.w);
-    float s = a0.x * g0.x + a0.y * g0.y + a1.x * g1.x + a1.y * g1.y + a2.x * g2.x + a2.y * g2.y + a3.x * g3.x + a3.y * g3.y;
-    if (LO) {
-      const uint4 l = *reinterpret_cast<const uint4*>(o_lo + t * o_stride + h * HD + sub * 8);
-      const float2 l0 = unpack_bf16x2(l.x), l1 = unpack_bf16x2(l.y), l2 = unpack_bf16x2(l.z), l3 = unpack_bf16x2(l.w);
-      s += l0.x * g0.x + l0.y * g0.y + l1.x * g1.x + l1.y * g1.y + l2.x * g2.x + l2.y * g2.y + l3.x * g3.x + l3.y * g3.y;
-    }
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(half_mask, s, m);
-    if (sub == 0) {
-      const long long bb = t / S, ss = t % S;
-      delta[(bb * Hq + h) * S + ss] = s;
-    }
-  }
-}
-
-// dst, dst + 64 (bf16) = f * (a, z): eight head dims and their partners 64 further on.  With `cs` (cos, sin of the eight dims) they
-// go back through the rotation on the way.
-YF_DEVINL void store_gradient(__nv_bfloat16* dst, float (&a)[8], float (&z)[8], const float4* cs, float f) {
-  if (cs != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float4 c = __ldg(cs + j);
-      const float a0 = a[2 * j], a1 = a[2 * j + 1];
-      a[2 * j] = a0 * c.x + z[2 * j] * c.y;
-      a[2 * j + 1] = a1 * c.z + z[2 * j + 1] * c.w;
-      z[2 * j] = z[2 * j] * c.x - a0 * c.y;
-      z[2 * j + 1] = z[2 * j + 1] * c.z - a1 * c.w;
-    }
-  }
-  uint4 w;
-  w.x = pack_bf16x2(a[0] * f, a[1] * f); w.y = pack_bf16x2(a[2] * f, a[3] * f);
-  w.z = pack_bf16x2(a[4] * f, a[5] * f); w.w = pack_bf16x2(a[6] * f, a[7] * f);
-  *reinterpret_cast<uint4*>(dst) = w;
-  w.x = pack_bf16x2(z[0] * f, z[1] * f); w.y = pack_bf16x2(z[2] * f, z[3] * f);
-  w.z = pack_bf16x2(z[4] * f, z[5] * f); w.w = pack_bf16x2(z[6] * f, z[7] * f);
-  *reinterpret_cast<uint4*>(dst + 64) = w;
-}
-YF_DEVINL const float4* rope_at(const float* rope, int pos, int dim) {
-  return rope == nullptr ? nullptr : reinterpret_cast<const float4*>(rope + ((long long)pos * 64 + dim) * 2);
-}
-
-// dq (bf16, strided rows) = scale * dq_accum (fp32, dense rows of 128 Hq); with dkv_parts also dk = scale * the sum of the parts' dK and
-// dv = that of their dV, in the order of the parts.  `rope` ([S, 64, 2]: cos, sin): dq and dk go back through the rotation.
-__global__ void __launch_bounds__(256) attn_convert_kernel(const float* __restrict__ dq_acc, const float4* __restrict__ dkv_parts, int parts, const float* __restrict__ rope,
-                                    __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv, int B,
-                                    int S, int Hq, int Hkv, long long dq_stride, long long dkv_stride, float scale) {
-  const long long first = blockIdx.x * (long long)blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
-  const long long n_dq = (long long)B * S * Hq * 8;
-  const int n_kt = (S + BKV - 1) / BKV;
-  const long long blocks = dkv_parts == nullptr ? 0 : (long long)B * n_kt * Hkv * 2;  // of a part
-  const long long total = n_dq + blocks * (BKV * 8);
-  for (long long i = first; i < total; i += step) {
-    float a[8], z[8];
-    if (i < n_dq) {
-      const long long t = i / (Hq * 8);
-      const int u = (int)(i - t * (Hq * 8)), h = u >> 3, v = (u & 7) * 8;
-      const float4* src = reinterpret_cast<const float4*>(dq_acc + (t * Hq + h) * HD + v);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 x = src[j], y = src[16 + j];
-        a[4 * j] = x.x; a[4 * j + 1] = x.y; a[4 * j + 2] = x.z; a[4 * j + 3] = x.w;
-        z[4 * j] = y.x; z[4 * j + 1] = y.y; z[4 * j + 2] = y.z; z[4 * j + 3] = y.w;
-      }
-      store_gradient(dq + t * dq_stride + h * HD + v, a, z, rope_at(rope, (int)(t % S), v), scale);
-    } else {  // a warp: eight keys x four groups of dims (whole lines read, 64 contiguous bytes per key written)
-      const long long k = i - n_dq, block = k >> 10;
-      const int v = ((int)k & 3) + ((int)(k >> 5) & 1) * 4, row = ((int)(k >> 2) & 7) + ((int)(k >> 6) & 15) * 8, is_v = (int)(block & 1);
-      const long long bj = (block >> 1) / Hkv;
-      const int hk = (int)((block >> 1) - bj * Hkv), s = (int)(bj % n_kt) * BKV + row;
-      if (s >= S) continue;
-      const float4* src = dkv_parts + block * PART_TILE + 2 * v * BKV + row;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] = z[j] = 0.f;
-      for (int p0 = 0; p0 < parts; p0 += 4, src += 4 * blocks * PART_TILE) {  // four parts in flight
-        float4 x[4][4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[p][j] = p0 + p < parts ? __ldcg(src + p * blocks * PART_TILE + ((j & 1) + (j >> 1) * 16) * BKV) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            a[4 * j] += x[p][j].x; a[4 * j + 1] += x[p][j].y; a[4 * j + 2] += x[p][j].z; a[4 * j + 3] += x[p][j].w;
-            z[4 * j] += x[p][2 + j].x; z[4 * j + 1] += x[p][2 + j].y; z[4 * j + 2] += x[p][2 + j].z; z[4 * j + 3] += x[p][2 + j].w;
-          }
-      }
-      __nv_bfloat16* dst = (is_v ? dv : dk) + ((bj / n_kt) * S + s) * dkv_stride + hk * HD + v * 8;
-      store_gradient(dst, a, z, is_v ? nullptr : rope_at(rope, s, v * 8), is_v ? 1.f : scale);
-    }
-  }
-}
-
-// CTAs per key tile of a KV head.  With grouped-query attention a KV head's key tiles are few and their walks long (every
-// query head of the group): the walk is cut by query heads where that is estimated to end sooner.  The main kernel takes its longest
-// walk or its share of all steps, 1.5 us a step and 8 us a CTA (start, end, first loads); the parts' sums (131 KB a CTA) are read at
-// 3.7 TB/s.  Measured, the whole backward pass, us, in 1 / 2 / 4 / 8 parts (* the choice):
-//   1 x 333 tokens, 64 / 8 heads 88 / 56 / 42 / 42*;  1 x 777, 64 / 8 166 / 103 / 72* / 92;  1 x 2048, 64 / 8 396 / 253* / 290 / 331;
-//   1 x 8192, 64 / 8 3422* / 3335 / 3455 / 3457;  8 x 300, 32 / 8 85* / 97 / 121;  4 x 1024, 32 / 8 162* / 204 / 255;
-//   1 x 4096, 32 / 8 455 / 479* / 542;  1 x 4096, 28 / 4 653 whole, 432* in seven.
-// (Cut until there were three CTAs per SM, 8 x 300 took 113, 4 x 1024 204 and 1 x 777 92 us.)
-int head_parts_for(int B, int S, int Hq, int Hkv) {
-  const int group = Hq / Hkv, n_kt = (S + BKV - 1) / BKV, n_qt = (S + BQ - 1) / BQ;
-  const float sms = (float)yf_num_sms(), walks = (float)n_kt * (float)Hkv * (float)B;
-  // steps of all walks, under the causal mask (key tile j starts at query tile 2 j)
-  const float longest = (float)n_qt * (float)group;
-  const float steps = (float)n_kt * (float)(n_qt - n_kt + 1) * (float)Hq * (float)B;
-  int best = 1;
-  float best_us = 0.f;
-  for (int parts = 1; parts <= group; ++parts) {
-    if (group % parts) continue;
-    const float walk = longest / (float)parts * 1.5f + 8.f, share = (steps * 1.5f + walks * (float)parts * 8.f) / sms;
-    const float us = (walk > share ? walk : share) + (parts > 1 ? walks * (float)parts * (131072.f / 3.7e6f) : 0.f);
-    if (parts == 1 || us < best_us) {
-      best = parts;
-      best_us = us;
-    }
-  }
-  return best;
-}
-
 }  // namespace
 
 // The three launches of one backward pass (delta pre-pass, main kernel, dQ conversion), shared by both entry points.
 // Allocates nothing: the tensor maps come by reference from the caller, the scratch by pointer.
-template <int MODS>
 static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& md,
                            const CUtensorMap& mdq, const void* out,
                            const void* dout, const float* lse, float* delta, float* dq_accum, void* dq, void* dk, void* dv, int B,
                            int S, int Hq, int Hkv, long long o_stride, long long do_stride, long long dq_stride,
-                           long long dkv_stride, float scale, int causal, const AttnMods& mods, cudaStream_t st) {
-  const auto kernel = dkv_parts != nullptr ? attn_bwd_kernel<true, MODS> : attn_bwd_kernel<false, MODS>;
+                           long long dkv_stride, float scale, int causal, cudaStream_t st) {
+  const auto kernel = dkv_parts != nullptr ? attn_bwd_kernel<true> : attn_bwd_kernel<false>;
   static bool optin[2][64] = {};  // the shared-memory opt-in is a per-device attribute
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
@@ -692,9 +423,9 @@ static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, 
     long long blocks = (groups * 16 + 255) / 256;
     const long long cap = (long long)yf_num_sms() * 8;
     if (blocks > cap) blocks = cap;
-    const auto pre = mods.out_lo != nullptr ? attn_delta_kernel<true> : attn_delta_kernel<false>;
-    pre<<<(int)blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(out), mods.out_lo, reinterpret_cast<const __nv_bfloat16*>(dout), delta, dq_accum,
-                                     B, S, Hq, o_stride, do_stride);
+    attn_delta_kernel<false><<<(int)blocks, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(out), nullptr,
+                                                  reinterpret_cast<const __nv_bfloat16*>(dout), delta, dq_accum, B, S, Hq,
+                                                  o_stride, do_stride);
   }
   BwdArgs a;
   a.lse = lse;
@@ -709,7 +440,6 @@ static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, 
   a.scale = scale;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal ? 1 : 0;
-  a.mods = mods;
   const int n_kt = (S + BKV - 1) / BKV;
   a.head_group = head_group_size(n_kt, B * Hkv * head_parts, T * Hq * HD * 4, yf_num_sms());  // the dQ accumulator
   const long long ctas = (long long)n_kt * B * Hkv * head_parts;
@@ -739,14 +469,14 @@ extern "C" int yf_attn_bwd_head_parts(int B, int S, int Hq, int Hkv) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
   return head_parts_for(B, S, Hq, Hkv);
 }
-static int attn_bwd_any(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                                  float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, const float* rope, void* dq, void* dk, void* dv, int B,
-                                 int S, int Hq, int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride,
-                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, int which, const AttnMods& mods, void* stream) {
+                                 int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
+                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, void* stream) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
   if (head_parts < 1 || (Hq / Hkv) % head_parts || (head_parts > 1) != (dkv_parts != nullptr)) return -1;
   if (dkv_parts != nullptr && dkv_floats < 4 * part_tile(head_parts, B, 0, (S + BKV - 1) / BKV, 0, Hkv, 0, 0)) return -1;
-  if ((q_stride % 8) || (k_stride % 8) || (v_stride % 8) || (o_stride % 8) || (do_stride % 8) || (dq_stride % 8) || (dkv_stride % 8)) return -1;
+  if ((q_stride % 8) || (kv_stride % 8) || (o_stride % 8) || (do_stride % 8) || (dq_stride % 8) || (dkv_stride % 8)) return -1;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(dq) |
        reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) | reinterpret_cast<uintptr_t>(dq_accum) |
@@ -754,40 +484,13 @@ static int attn_bwd_any(const void* q, const void* k, const void* v, const void*
     return -1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const CUtensorMap* mq = yf_tensor_map_3d(q, (uint64_t)Hq * HD, S, B, q_stride, (uint64_t)S * q_stride, 64, BQ, 1, 2, 1);
-  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, k_stride, (uint64_t)S * k_stride, 64, BKV, 1, 2, 1);
-  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, v_stride, (uint64_t)S * v_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mk = yf_tensor_map_3d(k, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
+  const CUtensorMap* mv = yf_tensor_map_3d(v, (uint64_t)Hkv * HD, S, B, kv_stride, (uint64_t)S * kv_stride, 64, BKV, 1, 2, 1);
   const CUtensorMap* md = yf_tensor_map_3d(dout, (uint64_t)Hq * HD, S, B, do_stride, (uint64_t)S * do_stride, 64, BQ, 1, 2, 1);
   const CUtensorMap* mdq = yf_tensor_map_3d(dq_accum, (uint64_t)Hq * HD, S, B, (uint64_t)Hq * HD, (uint64_t)S * Hq * HD, 32, BQ, 1, 4, 0);
   if (!mq || !mk || !mv || !md || !mdq) return -2;
-  const auto launch = which == 0 ? attn_bwd_launch<0>
-                      : which == MOD_SPANS ? attn_bwd_launch<MOD_SPANS>
-                      : which == (MOD_SPANS | MOD_CAP) ? attn_bwd_launch<MOD_SPANS | MOD_CAP>
-                      : which == (MOD_SPANS | MOD_BIAS) ? attn_bwd_launch<MOD_SPANS | MOD_BIAS>
-                                                        : attn_bwd_launch<MOD_SPANS | MOD_CAP | MOD_BIAS>;
-  return launch(head_parts, dkv_parts, rope, *mq, *mk, *mv, *md, *mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv,
-                o_stride, do_stride, dq_stride, dkv_stride, scale, causal, mods, st);
-}
-extern "C" int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
-                                 float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, const float* rope, void* dq, void* dk, void* dv, int B,
-                                 int S, int Hq, int Hkv, long long q_stride, long long kv_stride, long long o_stride,
-                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, int causal, void* stream) {
-  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, rope, dq, dk, dv, B, S, Hq, Hkv, q_stride, kv_stride,
-                      kv_stride, o_stride, do_stride, dq_stride, dkv_stride, scale, causal, 0, AttnMods{}, stream);
-}
-// Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal); out_lo as the forward pass left it, or null.
-extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse, float* delta,
-                                float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S,
-                                int Hq, int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride, long long do_stride,
-                                long long dq_stride, long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding,
-                                void* stream) {
-  if (!(softcap >= 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7) ||
-      (reinterpret_cast<uintptr_t>(out_lo) & 15))
-    return -1;
-  AttnMods m = attn_mods(scale, softcap, slopes, key_spans, padding);
-  m.out_lo = reinterpret_cast<__nv_bfloat16*>(const_cast<void*>(out_lo));
-  const int mods = MOD_SPANS | (softcap > 0.f ? MOD_CAP : 0) | (slopes != nullptr ? MOD_BIAS : 0);
-  return attn_bwd_any(q, k, v, out, dout, lse, delta, dq_accum, dkv_parts, dkv_floats, head_parts, nullptr, dq, dk, dv, B, S, Hq, Hkv, q_stride, k_stride,
-                      v_stride, o_stride, do_stride, dq_stride, dkv_stride, scale, 1, mods, m, stream);
+  return attn_bwd_launch(head_parts, dkv_parts, rope, *mq, *mk, *mv, *md, *mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv,
+                         o_stride, do_stride, dq_stride, dkv_stride, scale, causal, st);
 }
 extern "C" int yf_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                            float* delta, float* dq_accum, void* dq, void* dk, void* dv, int B, int S, int Hq, int Hkv,
@@ -876,6 +579,6 @@ extern "C" int yf_attn_bwd_noalloc(const void* q, const void* k, const void* v, 
       yf_tensor_map_3d_encode(&md, dout, (uint64_t)Hq * HD, S, B, do_stride, (uint64_t)S * do_stride, 64, BQ, 1, 2, 1) != 0 ||
       yf_tensor_map_3d_encode(&mdq, dq_accum, (uint64_t)Hq * HD, S, B, (uint64_t)Hq * HD, (uint64_t)S * Hq * HD, 32, BQ, 1, 4, 0) != 0)
     return -2;
-  return attn_bwd_launch<0>(1, nullptr, nullptr, mq, mk, mv, md, mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv, o_stride, do_stride, dq_stride,
-                         dkv_stride, scale, causal, AttnMods{}, st);
+  return attn_bwd_launch(1, nullptr, nullptr, mq, mk, mv, md, mdq, out, dout, lse, delta, dq_accum, dq, dk, dv, B, S, Hq, Hkv, o_stride, do_stride, dq_stride,
+                         dkv_stride, scale, causal, st);
 }

@@ -1,7 +1,7 @@
 // What the attention kernels do to a score between Q K^T and the softmax, and which keys a query sees, beyond the plain causal form:
 //   score = cap tanh(scale q.k / cap) - slope_h |i - j|       (either part optional)
 //   query i sees the keys spans[i] = [lo, hi); key j is seen by the queries key_spans[j]; padding sees and is seen by nothing
-// The kernels are instantiated for sets of these bits (0: plain causal attention, without any of this):
+// The kernels are instantiated for sets of these bits:
 #pragma once
 #include "common.cuh"
 
@@ -13,8 +13,8 @@ struct AttnMods {
   const int2* spans;    // [B, S] by query (forward) or by key (backward); null: causal
   const int* padding;   // [B, ceil(S / 128)] padded tokens of every 128; null with spans
   const float* slopes;  // [Hq]
-  __nv_bfloat16* out_lo;  // what rounding the output to bf16 left over, laid out like it; null: not kept.  D = rowsum(dO * O) wants it:
-                          // over documents of 2 to 20 tokens the rounding of O puts dQ and dK 0.5 to 0.33 % off, 0.25 % without it
+  __nv_bfloat16* out_lo;  // forward: what rounding the output to bf16 left over, laid out like it; null: not kept.  D = rowsum(dO * O) wants
+                          // it: over documents of 2 to 20 tokens the rounding of O puts dQ and dK 0.5 to 0.33 % off, 0.25 % without it
   float cap_log2;       // cap * log2(e)
   float cap_exp;        // 2 log2(e) scale / cap: tanh of a raw product s is 1 - 2 / (1 + 2^(s * cap_exp))
   float poly_max;       // |s| up to here: cap_log2 * tanh(s * scale / cap) = s * (poly[0] + poly[1] s^2 + ...)
