@@ -51,16 +51,17 @@ YF_DEVINL float capped_any(float s, const AttnMods& m) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(s * m.cap_exp)));
   return fabsf(s) <= m.poly_max ? capped_small(s, m) : fmaf(-2.f * m.cap_log2, r, m.cap_log2);
 }
-// 32 scores in place.  What becomes of a score does not depend on its neighbours.
-YF_DEVINL void cap_scores(uint32_t (&s)[32], const AttnMods& m) {
+// N scores in place.  What becomes of a score does not depend on its neighbours.
+template <int N>
+YF_DEVINL void cap_scores(uint32_t (&s)[N], const AttnMods& m) {
   float far = 0.f;
 #pragma unroll
-  for (int t = 0; t < 32; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
+  for (int t = 0; t < N; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
   if (far <= m.poly_max) {
     const uint64_t p0 = f32x2(m.poly[0], m.poly[0]), p1 = f32x2(m.poly[1], m.poly[1]), p2 = f32x2(m.poly[2], m.poly[2]),
                    p3 = f32x2(m.poly[3], m.poly[3]);
 #pragma unroll
-    for (int t = 0; t < 32; t += 2) {  // capped_small, two at a time
+    for (int t = 0; t < N; t += 2) {  // capped_small, two at a time
       const uint64_t x = f32x2(__uint_as_float(s[t]), __uint_as_float(s[t + 1])), z = mul_f32x2(x, x);
       const float2 y = f32x2_split(mul_f32x2(x, fma_f32x2(fma_f32x2(fma_f32x2(p3, z, p2), z, p1), z, p0)));
       s[t] = __float_as_uint(y.x);
@@ -68,7 +69,7 @@ YF_DEVINL void cap_scores(uint32_t (&s)[32], const AttnMods& m) {
     }
   } else {
 #pragma unroll
-    for (int t = 0; t < 32; ++t) s[t] = __float_as_uint(capped_any(__uint_as_float(s[t]), m));
+    for (int t = 0; t < N; ++t) s[t] = __float_as_uint(capped_any(__uint_as_float(s[t]), m));
   }
 }
 

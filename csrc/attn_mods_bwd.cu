@@ -15,7 +15,7 @@
 //   warps 21, 22     MMA issuers: the gradients of a step; S^T and dP^T of the step after next, into the columns that those leave
 //   warp 23          the query rows' statistics for the ring, read one step ahead; clears padded rows of tiles that have some
 // TMEM (512 columns): dV, dK (128 each) and two sets (even / odd steps) of [S^T | dP^T], 64 columns each: P^T and dS^T
-// (bf16, 16 + 16 columns per 32 queries) replace S^T once it has been read, dQ^T replaces dP^T.  So the softmax of one step runs under
+// (bf16, 8 + 8 columns per 16 queries) replace S^T once it has been read, dQ^T replaces dP^T.  So the softmax of one step runs under
 // the MMAs of its neighbours.  Bound: about 1700 cycles of MMA per step (S^T, dP^T and dQ^T with N = 64 are limited by the
 // 128 bytes per cycle that shared memory delivers: 48 instead of 32 cycles per instruction).
 // D = rowsum(dO * O) comes from a small pre-pass; scale and bf16 of dQ are applied by a post-pass, of dK at the end.
@@ -227,10 +227,10 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         const uint64_t q = mQ + (uint32_t)(st * (2 * QTILE >> 4));
 #pragma unroll
         for (int e = 0; e < BQ / 16; ++e)  // 16 queries: 8 TMEM columns of P^T, 16 rows of dO
-          tc_mma_bf16_ts(tdV, t + (e >> 1) * 32 + (e & 1) * 8, q + ((QTILE + e * 2048) >> 4), id_g, (it | e) != 0);
+          tc_mma_bf16_ts(tdV, t + e * 16, q + ((QTILE + e * 2048) >> 4), id_g, (it | e) != 0);
 #pragma unroll
         for (int e = 0; e < BQ / 16; ++e)
-          tc_mma_bf16_ts(tdK, t + (e >> 1) * 32 + 16 + (e & 1) * 8, q + (e * 2048 >> 4), id_g, (it | e) != 0);
+          tc_mma_bf16_ts(tdK, t + e * 16 + 8, q + (e * 2048 >> 4), id_g, (it | e) != 0);
         tc_commit(&vk_done[p]);
         tc_commit(&q_empty[st]);
         if (++st == STAGES) st = 0;
@@ -287,52 +287,52 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       const bool any_hidden = __any_sync(0xffffffffu, q0 < span.x || q0 + 32 > span.y);
       const uint32_t seen = bit_range(span.x - q0, span.y - q0);
       const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h0 + it / per_head) * LOG2E : 0.f;
-      const float far = (float)(q0 - key);
-      uint32_t s[32], dp[16], pk[16], dk[16];
-      tmem_ld32(t, s);
-      tmem_ld16(t + 64, dp);
-      tmem_ld_wait();
-      if (MODS & MOD_CAP) cap_scores(s, args.mods);
+      // 16 queries at a time, so that everything stays in registers: a spill goes to the L2, as shared memory leaves no L1
 #pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        if (v == 4) {  // dP^T in two parts, for want of registers
-          tmem_ld16(t + 64 + 16, dp);
-          tmem_ld_wait();
-        }
-        const float4 nl4 = stat[v], dl4 = stat[BQ / 4 + v];
-        const float nl[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, dl[4] = {dl4.x, dl4.y, dl4.z, dl4.w};
-        float x[4], g[4];
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[16], dp[16], pk[8], dk[8];
+        tmem_ld16(t + c * 16, s);
+        tmem_ld16(t + 64 + c * 16, dp);
+        tmem_ld_wait();
+        if (MODS & MOD_CAP) cap_scores(s, args.mods);
+        const float far = (float)(q0 + c * 16 - key);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y = __uint_as_float(s[4 * v + e]);
-          g[e] = __uint_as_float(dp[(4 * v + e) & 15]) - dl[e];
-          if (MODS & MOD_CAP) {
-            const float th = y * cap_inv;
-            g[e] *= fmaf(-th, th, 1.f);
-            y += nl[e];
-          } else {
-            y = fmaf(y, sl2, nl[e]);
+        for (int v = 0; v < 4; ++v) {
+          const float4 nl4 = stat[c * 4 + v], dl4 = stat[BQ / 4 + c * 4 + v];
+          const float nl[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, dl[4] = {dl4.x, dl4.y, dl4.z, dl4.w};
+          float x[4], g[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y = __uint_as_float(s[4 * v + e]);
+            g[e] = __uint_as_float(dp[4 * v + e]) - dl[e];
+            if (MODS & MOD_CAP) {
+              const float th = y * cap_inv;
+              g[e] *= fmaf(-th, th, 1.f);
+              y += nl[e];
+            } else {
+              y = fmaf(y, sl2, nl[e]);
+            }
+            if (MODS & MOD_BIAS) y = fmaf(-slope, fabsf(far + (float)(4 * v + e)), y);
+            x[e] = fast_exp2(y);
+            g[e] *= x[e];
           }
-          if (MODS & MOD_BIAS) y = fmaf(-slope, fabsf(far + (float)(4 * v + e)), y);
-          x[e] = fast_exp2(y);
-          g[e] *= x[e];
-        }
-        if (any_hidden) {
+          if (any_hidden) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!((seen >> (4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
+            for (int e = 0; e < 4; ++e)
+              if (!((seen >> (c * 16 + 4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
+          }
+          pk[2 * v] = pack_bf16x2(x[0], x[1]);
+          pk[2 * v + 1] = pack_bf16x2(x[2], x[3]);
+          dk[2 * v] = pack_bf16x2(g[0], g[1]);
+          dk[2 * v + 1] = pack_bf16x2(g[2], g[3]);
         }
-        pk[2 * v] = pack_bf16x2(x[0], x[1]);
-        pk[2 * v + 1] = pack_bf16x2(x[2], x[3]);
-        dk[2 * v] = pack_bf16x2(g[0], g[1]);
-        dk[2 * v + 1] = pack_bf16x2(g[2], g[3]);
+        // over the part of S^T that this thread has read: P^T, then dS^T
+        tmem_st8(t + c * 16, pk);
+        tmem_st8(t + c * 16 + 8, dk);
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+          *reinterpret_cast<uint4*>(ds_row + (((half * 4 + c * 2 + v) ^ (row & 7)) << 4)) = make_uint4(dk[4 * v], dk[4 * v + 1], dk[4 * v + 2], dk[4 * v + 3]);
       }
-      // over the part of S^T that this thread has read: P^T, then dS^T
-      tmem_st16(t, pk);
-      tmem_st16(t + 16, dk);
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-        *reinterpret_cast<uint4*>(ds_row + (((half * 4 + v) ^ (row & 7)) << 4)) = make_uint4(dk[4 * v], dk[4 * v + 1], dk[4 * v + 2], dk[4 * v + 3]);
       tmem_st_wait();
       fence_proxy_async_smem();
       tc_fence_before();
@@ -400,21 +400,21 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       if (!__all_sync(0xffffffffu, mbar_wait(&dq_full[p], (it >> 1) & 1, 530))) break;
       tc_fence_after();
       const uint32_t t = tmem_base + ((uint32_t)(w * 32) << 16) + p * 128 + 64;
-      uint32_t r[2][32];
-      tmem_ld32(t, r[0]);
-      tmem_ld32(t + 32, r[1]);
-      tmem_ld_wait();
-      tc_fence_before();
+      if (lane == 0) tma_store_wait_read0();  // the reduce of the step before has finished reading the block
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&dq_read[p]);
-        tma_store_wait_read0();  // the reduce of the step before has finished reading the block
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t r[32];
+        tmem_ld32(t + c * 32, r);
+        tmem_ld_wait();
+        if (c == 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&dq_read[p]);
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) stg[(c * 32 + e) * 32 + lane] = __uint_as_float(r[e]);
       }
-      __syncwarp();
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) stg[(c * 32 + e) * 32 + lane] = __uint_as_float(r[c][e]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
