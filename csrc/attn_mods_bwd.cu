@@ -285,11 +285,11 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       const float4* stat = reinterpret_cast<const float4*>(sStat + st * STAT_FLOATS) + half * 8;
       // the queries of the 32 that see this key
       const bool any_hidden = __any_sync(0xffffffffu, q0 < span.x || q0 + 32 > span.y);
-      const uint32_t seen = bit_range(span.x - q0, span.y - q0);
+      uint32_t seen = bit_range(span.x - q0, span.y - q0);
       const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h0 + it / per_head) * LOG2E : 0.f;
       // 16 queries at a time, so that everything stays in registers: a spill goes to the L2, as shared memory leaves no L1
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c, seen >>= 16) {
         uint32_t s[16], dp[16], pk[8], dk[8];
         tmem_ld16(t + c * 16, s);
         tmem_ld16(t + 64 + c * 16, dp);
@@ -319,7 +319,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           if (any_hidden) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (!((seen >> (c * 16 + 4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
+              if (!((seen >> (4 * v + e)) & 1u)) x[e] = g[e] = 0.f;
           }
           pk[2 * v] = pack_bf16x2(x[0], x[1]);
           pk[2 * v + 1] = pack_bf16x2(x[2], x[3]);
