@@ -73,6 +73,28 @@ YF_DEVINL void cap_scores(uint32_t (&s)[N], const AttnMods& m) {
   }
 }
 
+// N scores in place: s[e] = s[e] * scale - slope |d0 + e|.  `side`: 1 or -1 where d0 + e has that sign for all scores that count (those of the other
+// sign are hidden anyway), 0 where both do (prefixes).  The distances are whole numbers and stay exact.
+template <int N>
+YF_DEVINL void add_bias(uint32_t (&s)[N], float scale, float slope, float d0, int side) {
+  const uint64_t scale2 = f32x2(scale, scale);
+  if (side != 0) {
+    const float f = side > 0 ? -slope : slope;
+    const uint64_t f2 = f32x2(f, f), two = f32x2(2.f, 2.f);
+    uint64_t d = f32x2(d0, d0 + 1.f);
+#pragma unroll
+    for (int t = 0; t < N; t += 2) {
+      const float2 y = f32x2_split(fma_f32x2(d, f2, mul_f32x2(f32x2(__uint_as_float(s[t]), __uint_as_float(s[t + 1])), scale2)));
+      d = add_f32x2(d, two);
+      s[t] = __float_as_uint(y.x);
+      s[t + 1] = __float_as_uint(y.y);
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < N; ++t) s[t] = __float_as_uint(fmaf(-slope, fabsf(d0 + (float)t), __uint_as_float(s[t]) * scale));
+  }
+}
+
 // bits [from, to) of a word, for ends anywhere
 YF_DEVINL uint32_t bit_range(int from, int to) {
   const uint32_t below_to = to >= 32 ? 0xffffffffu : to <= 0 ? 0u : (1u << to) - 1u;

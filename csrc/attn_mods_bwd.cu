@@ -36,7 +36,7 @@ constexpr int STAGES = 3;          // ring of Q, dO and statistics
 constexpr int BWD_THREADS = 768;
 constexpr int DS_BYTES = ATOM;     // dS^T of a step: [128 keys x 64 queries] bf16
 constexpr int DQ_BYTES = BQ * HD * 4;
-constexpr int STAT_FLOATS = 2 * BQ;  // per stage: -lse * log2(e), D
+constexpr int STAT_FLOATS = 2 * BQ;  // per stage: -lse * log2(e), -D
 constexpr int BWD_SMEM = 1024 + 2 * TILE + STAGES * 2 * QTILE + 2 * DS_BYTES + DQ_BYTES + STAGES * STAT_FLOATS * 4 + 256;
 static_assert(BWD_SMEM <= 232448, "shared memory of one CTA");
 constexpr float LOG2E = 1.4426950408889634f;
@@ -189,7 +189,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         stat[lane + 32 * e] = nl[e];
-        stat[BQ + lane + 32 * e] = dl[e];
+        stat[BQ + lane + 32 * e] = -dl[e];
       }
       if (!__all_sync(0xffffffffu, mbar_wait(&q_land[st], ph ^ 1, 503))) break;
       const int q0 = (i_start + i) * BQ;
@@ -274,7 +274,8 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     uint8_t* ds_row = sdS + p * DS_BYTES + row * 128;
     int2 span = make_int2(key, args.S);       // queries [x, y) that see this key
     if (spans != nullptr || key >= args.S) span = key < args.S ? __ldg(spans + key) : make_int2(0, 0);
-    const float cap_inv = (MODS & MOD_CAP) ? 1.f / args.mods.cap_log2 : 0.f;
+    const float cap_sq = (MODS & MOD_CAP) ? -1.f / (args.mods.cap_log2 * args.mods.cap_log2) : 0.f;
+    int h = h0 + (n_it == 0 ? 0 : p / per_head);
     bool alive = true;
     int st = p, ph = 0, i = n_it == 0 ? 0 : p % per_head;  // ring stage and its parity, query tile of step p
     for (int it = p; it < n_it; it += 2) {
@@ -286,7 +287,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       // the queries of the 32 that see this key
       const bool any_hidden = __any_sync(0xffffffffu, q0 < span.x || q0 + 32 > span.y);
       uint32_t seen = bit_range(span.x - q0, span.y - q0);
-      const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h0 + it / per_head) * LOG2E : 0.f;
+      const float slope = (MODS & MOD_BIAS) ? __ldg(args.mods.slopes + h) * LOG2E : 0.f;
       // 16 queries at a time, so that everything stays in registers: a spill goes to the L2, as shared memory leaves no L1
 #pragma unroll 1
       for (int c = 0; c < 2; ++c, seen >>= 16) {
@@ -295,26 +296,34 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         tmem_ld16(t + 64 + c * 16, dp);
         tmem_ld_wait();
         if (MODS & MOD_CAP) cap_scores(s, args.mods);
-        const float far = (float)(q0 + c * 16 - key);
+        const uint64_t one = f32x2(1.f, 1.f), cap2 = f32x2(cap_sq, cap_sq);
+        uint64_t slopes2[8];  // 1 - tanh^2
+        if (MODS & MOD_CAP) {
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const uint64_t y = f32x2(__uint_as_float(s[2 * v]), __uint_as_float(s[2 * v + 1]));
+            slopes2[v] = fma_f32x2(mul_f32x2(y, y), cap2, one);
+          }
+        }
+        if (MODS & MOD_BIAS) add_bias(s, (MODS & MOD_CAP) ? 1.f : sl2, slope, (float)(q0 + c * 16 - key), span.x < key ? 0 : 1);
+        const float m = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
+        const uint64_t m2 = f32x2(m, m);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float4 nl4 = stat[c * 4 + v], dl4 = stat[BQ / 4 + c * 4 + v];
-          const float nl[4] = {nl4.x, nl4.y, nl4.z, nl4.w}, dl[4] = {dl4.x, dl4.y, dl4.z, dl4.w};
+          const float4 nl = stat[c * 4 + v], nd = stat[BQ / 4 + c * 4 + v];
           float x[4], g[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = __uint_as_float(s[4 * v + e]);
-            g[e] = __uint_as_float(dp[4 * v + e]) - dl[e];
-            if (MODS & MOD_CAP) {
-              const float th = y * cap_inv;
-              g[e] *= fmaf(-th, th, 1.f);
-              y += nl[e];
-            } else {
-              y = fmaf(y, sl2, nl[e]);
-            }
-            if (MODS & MOD_BIAS) y = fmaf(-slope, fabsf(far + (float)(4 * v + e)), y);
-            x[e] = fast_exp2(y);
-            g[e] *= x[e];
+          for (int e = 0; e < 2; ++e) {
+            const uint64_t n2 = e == 0 ? f32x2(nl.x, nl.y) : f32x2(nl.z, nl.w), d2 = e == 0 ? f32x2(nd.x, nd.y) : f32x2(nd.z, nd.w);
+            const int at = 4 * v + 2 * e;
+            const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), m2, n2));
+            x[2 * e] = fast_exp2(y.x);
+            x[2 * e + 1] = fast_exp2(y.y);
+            uint64_t z = mul_f32x2(add_f32x2(f32x2(__uint_as_float(dp[at]), __uint_as_float(dp[at + 1])), d2), f32x2(x[2 * e], x[2 * e + 1]));
+            if (MODS & MOD_CAP) z = mul_f32x2(z, slopes2[2 * v + e]);
+            const float2 w = f32x2_split(z);
+            g[2 * e] = w.x;
+            g[2 * e + 1] = w.y;
           }
           if (any_hidden) {
 #pragma unroll
@@ -339,7 +348,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       __syncwarp();
       if (lane == 0) mbar_arrive(&pds_ready[p]);
       i += 2;
-      while (i >= per_head) i -= per_head;
+      while (i >= per_head) { i -= per_head; ++h; }
       st += 2;
       if (st >= STAGES) { st -= STAGES; ph ^= 1; }
     }

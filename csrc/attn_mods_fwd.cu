@@ -282,14 +282,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         *gone = t + 1;
       }
       if (MODS & MOD_CAP) cap_scores(sc, args.mods);
-      if (MODS & MOD_BIAS) {
-        const float far = (float)(kv0 - qrow);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float x = __uint_as_float(sc[e]);
-          sc[e] = __float_as_uint(fmaf(-slope, fabsf(far + (float)e), (MODS & MOD_CAP) ? x : x * sl2));
-        }
-      }
+      if (MODS & MOD_BIAS) add_bias(sc, (MODS & MOD_CAP) ? 1.f : sl2, slope, (float)(kv0 - qrow), span.y > qrow + 1 ? 0 : -1);
       if (kv0 < span.x || kv0 + 32 > span.y) {  // the ends of a row's range
         const uint32_t seen = bit_range(span.x - kv0, span.y - kv0);
 #pragma unroll
