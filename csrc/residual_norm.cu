@@ -12,29 +12,48 @@
 #include "vec8.cuh"
 #include "yafsdp_b200.h"
 
+YF_TU_STATUS()
+
 namespace {
 
 constexpr int NV = 2;  // vectors of 8 per thread: TPR threads hold a row of up to 16 TPR elements
 
+// TPR threads take a row at a time, a block of at least 256 threads as many rows as that makes.  Every row group has a ring of shared memory into
+// which bulk copies bring its next rows while it works on one, so that the memory is busy during the two reductions of a row, and the
+// registers hold one row only.
 template <int TPR>
 constexpr int BLOCK = TPR < 256 ? 256 : TPR;
-
-// sum over the TPR threads of a row.  `slots`: one float per warp of the block, not used again before the row's threads have met at another
-// barrier.
 template <int TPR>
-YF_DEVINL float row_sum(float v, float* slots, int group) {
+constexpr int BLOCKS_PER_SM = TPR < 512 ? 2 : 1;
+constexpr int MAX_STAGES = 4;
+// rows that a group's ring holds: what leaves room for the L1 that the weights come from, and for the other block
+constexpr int RING_BYTES = 96 * 1024;  // of one block, two blocks per SM
+constexpr int RING_BYTES_ONE = 160 * 1024;
+template <int TPR>
+int ring_stages(int row_bytes) {
+  const int rows = BLOCK<TPR> / TPR, n = (BLOCKS_PER_SM<TPR> == 2 ? RING_BYTES : RING_BYTES_ONE) / (rows * row_bytes);
+  return n < 1 ? 1 : n > MAX_STAGES ? MAX_STAGES : n;
+}
+
+YF_DEVINL bool group_bar_or(int tpr, int group, bool flag) {
+  // literal barrier numbers: a computed one reserves all sixteen
+  if (group == 0) return named_bar_or(1, tpr, flag);
+  if (group == 1) return named_bar_or(2, tpr, flag);
+  if (group == 2) return named_bar_or(3, tpr, flag);
+  return named_bar_or(4, tpr, flag);
+}
+// sum over the TPR threads of a row; false when one of them says so.  `slots`: one float per warp of the block, not used again before the row's
+// threads have met at another barrier.
+template <int TPR>
+YF_DEVINL bool row_sum(float& v, float* slots, int group, bool ok = true) {
   v = warp_sum(v);
-  if (TPR == 32) return v;
+  if (TPR == 32) return __all_sync(0xffffffffu, ok);
   if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-  if (TPR >= 256) __syncthreads();
-  else if (group == 0) named_bar_sync(1, TPR);  // literal barrier numbers: a computed one reserves all sixteen
-  else if (group == 1) named_bar_sync(2, TPR);
-  else if (group == 2) named_bar_sync(3, TPR);
-  else named_bar_sync(4, TPR);
+  if (group_bar_or(TPR, group, !ok)) return false;
   v = 0.f;
 #pragma unroll
   for (int g = 0; g < TPR / 32; ++g) v += slots[group * (TPR / 32) + g];
-  return v;
+  return true;
 }
 
 struct NormArgs {
@@ -46,74 +65,132 @@ struct NormArgs {
   float *w_parts, *z_parts;  // [CTAs, D]: sums of dn hhat and of g yhat (g y without post; e yhat with a gate per token)
   float scale, eps;
   int T, D;
-  int group_rows;    // tokens that share a row of the gate (1: a gate per token)
+  int group_rows;    // tokens that share a row of the gate
   int ctas_per_group;
+  int token_gate;    // a row of the gate for every token
+  int stages;
+};
+
+// The ring of a row group: `tensors` rows of D elements side by side in each stage.
+template <typename T, int TPR>
+struct Ring {
+  uint8_t* base;
+  uint64_t* full;
+  const void* src[5];
+  int tensors, row_bytes, stages;
+  int stage, phase;
+
+  YF_DEVINL void start(uint8_t* smem, uint64_t* bars, int group, int n_stages, int n_tensors, int D) {
+    tensors = n_tensors;
+    row_bytes = D * (int)sizeof(T);
+    stages = n_stages;
+    base = smem + (size_t)group * stages * tensors * row_bytes;
+    full = bars + group * MAX_STAGES;
+    stage = phase = 0;
+  }
+  // one thread: row `row` of every tensor into stage s
+  YF_DEVINL void fetch(int s, long long row) {
+    mbar_expect_tx(&full[s], (uint32_t)(tensors * row_bytes));
+#pragma unroll
+    for (int t = 0; t < 5; ++t)
+      if (t < tensors)
+        bulk_load(base + (size_t)(s * tensors + t) * row_bytes, reinterpret_cast<const uint8_t*>(src[t]) + row * row_bytes, (uint32_t)row_bytes, &full[s]);
+  }
+  YF_DEVINL const T* row(int t) const { return reinterpret_cast<const T*>(base + (size_t)(stage * tensors + t) * row_bytes); }
+  YF_DEVINL bool wait(int site) { return mbar_wait(&full[stage], phase, site); }
+  YF_DEVINL void next() {
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
 };
 
 template <typename T, int TPR>
-__global__ void __launch_bounds__(BLOCK<TPR>) residual_norm_fwd_kernel(NormArgs a) {
+__global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_fwd_kernel(NormArgs a) {
   constexpr int ROWS = BLOCK<TPR> / TPR;
-  __shared__ float slots[2][BLOCK<TPR> / 32];
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t bars[ROWS * MAX_STAGES];
+  __shared__ float slots[2][2][BLOCK<TPR> / 32];
   const int group = threadIdx.x / TPR, tr = threadIdx.x % TPR;
-  const int row = blockIdx.x * ROWS + group;
-  if (row >= a.T) return;
-  const long long at = (long long)row * a.D;
-  const T* x = reinterpret_cast<const T*>(a.x) + at;
-  const T* y = reinterpret_cast<const T*>(a.y) + at;
-  const T* gate = reinterpret_cast<const T*>(a.gate) + (a.gate ? (long long)(row / a.group_rows) * a.D : 0);
-  const T *post = reinterpret_cast<const T*>(a.post), *w = reinterpret_cast<const T*>(a.weight);
   const int nvec = a.D / 8;
-  float h[NV][8], u[NV][8];
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = tr + TPR * i;
-    if (v < nvec) {
-      load_f8<T>(x + v * 8, h[i]);
-      load_f8<T>(y + v * 8, u[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss += u[i][j] * u[i][j];
-    }
+  const int first = blockIdx.x * ROWS + group, step = gridDim.x * ROWS;
+  Ring<T, TPR> ring;
+  ring.start(smem, bars, group, a.stages, a.token_gate ? 3 : 2, a.D);
+  ring.src[0] = a.x;
+  ring.src[1] = a.y;
+  ring.src[2] = a.gate;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ROWS * MAX_STAGES; ++i) mbar_init(&bars[i], 1);
+    mbar_fence_init();
   }
-  float ry = 1.f;
-  if (a.post) ry = rsqrtf(row_sum<TPR>(ss, slots[0], group) / (float)a.D + a.eps);
-  ss = 0.f;
+  __syncthreads();
+  if (tr == 0)
+    for (int s = 0; s < a.stages; ++s)
+      if (first + s * step < a.T) ring.fetch(s, first + s * step);
+  const T *post = reinterpret_cast<const T*>(a.post), *w = reinterpret_cast<const T*>(a.weight);
+  int parity = 0;
+  for (int row = first; row < a.T; row += step, parity ^= 1) {
+    const long long at = (long long)row * a.D;
+    // a wait that runs out ends the work of the row's threads together
+    const bool ok = ring.wait(600);
+    const T *x = ring.row(0), *y = ring.row(1);
+    const T* gate = a.token_gate ? ring.row(2) : reinterpret_cast<const T*>(a.gate) + (a.gate ? (long long)(row / a.group_rows) * a.D : 0);
+    float h[NV][8], u[NV][8], s[NV][8];
+    float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = tr + TPR * i;
-    if (v < nvec) {
-      float f[8], s[8];
+    for (int i = 0; i < NV; ++i) {
+      const int v = tr + TPR * i;
+      if (v < nvec) {
+        load_f8<T>(x + v * 8, h[i]);
+        load_f8<T>(y + v * 8, u[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = a.scale;
-      if (a.gate) {
-        load_f8<T>(gate + v * 8, f);
+        for (int j = 0; j < 8; ++j) {
+          ss += u[i][j] * u[i][j];
+          s[i][j] = a.scale;
+        }
+        if (a.gate) {
+          float f[8];
+          load_f8<T>(gate + v * 8, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] *= f[j];
+          for (int j = 0; j < 8; ++j) s[i][j] *= f[j];
+        }
       }
-      if (a.post) {
-        load_f8<T>(post + v * 8, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[i][j] *= ry * f[j];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        h[i][j] += s[j] * u[i][j];
-        ss += h[i][j] * h[i][j];
-      }
-      store_f8<T>(reinterpret_cast<T*>(a.h) + at + v * 8, h[i]);
     }
-  }
-  const float rh = rsqrtf(row_sum<TPR>(ss, slots[1], group) / (float)a.D + a.eps);
-  if (tr == 0 && a.rstd) reinterpret_cast<float2*>(a.rstd)[row] = make_float2(ry, rh);
+    // behind this sum the row is in registers, and its stage is free
+    if (!row_sum<TPR>(ss, slots[0][parity], group, ok)) break;
+    if (tr == 0 && row + (long long)a.stages * step < a.T) ring.fetch(ring.stage, row + (long long)a.stages * step);
+    ring.next();
+    const float ry = a.post ? rsqrtf(ss / (float)a.D + a.eps) : 1.f;
+    ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = tr + TPR * i;
-    if (v < nvec) {
-      float f[8];
-      load_f8<T>(w + v * 8, f);
+    for (int i = 0; i < NV; ++i) {
+      const int v = tr + TPR * i;
+      if (v < nvec) {
+        if (a.post) {
+          float f[8];
+          load_f8<T>(post + v * 8, f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= h[i][j] * rh;
-      store_f8<T>(reinterpret_cast<T*>(a.n) + at + v * 8, f);
+          for (int j = 0; j < 8; ++j) u[i][j] *= ry * f[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          h[i][j] += s[i][j] * u[i][j];
+          ss += h[i][j] * h[i][j];
+        }
+        store_f8<T>(reinterpret_cast<T*>(a.h) + at + v * 8, h[i]);
+      }
+    }
+    row_sum<TPR>(ss, slots[1][parity], group);
+    const float rh = rsqrtf(ss / (float)a.D + a.eps);
+    if (tr == 0 && a.rstd) reinterpret_cast<float2*>(a.rstd)[row] = make_float2(ry, rh);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int v = tr + TPR * i;
+      if (v < nvec) {
+        float f[8];
+        load_f8<T>(w + v * 8, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= h[i][j] * rh;
+        store_f8<T>(reinterpret_cast<T*>(a.n) + at + v * 8, f);
+      }
     }
   }
 }
@@ -121,109 +198,148 @@ __global__ void __launch_bounds__(BLOCK<TPR>) residual_norm_fwd_kernel(NormArgs 
 // A CTA walks over the rows of one group of tokens (all tokens where the gate is per token); its threads hold the same columns of every
 // row and sum the parameters' gradients in registers on the way.
 template <typename T, int TPR, bool TOKEN_GATE>
-__global__ void __launch_bounds__(BLOCK<TPR>) residual_norm_bwd_kernel(NormArgs a) {
+__global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_bwd_kernel(NormArgs a) {
   constexpr int THREADS = BLOCK<TPR>, ROWS = THREADS / TPR;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t bars[ROWS * MAX_STAGES];
   __shared__ float slots[2][2][THREADS / 32];
-  __shared__ float sums[ROWS > 1 ? TPR * NV * 8 : 1];
   const int group = threadIdx.x / TPR, tr = threadIdx.x % TPR;
   const int nvec = a.D / 8;
   const int part = blockIdx.x % a.ctas_per_group, gg = blockIdx.x / a.ctas_per_group;
   const int rows = TOKEN_GATE ? a.T : a.group_rows;
+  const int first = part * ROWS + group, step = a.ctas_per_group * ROWS;
+  const long long row0 = (long long)gg * rows;
   const float inv_d = 1.f / (float)a.D;
   const T *post = reinterpret_cast<const T*>(a.post), *w = reinterpret_cast<const T*>(a.weight);
-  const T* gate = reinterpret_cast<const T*>(a.gate) + (a.gate && !TOKEN_GATE ? (long long)gg * a.D : 0);
+  Ring<T, TPR> ring;
+  {
+    int n = 0;
+    ring.src[n++] = a.x;
+    ring.src[n++] = a.y;
+    if (a.dh) ring.src[n++] = a.dh;
+    if (a.dn) ring.src[n++] = a.dn;
+    if (TOKEN_GATE) ring.src[n++] = a.gate;
+    ring.start(smem, bars, group, a.stages, n, a.D);
+  }
+  const int at_dn = a.dh ? 3 : 2, at_gate = at_dn + (a.dn ? 1 : 0);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ROWS * MAX_STAGES; ++i) mbar_init(&bars[i], 1);
+    mbar_fence_init();
+  }
+  __syncthreads();
+  if (tr == 0)
+    for (int s = 0; s < a.stages; ++s)
+      if (first + s * step < rows) ring.fetch(s, row0 + first + s * step);
   float acc_w[NV][8], acc_z[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc_w[i][j] = acc_z[i][j] = 0.f;
   int parity = 0;
-  for (int r = part * ROWS + group; r < rows; r += a.ctas_per_group * ROWS, parity ^= 1) {
-    const long long row = (long long)gg * rows + r, at = row * a.D;
-    const T *x = reinterpret_cast<const T*>(a.x) + at, *y = reinterpret_cast<const T*>(a.y) + at;
-    const T *dh = reinterpret_cast<const T*>(a.dh) + (a.dh ? at : 0), *dn = reinterpret_cast<const T*>(a.dn) + (a.dn ? at : 0);
-    const T* gr = gate + (TOKEN_GATE ? at : 0);
+  for (int r = first; r < rows; r += step, parity ^= 1) {
+    const long long row = row0 + r, at = row * a.D;
     const float2 rs = reinterpret_cast<const float2*>(a.rstd)[row];
     const float ry = rs.x, rh = rs.y;
-    float yv[NV][8], hv[NV][8], g[NV][8], cv[NV][8], s[NV][8];
+    const bool ok = ring.wait(601);
+    Raw8<T> yr[NV], dhr[NV], gr[NV];
+    float hv[NV][8], cv[NV][8];
     float dot = 0.f;
+    // s = scale * gate of eight elements
+    auto factor = [&](int i, int v, float(&s)[8]) {
+      if (TOKEN_GATE) unpack_raw8<T>(gr[i], s);
+      else if (a.gate) load_f8<T>(reinterpret_cast<const T*>(a.gate) + (long long)gg * a.D + v * 8, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = a.gate ? s[j] * a.scale : a.scale;
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
-        float f[8];
-        load_f8<T>(x + v * 8, hv[i]);
-        load_f8<T>(y + v * 8, yv[i]);
+        yr[i] = load_raw8<T>(ring.row(1) + v * 8);
+        if (a.dh) dhr[i] = load_raw8<T>(ring.row(2) + v * 8);
+        if (TOKEN_GATE) gr[i] = load_raw8<T>(ring.row(at_gate) + v * 8);
+        float f[8], s[8], yv[8];
+        load_f8<T>(ring.row(0) + v * 8, hv[i]);
+        unpack_raw8<T>(yr[i], yv);
+        factor(i, v, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] *= yv[j] * ry;
+        if (a.post) {
+          load_f8<T>(post + v * 8, f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[j] *= f[j];
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          yv[i][j] *= ry;  // yhat (y itself without post)
-          s[i][j] = a.scale;
-          g[i][j] = cv[i][j] = 0.f;
+          hv[i][j] = (hv[i][j] + s[j]) * rh;  // hhat
+          cv[i][j] = 0.f;
         }
-        if (a.gate) {
-          load_f8<T>(gr + v * 8, f);
+        if (a.dn) {
+          load_f8<T>(ring.row(at_dn) + v * 8, cv[i]);
+          load_f8<T>(w + v * 8, f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) s[i][j] *= f[j];
-        }
-        if (a.dh) load_f8<T>(dh + v * 8, g[i]);
-        if (a.dn) load_f8<T>(dn + v * 8, cv[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 1.f;
-        if (a.post) load_f8<T>(post + v * 8, f);
-        float wf[8];
-        load_f8<T>(w + v * 8, wf);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          hv[i][j] = (hv[i][j] + s[i][j] * (yv[i][j] * f[j])) * rh;  // hhat
-          acc_w[i][j] += cv[i][j] * hv[i][j];
-          cv[i][j] *= wf[j];
-          dot += cv[i][j] * hv[i][j];
+          for (int j = 0; j < 8; ++j) {
+            acc_w[i][j] += cv[i][j] * hv[i][j];
+            cv[i][j] *= f[j];
+            dot += cv[i][j] * hv[i][j];
+          }
         }
       }
     }
-    dot = row_sum<TPR>(dot, slots[0][parity], group) * inv_d;
+    // behind this sum the row is in registers, and its stage is free
+    if (!row_sum<TPR>(dot, slots[0][parity], group, ok)) break;
+    if (tr == 0 && r + (long long)a.stages * step < rows) ring.fetch(ring.stage, row + (long long)a.stages * step);
+    ring.next();
+    dot *= inv_d;
     float dot2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
-        float f[8];
+        float g[8], f[8], s[8], yv[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          g[i][j] += rh * (cv[i][j] - hv[i][j] * dot);
+          g[j] = 0.f;
           f[j] = 1.f;
         }
-        store_f8<T>(reinterpret_cast<T*>(a.dx) + at + v * 8, g[i]);
+        if (a.dh) unpack_raw8<T>(dhr[i], g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += rh * (cv[i][j] - hv[i][j] * dot);
+        store_f8<T>(reinterpret_cast<T*>(a.dx) + at + v * 8, g);
         if (a.post) load_f8<T>(post + v * 8, f);
+        unpack_raw8<T>(yr[i], yv);
+        factor(i, v, s);
         float dg[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float gy = g[i][j] * yv[i][j];
+          hv[i][j] = yv[j] * ry;  // yhat (y itself without post)
+          const float gy = g[j] * hv[i][j];
           if (TOKEN_GATE) {
             dg[j] = a.scale * gy * f[j];
-            acc_z[i][j] += s[i][j] * gy;
+            acc_z[i][j] += s[j] * gy;
           } else {
             acc_z[i][j] += gy;
           }
-          cv[i][j] = s[i][j] * g[i][j] * f[j];  // e post
-          dot2 += cv[i][j] * yv[i][j];
+          cv[i][j] = s[j] * g[j] * f[j];  // e post
+          dot2 += cv[i][j] * hv[i][j];
         }
         if (TOKEN_GATE) store_f8<T>(reinterpret_cast<T*>(a.dgate) + at + v * 8, dg);
       }
     }
-    if (a.post) dot2 = row_sum<TPR>(dot2, slots[1][parity], group) * inv_d;
-    else dot2 = 0.f;
+    if (a.post) row_sum<TPR>(dot2, slots[1][parity], group);
+    dot2 = a.post ? dot2 * inv_d : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
         float o[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = ry * (cv[i][j] - yv[i][j] * dot2);
+        for (int j = 0; j < 8; ++j) o[j] = ry * (cv[i][j] - hv[i][j] * dot2);
         store_f8<T>(reinterpret_cast<T*>(a.dy) + at + v * 8, o);
       }
     }
   }
+  float* sums = reinterpret_cast<float*>(smem);  // ROWS > 1: every row has been read by now
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     float* parts = k == 0 ? a.w_parts : a.z_parts;
@@ -348,44 +464,72 @@ int row_threads(int D) {  // threads that hold a row: 16 elements each
   while (t * NV * 8 < D) t *= 2;
   return t;
 }
-// CTAs that walk over one group of tokens: two per SM altogether, no more than there are rows for
+int blocks_per_sm(int D) { return row_threads(D) < 512 ? 2 : 1; }
+int rows_per_block(int D) { return row_threads(D) < 256 ? 256 / row_threads(D) : 1; }
+// CTAs that walk over one group of tokens: what is resident altogether, no more than there are rows for
 int ctas_per_group(int T, int D, int groups) {
-  const int tpr = row_threads(D), rows = tpr < 256 ? 256 / tpr : 1, in_group = T / groups;
-  int want = (2 * yf_num_sms() + groups - 1) / groups;
+  const int rows = rows_per_block(D), in_group = T / groups;
+  int want = (blocks_per_sm(D) * yf_num_sms() + groups - 1) / groups;
   const int most = (in_group + rows - 1) / rows;
   if (want > most) want = most;
   return want < 1 ? 1 : want;
 }
 
+template <typename T, int N>
+int launch_rows(void (*kernel)(NormArgs), bool (&optin)[64], NormArgs a, int tensors, int grid, cudaStream_t st) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (!optin[dev]) {  // the shared-memory opt-in is a per-device attribute
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES_ONE);
+    if (e != cudaSuccess) return -(int)e;
+    optin[dev] = true;
+  }
+  if (int rc = yf_tu_bind_status()) return rc;
+  const int row_bytes = tensors * a.D * (int)sizeof(T), rows = BLOCK<N> / N;
+  a.stages = ring_stages<N>(row_bytes);
+  int bytes = a.stages * rows * row_bytes;
+  if (bytes < N * NV * 8 * 4) bytes = N * NV * 8 * 4;  // the sums of the row groups meet there
+  kernel<<<grid, BLOCK<N>, bytes, st>>>(a);
+  return -(int)cudaGetLastError();
+}
+template <typename T, int N>
+int fwd_launch_n(const NormArgs& a, cudaStream_t st) {
+  static bool optin[64] = {};
+  constexpr int rows = BLOCK<N> / N;
+  int grid = (a.T + rows - 1) / rows;
+  const int most = BLOCKS_PER_SM<N> * yf_num_sms();
+  if (grid > most) grid = most;
+  return launch_rows<T, N>(residual_norm_fwd_kernel<T, N>, optin, a, a.token_gate ? 3 : 2, grid, st);
+}
+template <typename T, int N>
+int bwd_launch_n(const NormArgs& a, int grid, cudaStream_t st) {
+  static bool optin[2][64] = {};
+  const int tensors = 2 + (a.dh ? 1 : 0) + (a.dn ? 1 : 0) + (a.token_gate ? 1 : 0);
+  return a.token_gate ? launch_rows<T, N>(residual_norm_bwd_kernel<T, N, true>, optin[1], a, tensors, grid, st)
+                      : launch_rows<T, N>(residual_norm_bwd_kernel<T, N, false>, optin[0], a, tensors, grid, st);
+}
 template <typename T>
 int fwd_launch(const NormArgs& a, cudaStream_t st) {
-  const int tpr = row_threads(a.D);
-#define YF_LAUNCH(N)                                                                                              \
-  case N: {                                                                                                       \
-    constexpr int rows = BLOCK<N> / N;                                                                  \
-    residual_norm_fwd_kernel<T, N><<<(a.T + rows - 1) / rows, BLOCK<N>, 0, st>>>(a);                    \
-    break;                                                                                                        \
+  switch (row_threads(a.D)) {
+    case 32: return fwd_launch_n<T, 32>(a, st);
+    case 64: return fwd_launch_n<T, 64>(a, st);
+    case 128: return fwd_launch_n<T, 128>(a, st);
+    case 256: return fwd_launch_n<T, 256>(a, st);
+    default: return fwd_launch_n<T, 512>(a, st);
   }
-  switch (tpr) {
-    YF_LAUNCH(32) YF_LAUNCH(64) YF_LAUNCH(128) YF_LAUNCH(256) YF_LAUNCH(512) YF_LAUNCH(1024)
-    default: return -1;
-  }
-#undef YF_LAUNCH
-  return -(int)cudaGetLastError();
 }
 template <typename T>
 int bwd_launch(const NormArgs& a, const ParamArgs& p, cudaStream_t st) {
-  const int tpr = row_threads(a.D), grid = p.groups * p.ctas_per_group;
-#define YF_LAUNCH(N)                                                                                              \
-  case N:                                                                                                         \
-    if (p.token_gate) residual_norm_bwd_kernel<T, N, true><<<grid, BLOCK<N>, 0, st>>>(a);               \
-    else residual_norm_bwd_kernel<T, N, false><<<grid, BLOCK<N>, 0, st>>>(a);                           \
-    break;
-  switch (tpr) {
-    YF_LAUNCH(32) YF_LAUNCH(64) YF_LAUNCH(128) YF_LAUNCH(256) YF_LAUNCH(512) YF_LAUNCH(1024)
-    default: return -1;
+  const int grid = p.groups * p.ctas_per_group;
+  int rc = 0;
+  switch (row_threads(a.D)) {
+    case 32: rc = bwd_launch_n<T, 32>(a, grid, st); break;
+    case 64: rc = bwd_launch_n<T, 64>(a, grid, st); break;
+    case 128: rc = bwd_launch_n<T, 128>(a, grid, st); break;
+    case 256: rc = bwd_launch_n<T, 256>(a, grid, st); break;
+    default: rc = bwd_launch_n<T, 512>(a, grid, st); break;
   }
-#undef YF_LAUNCH
+  if (rc) return rc;
   residual_norm_param_kernel<T><<<(a.D + 31) / 32, 1024, 0, st>>>(p);
   return -(int)cudaGetLastError();
 }
@@ -396,14 +540,14 @@ bool misaligned(const void* const* p, int n) {
   return (bits & 15) != 0;
 }
 bool bad_shape(int T, int D, int gate_rows, const void* gate, int dtype) {
-  if (T <= 0 || D <= 0 || D % 8 || D > 16384 || dtype < 0 || dtype > 2) return true;
+  if (T <= 0 || D <= 0 || D % 8 || D > 8192 || dtype < 0 || dtype > 2) return true;
   return gate != nullptr ? gate_rows <= 0 || T % gate_rows != 0 : gate_rows != 0;
 }
 
 }  // namespace
 
 // x, y, h, n: [T, D] without gaps; weight, post: [D]; gate: [gate_rows, D], row t / (T / gate_rows) for token t (gate_rows 0 without one); all
-// of one type (dtype 0 bf16, 1 fp16, 2 fp32), 16-byte aligned, D a multiple of 8 up to 16384.  rstd: [T, 2] fp32 for the backward
+// of one type (dtype 0 bf16, 1 fp16, 2 fp32), 16-byte aligned, D a multiple of 8 up to 8192.  rstd: [T, 2] fp32 for the backward
 // pass, or null. 
 extern "C" int yf_residual_norm_fwd(const void* x, const void* y, const void* weight, const void* post, const void* gate, int gate_rows, void* h,
                                     void* n, float* rstd, int T, int D, float scale, float eps, int dtype, void* stream) {
@@ -416,13 +560,14 @@ extern "C" int yf_residual_norm_fwd(const void* x, const void* y, const void* we
   a.T = T; a.D = D;
   a.scale = scale; a.eps = eps;
   a.group_rows = gate ? T / gate_rows : T;
+  a.token_gate = gate != nullptr && gate_rows == T;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == 0 ? fwd_launch<__nv_bfloat16>(a, st) : dtype == 1 ? fwd_launch<__half>(a, st) : fwd_launch<float>(a, st);
 }
 
 // Rows of [rows, D] fp32 scratch that the backward pass wants (twice that with a post norm or a gate).
 extern "C" int yf_residual_norm_parts(int T, int D, int gate_rows) {
-  if (T <= 0 || D <= 0 || D % 8 || D > 16384 || gate_rows < 0 || (gate_rows > 0 && T % gate_rows)) return -1;
+  if (T <= 0 || D <= 0 || D % 8 || D > 8192 || gate_rows < 0 || (gate_rows > 0 && T % gate_rows)) return -1;
   const int groups = gate_rows == 0 || gate_rows == T ? 1 : gate_rows;
   const long long n = (long long)groups * ctas_per_group(T, D, groups);
   return n > 0x7fffffff ? -1 : (int)n;
@@ -456,6 +601,7 @@ extern "C" int yf_residual_norm_bwd(const void* x, const void* y, const void* we
   a.scale = scale;
   a.group_rows = T / groups;
   a.ctas_per_group = per;
+  a.token_gate = token_gate ? 1 : 0;
   ParamArgs p = {};
   p.w_parts = a.w_parts; p.z_parts = a.z_parts;
   p.post = post; p.gate = gate;

@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 template <typename T>
@@ -48,4 +50,32 @@ YF_DEVINL void store_f8<__half>(__half* p, const float (&f)[8]) {
     w[i] = *reinterpret_cast<const uint32_t*>(&t);
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// eight elements as they lie in memory, and as floats
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T>
+YF_DEVINL Raw8<T> load_raw8(const void* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T>
+YF_DEVINL void unpack_raw8(const Raw8<T>& r, float (&f)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (sizeof(T) == 4) {
+      f[2 * i] = __uint_as_float(w[2 * i]);
+      f[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
+    } else {
+      const float2 t = std::is_same<T, __half>::value ? __half22float2(*reinterpret_cast<const __half2*>(w + i)) : unpack_bf16x2(w[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
 }

@@ -346,7 +346,7 @@ def _norm_check(x, y, w, post, gate, dh, dn, scale=0.7):
         oracle.close(got, want[name], name)
 
 
-@pytest.mark.parametrize("shape", [(1, 1, 8), (2, 3, 64), (3, 111, 512), (2, 45, 1000), (1, 200, 1368), (4, 30, 4096), (3, 50, 5120), (2, 33, 8192), (1, 5, 16384)])
+@pytest.mark.parametrize("shape", [(1, 1, 8), (2, 3, 64), (3, 111, 512), (2, 45, 1000), (1, 200, 1368), (4, 30, 4096), (3, 50, 5120), (2, 33, 8192), (1, 5, 8184)])
 @pytest.mark.parametrize("gate", ["none", "channel", "sample", "token"])
 @pytest.mark.parametrize("post", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
@@ -408,7 +408,7 @@ def test_refusals():
     with pytest.raises(ValueError):
         Fn.residual_norm(torch.ones(2, 12, device=DEV), torch.ones(2, 12, device=DEV), torch.ones(12, device=DEV))
     with pytest.raises(ValueError):
-        Fn.residual_norm(*[torch.ones(2, 16392, device=DEV)] * 2, torch.ones(16392, device=DEV))
+        Fn.residual_norm(*[torch.ones(2, 8200, device=DEV)] * 2, torch.ones(8200, device=DEV))
     with pytest.raises(ValueError):
         Fn.residual_norm(torch.ones(2, 16, device=DEV), torch.ones(2, 16), torch.ones(16, device=DEV))
     # the C entries refuse what the host can see
