@@ -16,22 +16,22 @@ YF_TU_STATUS()
 
 namespace {
 
-constexpr int NV = 2;  // vectors of 8 per thread: TPR threads hold a row of up to 16 TPR elements
-
-// TPR threads take a row at a time, a block of at least 256 threads as many rows as that makes.  Every row group has a ring of shared memory into
+// TPR threads take a row at a time (16 elements each, 32 in the forward pass of wide rows: two blocks of 256 threads overlap their reductions better
+// than one of 512), a block of at least 256 threads as many rows as that makes.  Every row group has a ring of shared memory into
 // which bulk copies bring its next rows while it works on one, so that the memory is busy during the two reductions of a row, and the
 // registers hold one row only.
 template <int TPR>
 constexpr int BLOCK = TPR < 256 ? 256 : TPR;
+template <int TPR, int NV>
+constexpr int FWD_BLOCKS = NV == 2 ? 3 : 2;  // per SM
 template <int TPR>
-constexpr int BLOCKS_PER_SM = TPR < 512 ? 2 : 1;
+constexpr int BWD_BLOCKS = TPR < 512 ? 2 : 1;
 constexpr int MAX_STAGES = 4;
-// rows that a group's ring holds: what leaves room for the L1 that the weights come from, and for the other block
-constexpr int RING_BYTES = 96 * 1024;  // of one block, two blocks per SM
-constexpr int RING_BYTES_ONE = 160 * 1024;
-template <int TPR>
-int ring_stages(int row_bytes) {
-  const int rows = BLOCK<TPR> / TPR, n = (BLOCKS_PER_SM<TPR> == 2 ? RING_BYTES : RING_BYTES_ONE) / (rows * row_bytes);
+// What the rings of an SM's blocks take together: 160 KB, which leaves room for the L1 that the weights come from, and more only for rows of which
+// not even one would fit.
+constexpr int RING_BYTES = 160 * 1024, RING_BYTES_MOST = 192 * 1024;
+int ring_stages(int stage_bytes, int blocks) {
+  const int n = RING_BYTES / blocks / stage_bytes;
   return n < 1 ? 1 : n > MAX_STAGES ? MAX_STAGES : n;
 }
 
@@ -62,7 +62,7 @@ struct NormArgs {
   float* rstd;  // [T, 2]: r_y (with post), r_h; may be null
   const void *dh, *dn;  // either may be null: zeros
   void *dx, *dy, *dgate;
-  float *w_parts, *z_parts;  // [CTAs, D]: sums of dn hhat and of g yhat (g y without post; e yhat with a gate per token)
+  float *w_parts, *z_parts;  // [CTAs, D]: sums of dn hhat and of g yhat (g y without post; gate g yhat with a gate per token)
   float scale, eps;
   int T, D;
   int group_rows;    // tokens that share a row of the gate
@@ -103,15 +103,31 @@ struct Ring {
   }
 };
 
-template <typename T, int TPR>
-__global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_fwd_kernel(NormArgs a) {
+// scale * gate * post of the thread's columns: what a normalised y is multiplied by, and one vector for what would be two
+template <typename T, int NV, int TPR>
+YF_DEVINL void factors(F8 (&f)[NV], float scale, const void* gate, const void* post, int tr, int nvec) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = tr + TPR * i;
+    f[i] = splat8(scale);
+    if (v < nvec) {
+      if (gate) f[i] = mul8(f[i], unpack8<T>(load_raw8<T>(reinterpret_cast<const T*>(gate) + v * 8)));
+      if (post) f[i] = mul8(f[i], unpack8<T>(load_raw8<T>(reinterpret_cast<const T*>(post) + v * 8)));
+    }
+  }
+}
+
+// A row group walks over adjacent rows, so that the gate's row seldom changes.
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(BLOCK<TPR>, FWD_BLOCKS<TPR, NV>) residual_norm_fwd_kernel(NormArgs a) {
   constexpr int ROWS = BLOCK<TPR> / TPR;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[ROWS * MAX_STAGES];
   __shared__ float slots[2][2][BLOCK<TPR> / 32];
   const int group = threadIdx.x / TPR, tr = threadIdx.x % TPR;
   const int nvec = a.D / 8;
-  const int first = blockIdx.x * ROWS + group, step = gridDim.x * ROWS;
+  const int walkers = gridDim.x * ROWS, each = (a.T + walkers - 1) / walkers;
+  const int first = min((long long)(blockIdx.x * ROWS + group) * each, (long long)a.T), end = min(first + each, a.T);
   Ring<T, TPR> ring;
   ring.start(smem, bars, group, a.stages, a.token_gate ? 3 : 2, a.D);
   ring.src[0] = a.x;
@@ -124,73 +140,62 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
   __syncthreads();
   if (tr == 0)
     for (int s = 0; s < a.stages; ++s)
-      if (first + s * step < a.T) ring.fetch(s, first + s * step);
-  const T *post = reinterpret_cast<const T*>(a.post), *w = reinterpret_cast<const T*>(a.weight);
+      if (first + s < end) ring.fetch(s, first + s);
+  const T *w = reinterpret_cast<const T*>(a.weight), *gate = reinterpret_cast<const T*>(a.gate);
+  int in_group = 0;  // rows until the gate's row changes
+  if (gate && !a.token_gate && first < end) {
+    gate += (long long)(first / a.group_rows) * a.D;
+    in_group = a.group_rows - first % a.group_rows;
+  }
+  F8 f[NV];
+  factors<T, NV, TPR>(f, a.scale, a.token_gate ? nullptr : gate, a.post, tr, nvec);
   int parity = 0;
-  for (int row = first; row < a.T; row += step, parity ^= 1) {
+  for (int row = first; row < end; ++row, parity ^= 1) {
     const long long at = (long long)row * a.D;
     // a wait that runs out ends the work of the row's threads together
     const bool ok = ring.wait(600);
     const T *x = ring.row(0), *y = ring.row(1);
-    const T* gate = a.token_gate ? ring.row(2) : reinterpret_cast<const T*>(a.gate) + (a.gate ? (long long)(row / a.group_rows) * a.D : 0);
-    float h[NV][8], u[NV][8], s[NV][8];
-    float ss = 0.f;
+    F8 h[NV], u[NV];
+    uint64_t ss = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
-        load_f8<T>(x + v * 8, h[i]);
-        load_f8<T>(y + v * 8, u[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ss += u[i][j] * u[i][j];
-          s[i][j] = a.scale;
-        }
-        if (a.gate) {
-          float f[8];
-          load_f8<T>(gate + v * 8, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s[i][j] *= f[j];
-        }
+        h[i] = unpack8<T>(load_raw8<T>(x + v * 8));
+        u[i] = unpack8<T>(load_raw8<T>(y + v * 8));
+        dot8(ss, u[i], u[i]);
+        if (a.token_gate) u[i] = mul8(u[i], unpack8<T>(load_raw8<T>(ring.row(2) + v * 8)));
       }
     }
     // behind this sum the row is in registers, and its stage is free
-    if (!row_sum<TPR>(ss, slots[0][parity], group, ok)) break;
-    if (tr == 0 && row + (long long)a.stages * step < a.T) ring.fetch(ring.stage, row + (long long)a.stages * step);
+    float sum = both(ss);
+    if (!row_sum<TPR>(sum, slots[0][parity], group, ok)) break;
+    if (tr == 0 && row + a.stages < end) ring.fetch(ring.stage, row + a.stages);
     ring.next();
-    const float ry = a.post ? rsqrtf(ss / (float)a.D + a.eps) : 1.f;
-    ss = 0.f;
+    const float ry = a.post ? rsqrtf(sum / (float)a.D + a.eps) : 1.f;
+    ss = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
-        if (a.post) {
-          float f[8];
-          load_f8<T>(post + v * 8, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) u[i][j] *= ry * f[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          h[i][j] += s[i][j] * u[i][j];
-          ss += h[i][j] * h[i][j];
-        }
-        store_f8<T>(reinterpret_cast<T*>(a.h) + at + v * 8, h[i]);
+        h[i] = fma8(mul8(u[i], ry), f[i], h[i]);
+        dot8(ss, h[i], h[i]);
+        store8<T>(reinterpret_cast<T*>(a.h) + at + v * 8, h[i]);
       }
     }
-    row_sum<TPR>(ss, slots[1][parity], group);
-    const float rh = rsqrtf(ss / (float)a.D + a.eps);
+    sum = both(ss);
+    row_sum<TPR>(sum, slots[1][parity], group);
+    const float rh = rsqrtf(sum / (float)a.D + a.eps);
     if (tr == 0 && a.rstd) reinterpret_cast<float2*>(a.rstd)[row] = make_float2(ry, rh);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
-      if (v < nvec) {
-        float f[8];
-        load_f8<T>(w + v * 8, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= h[i][j] * rh;
-        store_f8<T>(reinterpret_cast<T*>(a.n) + at + v * 8, f);
-      }
+      if (v < nvec) store8<T>(reinterpret_cast<T*>(a.n) + at + v * 8, mul8(mul8(h[i], rh), unpack8<T>(load_raw8<T>(w + v * 8))));
+    }
+    if (in_group > 0 && --in_group == 0 && row + 1 < end) {
+      gate += a.D;
+      in_group = a.group_rows;
+      factors<T, NV, TPR>(f, a.scale, gate, a.post, tr, nvec);
     }
   }
 }
@@ -198,9 +203,9 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
 // A CTA walks over the rows of one group of tokens (all tokens where the gate is per token); its threads hold the same columns of every
 // row and sum the parameters' gradients in registers on the way.
 template <typename T, int TPR, bool TOKEN_GATE>
-__global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_bwd_kernel(NormArgs a) {
-  constexpr int THREADS = BLOCK<TPR>, ROWS = THREADS / TPR;
-  extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(BLOCK<TPR>, BWD_BLOCKS<TPR>) residual_norm_bwd_kernel(NormArgs a) {
+  constexpr int THREADS = BLOCK<TPR>, ROWS = THREADS / TPR, NV = 2;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t bars[ROWS * MAX_STAGES];
   __shared__ float slots[2][2][THREADS / 32];
   const int group = threadIdx.x / TPR, tr = threadIdx.x % TPR;
@@ -210,18 +215,15 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
   const int first = part * ROWS + group, step = a.ctas_per_group * ROWS;
   const long long row0 = (long long)gg * rows;
   const float inv_d = 1.f / (float)a.D;
-  const T *post = reinterpret_cast<const T*>(a.post), *w = reinterpret_cast<const T*>(a.weight);
+  const T* w = reinterpret_cast<const T*>(a.weight);
   Ring<T, TPR> ring;
-  {
-    int n = 0;
-    ring.src[n++] = a.x;
-    ring.src[n++] = a.y;
-    if (a.dh) ring.src[n++] = a.dh;
-    if (a.dn) ring.src[n++] = a.dn;
-    if (TOKEN_GATE) ring.src[n++] = a.gate;
-    ring.start(smem, bars, group, a.stages, n, a.D);
-  }
+  ring.src[0] = a.x;
+  ring.src[1] = a.y;
+  ring.src[2] = a.dh ? a.dh : a.dn;
+  ring.src[3] = a.dh && a.dn ? a.dn : a.gate;
+  ring.src[4] = a.gate;
   const int at_dn = a.dh ? 3 : 2, at_gate = at_dn + (a.dn ? 1 : 0);
+  ring.start(smem, bars, group, a.stages, at_gate + (TOKEN_GATE ? 1 : 0), a.D);
   if (threadIdx.x == 0) {
     for (int i = 0; i < ROWS * MAX_STAGES; ++i) mbar_init(&bars[i], 1);
     mbar_fence_init();
@@ -230,27 +232,21 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
   if (tr == 0)
     for (int s = 0; s < a.stages; ++s)
       if (first + s * step < rows) ring.fetch(s, row0 + first + s * step);
-  float acc_w[NV][8], acc_z[NV][8];
+  F8 acc_w[NV], acc_z[NV], f[NV];  // f: without the gate where it is per token
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc_w[i][j] = acc_z[i][j] = 0.f;
+  for (int i = 0; i < NV; ++i) acc_w[i] = acc_z[i] = splat8(0.f);
+  factors<T, NV, TPR>(f, a.scale, TOKEN_GATE || !a.gate ? nullptr : reinterpret_cast<const T*>(a.gate) + (long long)gg * a.D, a.post, tr, nvec);
   int parity = 0;
+  const float2* rstd = reinterpret_cast<const float2*>(a.rstd) + row0;
+  float2 rs = first < rows ? rstd[first] : make_float2(0.f, 0.f);  // read a row ahead
   for (int r = first; r < rows; r += step, parity ^= 1) {
     const long long row = row0 + r, at = row * a.D;
-    const float2 rs = reinterpret_cast<const float2*>(a.rstd)[row];
     const float ry = rs.x, rh = rs.y;
+    if (r + step < rows) rs = rstd[r + step];
     const bool ok = ring.wait(601);
     Raw8<T> yr[NV], dhr[NV], gr[NV];
-    float hv[NV][8], cv[NV][8];
-    float dot = 0.f;
-    // s = scale * gate of eight elements
-    auto factor = [&](int i, int v, float(&s)[8]) {
-      if (TOKEN_GATE) unpack_raw8<T>(gr[i], s);
-      else if (a.gate) load_f8<T>(reinterpret_cast<const T*>(a.gate) + (long long)gg * a.D + v * 8, s);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = a.gate ? s[j] * a.scale : a.scale;
-    };
+    F8 hv[NV], cv[NV];
+    uint64_t dot = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
@@ -258,85 +254,52 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
         yr[i] = load_raw8<T>(ring.row(1) + v * 8);
         if (a.dh) dhr[i] = load_raw8<T>(ring.row(2) + v * 8);
         if (TOKEN_GATE) gr[i] = load_raw8<T>(ring.row(at_gate) + v * 8);
-        float f[8], s[8], yv[8];
-        load_f8<T>(ring.row(0) + v * 8, hv[i]);
-        unpack_raw8<T>(yr[i], yv);
-        factor(i, v, s);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] *= yv[j] * ry;
-        if (a.post) {
-          load_f8<T>(post + v * 8, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) s[j] *= f[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          hv[i][j] = (hv[i][j] + s[j]) * rh;  // hhat
-          cv[i][j] = 0.f;
-        }
+        F8 u = mul8(unpack8<T>(yr[i]), ry);
+        if (TOKEN_GATE) u = mul8(u, unpack8<T>(gr[i]));
+        hv[i] = mul8(fma8(u, f[i], unpack8<T>(load_raw8<T>(ring.row(0) + v * 8))), rh);  // hhat
+        cv[i] = splat8(0.f);
         if (a.dn) {
-          load_f8<T>(ring.row(at_dn) + v * 8, cv[i]);
-          load_f8<T>(w + v * 8, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            acc_w[i][j] += cv[i][j] * hv[i][j];
-            cv[i][j] *= f[j];
-            dot += cv[i][j] * hv[i][j];
-          }
+          const F8 dn = unpack8<T>(load_raw8<T>(ring.row(at_dn) + v * 8));
+          acc_w[i] = fma8(dn, hv[i], acc_w[i]);
+          cv[i] = mul8(dn, unpack8<T>(load_raw8<T>(w + v * 8)));
+          dot8(dot, cv[i], hv[i]);
         }
       }
     }
     // behind this sum the row is in registers, and its stage is free
-    if (!row_sum<TPR>(dot, slots[0][parity], group, ok)) break;
+    float sum = both(dot);
+    if (!row_sum<TPR>(sum, slots[0][parity], group, ok)) break;
     if (tr == 0 && r + (long long)a.stages * step < rows) ring.fetch(ring.stage, row + (long long)a.stages * step);
     ring.next();
-    dot *= inv_d;
-    float dot2 = 0.f;
+    sum *= -inv_d;
+    dot = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
       if (v < nvec) {
-        float g[8], f[8], s[8], yv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          g[j] = 0.f;
-          f[j] = 1.f;
+        F8 g = fma8(hv[i], sum, cv[i]);
+        g = a.dh ? fma8(g, rh, unpack8<T>(dhr[i])) : mul8(g, rh);
+        store8<T>(reinterpret_cast<T*>(a.dx) + at + v * 8, g);
+        hv[i] = mul8(unpack8<T>(yr[i]), ry);  // yhat (y itself without post)
+        if (TOKEN_GATE) {
+          const F8 gy = mul8(g, hv[i]), gate = unpack8<T>(gr[i]);
+          store8<T>(reinterpret_cast<T*>(a.dgate) + at + v * 8, mul8(gy, f[i]));
+          acc_z[i] = fma8(gy, gate, acc_z[i]);
+          g = mul8(g, gate);
+        } else {
+          acc_z[i] = fma8(g, hv[i], acc_z[i]);
         }
-        if (a.dh) unpack_raw8<T>(dhr[i], g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] += rh * (cv[i][j] - hv[i][j] * dot);
-        store_f8<T>(reinterpret_cast<T*>(a.dx) + at + v * 8, g);
-        if (a.post) load_f8<T>(post + v * 8, f);
-        unpack_raw8<T>(yr[i], yv);
-        factor(i, v, s);
-        float dg[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          hv[i][j] = yv[j] * ry;  // yhat (y itself without post)
-          const float gy = g[j] * hv[i][j];
-          if (TOKEN_GATE) {
-            dg[j] = a.scale * gy * f[j];
-            acc_z[i][j] += s[j] * gy;
-          } else {
-            acc_z[i][j] += gy;
-          }
-          cv[i][j] = s[j] * g[j] * f[j];  // e post
-          dot2 += cv[i][j] * hv[i][j];
-        }
-        if (TOKEN_GATE) store_f8<T>(reinterpret_cast<T*>(a.dgate) + at + v * 8, dg);
+        cv[i] = mul8(g, f[i]);  // e post
+        dot8(dot, cv[i], hv[i]);
       }
     }
-    if (a.post) row_sum<TPR>(dot2, slots[1][parity], group);
-    dot2 = a.post ? dot2 * inv_d : 0.f;
+    sum = both(dot);
+    if (a.post) row_sum<TPR>(sum, slots[1][parity], group);
+    sum = a.post ? -sum * inv_d : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = tr + TPR * i;
-      if (v < nvec) {
-        float o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = ry * (cv[i][j] - hv[i][j] * dot2);
-        store_f8<T>(reinterpret_cast<T*>(a.dy) + at + v * 8, o);
-      }
+      if (v < nvec) store8<T>(reinterpret_cast<T*>(a.dy) + at + v * 8, mul8(fma8(hv[i], sum, cv[i]), ry));
     }
   }
   float* sums = reinterpret_cast<float*>(smem);  // ROWS > 1: every row has been read by now
@@ -344,7 +307,15 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BLOCKS_PER_SM<TPR>) residual_norm_
   for (int k = 0; k < 2; ++k) {
     float* parts = k == 0 ? a.w_parts : a.z_parts;
     if (parts == nullptr) continue;
-    float(&acc)[NV][8] = k == 0 ? acc_w : acc_z;
+    float acc[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 t = f32x2_split(k == 0 ? acc_w[i].p[j] : acc_z[i].p[j]);
+        acc[i][2 * j] = t.x;
+        acc[i][2 * j + 1] = t.y;
+      }
     if (ROWS > 1) {  // the row groups in turn: the last one ends up with the sum
       __syncthreads();
 #pragma unroll 1
@@ -429,7 +400,7 @@ __global__ void __launch_bounds__(1024) residual_norm_param_kernel(ParamArgs a) 
   if (a.token_gate) {
     if (col < a.D)
       for (int i = lane_row; i < n; i += 32) dpost += a.z_parts[(long long)i * a.D + col];
-    dpost = finish(dpost);
+    dpost = a.scale * finish(dpost);
   } else if (a.ctas_per_group == 1) {  // a thread has whole groups
     if (col < a.D) {
       const float p = post ? (float)post[col] : 1.f;
@@ -461,61 +432,59 @@ __global__ void __launch_bounds__(1024) residual_norm_param_kernel(ParamArgs a) 
 
 int row_threads(int D) {  // threads that hold a row: 16 elements each
   int t = 32;
-  while (t * NV * 8 < D) t *= 2;
+  while (t * 16 < D) t *= 2;
   return t;
 }
-int blocks_per_sm(int D) { return row_threads(D) < 512 ? 2 : 1; }
 int rows_per_block(int D) { return row_threads(D) < 256 ? 256 / row_threads(D) : 1; }
 // CTAs that walk over one group of tokens: what is resident altogether, no more than there are rows for
 int ctas_per_group(int T, int D, int groups) {
   const int rows = rows_per_block(D), in_group = T / groups;
-  int want = (blocks_per_sm(D) * yf_num_sms() + groups - 1) / groups;
+  int want = (row_threads(D) < 512 ? BWD_BLOCKS<256> : BWD_BLOCKS<512>) * yf_num_sms() / groups;
   const int most = (in_group + rows - 1) / rows;
   if (want > most) want = most;
   return want < 1 ? 1 : want;
 }
 
-template <typename T, int N>
-int launch_rows(void (*kernel)(NormArgs), bool (&optin)[64], NormArgs a, int tensors, int grid, cudaStream_t st) {
+// sums: bytes that the sums of the row groups want
+int launch_rows(void (*kernel)(NormArgs), bool (&optin)[64], NormArgs a, int stage_bytes, int blocks, int sums, int grid, int threads, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
   if (!optin[dev]) {  // the shared-memory opt-in is a per-device attribute
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES_ONE);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES_MOST);
     if (e != cudaSuccess) return -(int)e;
     optin[dev] = true;
   }
   if (int rc = yf_tu_bind_status()) return rc;
-  const int row_bytes = tensors * a.D * (int)sizeof(T), rows = BLOCK<N> / N;
-  a.stages = ring_stages<N>(row_bytes);
-  int bytes = a.stages * rows * row_bytes;
-  if (bytes < N * NV * 8 * 4) bytes = N * NV * 8 * 4;  // the sums of the row groups meet there
-  kernel<<<grid, BLOCK<N>, bytes, st>>>(a);
+  a.stages = ring_stages(stage_bytes, blocks);
+  const int bytes = a.stages * stage_bytes;
+  if (bytes > RING_BYTES_MOST) return -1;
+  kernel<<<grid, threads, bytes < sums ? sums : bytes, st>>>(a);
   return -(int)cudaGetLastError();
 }
-template <typename T, int N>
+template <typename T, int N, int NV>
 int fwd_launch_n(const NormArgs& a, cudaStream_t st) {
   static bool optin[64] = {};
   constexpr int rows = BLOCK<N> / N;
   int grid = (a.T + rows - 1) / rows;
-  const int most = BLOCKS_PER_SM<N> * yf_num_sms();
+  const int most = FWD_BLOCKS<N, NV> * yf_num_sms();
   if (grid > most) grid = most;
-  return launch_rows<T, N>(residual_norm_fwd_kernel<T, N>, optin, a, a.token_gate ? 3 : 2, grid, st);
+  return launch_rows(residual_norm_fwd_kernel<T, N, NV>, optin, a, (a.token_gate ? 3 : 2) * rows * a.D * (int)sizeof(T), FWD_BLOCKS<N, NV>, 0, grid, BLOCK<N>, st);
 }
 template <typename T, int N>
 int bwd_launch_n(const NormArgs& a, int grid, cudaStream_t st) {
   static bool optin[2][64] = {};
-  const int tensors = 2 + (a.dh ? 1 : 0) + (a.dn ? 1 : 0) + (a.token_gate ? 1 : 0);
-  return a.token_gate ? launch_rows<T, N>(residual_norm_bwd_kernel<T, N, true>, optin[1], a, tensors, grid, st)
-                      : launch_rows<T, N>(residual_norm_bwd_kernel<T, N, false>, optin[0], a, tensors, grid, st);
+  const int tensors = 2 + (a.dh ? 1 : 0) + (a.dn ? 1 : 0) + (a.token_gate ? 1 : 0), stage = tensors * (BLOCK<N> / N) * a.D * (int)sizeof(T);
+  return a.token_gate ? launch_rows(residual_norm_bwd_kernel<T, N, true>, optin[1], a, stage, BWD_BLOCKS<N>, N * 64, grid, BLOCK<N>, st)
+                      : launch_rows(residual_norm_bwd_kernel<T, N, false>, optin[0], a, stage, BWD_BLOCKS<N>, N * 64, grid, BLOCK<N>, st);
 }
 template <typename T>
 int fwd_launch(const NormArgs& a, cudaStream_t st) {
   switch (row_threads(a.D)) {
-    case 32: return fwd_launch_n<T, 32>(a, st);
-    case 64: return fwd_launch_n<T, 64>(a, st);
-    case 128: return fwd_launch_n<T, 128>(a, st);
-    case 256: return fwd_launch_n<T, 256>(a, st);
-    default: return fwd_launch_n<T, 512>(a, st);
+    case 32: return fwd_launch_n<T, 32, 2>(a, st);
+    case 64: return fwd_launch_n<T, 64, 2>(a, st);
+    case 128: return fwd_launch_n<T, 128, 2>(a, st);
+    case 256: return fwd_launch_n<T, 256, 2>(a, st);
+    default: return fwd_launch_n<T, 256, 4>(a, st);
   }
 }
 template <typename T>
