@@ -12,99 +12,138 @@ namespace {
 //   query i sees keys          [start(i), lead(i) ? run(i) : i + 1)        from i - window + 1 on
 //   key i is seen by queries   [lead(i) ? start(i) : i, end(i))            before i + window
 // so both are single ranges, and both ends of both never decrease along a row, padding's empty [i, i) included.
-// One CTA per row: a running maximum from the left finds starts, one of the mirrored row from the right the ends.
-constexpr int DM_THREADS = 1024;
+// A CTA takes 1024 tokens of a row, one per thread.  The tokens at which a document starts, and those that are not flagged, are bits of words
+// in shared memory, for the 1024 tokens before and after the tile as well; a token finds the start of its document as the last bit before it and
+// the end as the next one behind it.  Only documents longer than that make a CTA read on to the left or the right.  Every CTA works on its
+// own: 4 x 32768 tokens 8 us (with one CTA per row, and running maxima over the row, 90 us).  Bound by the latency of the loads and of
+// four passes through shared memory.
+constexpr int DM_TILE = 1024, DM_WORDS = DM_TILE / 32;
 
-YF_DEVINL int warp_scan_max(int v) {
+// Positions around i whose bits are set in 3 x DM_WORDS words that start at position `origin`: the last one <= i, and the first one > i;
+// -1 and INT_MAX where there is none.  i is lane's position in word `at`; all lanes of a warp call with the same `at`.
+YF_DEVINL int last_at_or_before(const uint32_t* words, int at, int origin) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v = max(v, u);
-  }
-  return v;
+  const uint32_t own = words[at] & (0xffffffffu >> (31 - lane));
+  // the last word before this one that is not empty: of the 64 words that can be
+  const int w1 = at - 1 - lane, w2 = at - 33 - lane;
+  const unsigned near = __ballot_sync(0xffffffffu, w1 >= 0 && words[max(w1, 0)] != 0), far = __ballot_sync(0xffffffffu, w2 >= 0 && words[max(w2, 0)] != 0);
+  if (own) return origin + at * 32 + 31 - __clz(own);
+  if (!(near | far)) return -1;
+  const int w = near ? at - __ffs(near) : at - 32 - __ffs(far);
+  return origin + w * 32 + 31 - __clz(words[w]);
 }
-// inclusive running maximum over the block's threads, on top of `carry` (the same in every thread); returns the block's total in it
-YF_DEVINL int block_scan_max(int v, int& carry, int* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v = warp_scan_max(v);
-  __syncthreads();
-  if (lane == 31) red[warp] = v;
-  __syncthreads();
-  const int sums = warp_scan_max(red[lane]);
-  const int before = __shfl_sync(0xffffffffu, sums, max(warp, 1) - 1);
-  v = max(v, warp == 0 ? carry : max(carry, before));
-  carry = max(carry, __shfl_sync(0xffffffffu, sums, 31));
-  return v;
+YF_DEVINL int first_behind(const uint32_t* words, int at, int origin) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t own = lane == 31 ? 0u : words[at] & (0xffffffffu << (lane + 1));
+  const int w1 = at + 1 + lane, w2 = at + 33 + lane, n = 3 * DM_WORDS;
+  const unsigned near = __ballot_sync(0xffffffffu, w1 < n && words[min(w1, n - 1)] != 0), far = __ballot_sync(0xffffffffu, w2 < n && words[min(w2, n - 1)] != 0);
+  if (own) return origin + at * 32 + __ffs(own) - 1;
+  if (!(near | far)) return 0x7fffffff;
+  const int w = near ? at + __ffs(near) : at + 32 + __ffs(far);
+  return origin + w * 32 + __ffs(words[w]) - 1;
 }
 
 template <typename ID>
-__global__ void __launch_bounds__(DM_THREADS) document_mask_kernel(const ID* __restrict__ ids, const uint8_t* __restrict__ prefix,
-                                                                   int2* __restrict__ spans, int2* __restrict__ key_spans,
-                                                                   int* __restrict__ positions, int* __restrict__ padding, int S,
-                                                                   long long ids_stride, long long prefix_stride, int window) {
-  __shared__ int red[32], pads[32];
-  const long long row = blockIdx.x;
+__global__ void __launch_bounds__(DM_TILE) document_mask_kernel(const ID* __restrict__ ids, const uint8_t* __restrict__ prefix,
+                                                                int2* __restrict__ spans, int2* __restrict__ key_spans,
+                                                                int* __restrict__ positions, int* __restrict__ padding, int S,
+                                                                long long ids_stride, long long prefix_stride, int window) {
+  __shared__ uint32_t starts[3 * DM_WORDS], plain[3 * DM_WORDS];
+  __shared__ int pads[DM_WORDS], found[4];
+  const long long row = blockIdx.y;
+  const int t0 = blockIdx.x * DM_TILE, origin = t0 - DM_TILE, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ids += row * ids_stride;
   if (prefix) prefix += row * prefix_stride;
   spans += row * S;
   key_spans += row * S;
   positions += row * S;
   padding += row * ((S + 127) / 128);
-  const int chunks = (S + DM_THREADS - 1) / DM_THREADS;
-  // left to right: start(i), lead(i) (parked in key_spans by the thread that fetches them below)
-  int last_start = 0, last_plain = -1;
-  for (int c = 0; c < chunks; ++c) {
-    const int i = c * DM_THREADS + threadIdx.x;
-    const bool in = i < S;
-    const ID id = in ? ids[i] : (ID)-1;
-    const bool starts = in && (i == 0 || ids[i - 1] != id);
-    const int start = block_scan_max(starts ? i : 0, last_start, red);
-    int lead = 0;
-    if (prefix) {
-      const bool plain = in && prefix[i] == 0;
-      lead = block_scan_max(plain ? i : -1, last_plain, red) < start;
+  // a document starts at p; what is behind the row starts there
+  auto starts_at = [&](int p) { return p == 0 || p == S || ids[p] != ids[p - 1]; };
+  const int i = t0 + threadIdx.x;
+  const bool in = i < S;
+  const ID id = in ? ids[i] : (ID)0;
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    const int p = origin + part * DM_TILE + threadIdx.x;
+    const unsigned s = __ballot_sync(0xffffffffu, p >= 0 && p <= S && starts_at(p));
+    const unsigned f = prefix ? __ballot_sync(0xffffffffu, p >= 0 && p < S && prefix[p] == 0) : 0u;
+    if (lane == 0) {
+      starts[part * DM_WORDS + warp] = s;
+      plain[part * DM_WORDS + warp] = f;
     }
-    if (in) key_spans[i] = make_int2(start, lead);
-    const unsigned dead = __ballot_sync(0xffffffffu, in && id < 0);
-    if ((threadIdx.x & 31) == 0) pads[threadIdx.x >> 5] = __popc(dead);
-    __syncthreads();
-    if (threadIdx.x < 8 && c * 8 + threadIdx.x < (S + 127) / 128)
-      padding[c * 8 + threadIdx.x] = pads[4 * threadIdx.x] + pads[4 * threadIdx.x + 1] + pads[4 * threadIdx.x + 2] + pads[4 * threadIdx.x + 3];
   }
-  // right to left: end(i), run(i), as running maxima of the negated positions
-  int next_end = -S, next_plain = -S;
-  for (int c = chunks - 1; c >= 0; --c) {
-    const int i = c * DM_THREADS + (DM_THREADS - 1 - (int)threadIdx.x);
-    const bool in = i < S;
-    const ID id = in ? ids[i] : (ID)-1;
-    const bool ends = in && (i == S - 1 || ids[i + 1] != id);
-    const int end = -block_scan_max(ends ? -(i + 1) : -S, next_end, red);
-    int run = end;
-    if (prefix) run = min(run, -block_scan_max(in && prefix[i] == 0 ? -i : -S, next_plain, red));
-    if (!in) continue;
-    if (id < 0) {
-      spans[i] = key_spans[i] = make_int2(i, i);
-      positions[i] = 0;
-      continue;
+  const unsigned dead = __ballot_sync(0xffffffffu, in && id < 0);
+  if (lane == 0) pads[warp] = __popc(dead);
+  if (threadIdx.x < 4) found[threadIdx.x] = threadIdx.x < 2 ? -1 : 0x7fffffff;
+  __syncthreads();
+  if (threadIdx.x < DM_TILE / 128 && t0 / 128 + threadIdx.x < (S + 127) / 128) {
+    const int* p = pads + 4 * threadIdx.x;
+    padding[t0 / 128 + threadIdx.x] = p[0] + p[1] + p[2] + p[3];
+  }
+  const int at = DM_WORDS + warp;
+  int start = last_at_or_before(starts, at, origin), end = first_behind(starts, at, origin);
+  int last_plain = -1, next_plain = 0x7fffffff;
+  if (prefix) {
+    last_plain = last_at_or_before(plain, at, origin);
+    next_plain = first_behind(plain, at, origin);
+  }
+  // A document that is longer than the words reach: on to the left, to the right, until it starts and ends.  (The threads decide together.)
+  if (__syncthreads_or(in && start < 0)) {
+    for (int p0 = origin; p0 > 0; p0 -= 4 * DM_TILE) {
+      int s = -1, f = -1;
+#pragma unroll
+      for (int k = 1; k <= 4; ++k) {
+        const int p = p0 - k * DM_TILE + (int)threadIdx.x;
+        if (p < 0) continue;
+        if (s < 0 && starts_at(p)) s = p;
+        if (f < 0 && prefix && prefix[p] == 0) f = p;
+      }
+      if (s >= 0) atomicMax(&found[0], s);
+      if (f >= 0) atomicMax(&found[1], f);
+      if (__syncthreads_or(s >= 0)) break;
     }
-    const int2 parked = key_spans[i];
-    const int start = parked.x;
-    const bool lead = parked.y != 0;
-    const int far = window > 0 && end - i > window ? i + window : end;
-    spans[i] = make_int2(window > 0 ? max(start, i - window + 1) : start, lead ? run : i + 1);
-    key_spans[i] = make_int2(lead ? start : i, far);
-    positions[i] = i - start;
+    if (start < 0) start = found[0];
+    last_plain = max(last_plain, found[1]);
   }
+  if (__syncthreads_or(in && end == 0x7fffffff)) {
+    for (int p0 = origin + 3 * DM_TILE; p0 <= S; p0 += 4 * DM_TILE) {
+      int s = 0x7fffffff, f = 0x7fffffff;
+#pragma unroll
+      for (int k = 3; k >= 0; --k) {
+        const int p = p0 + k * DM_TILE + (int)threadIdx.x;
+        if (p > S) continue;
+        if (starts_at(p)) s = p;
+        if (prefix && p < S && prefix[p] == 0) f = p;
+      }
+      if (s != 0x7fffffff) atomicMin(&found[2], s);
+      if (f != 0x7fffffff) atomicMin(&found[3], f);
+      if (__syncthreads_or(s != 0x7fffffff)) break;
+    }
+    if (end == 0x7fffffff) end = found[2];
+    next_plain = min(next_plain, found[3]);
+  }
+  if (!in) return;
+  if (id < 0) {
+    spans[i] = key_spans[i] = make_int2(i, i);
+    positions[i] = 0;
+    return;
+  }
+  const bool lead = prefix && last_plain < start;
+  const int run = min(end, next_plain);
+  spans[i] = make_int2(window > 0 ? max(start, i - window + 1) : start, lead ? run : i + 1);
+  key_spans[i] = make_int2(lead ? start : i, window > 0 && end - i > window ? i + window : end);
+  positions[i] = i - start;
 }
 
 // ------------------------------------------------------------------ rotary embedding by positions
 // Pair (j, j + half) of a head is turned by positions[axis_j][token] * frequency_j.  The angle is kept as a fraction of a whole turn in
 // 64-bit fixed point: table[j] = (2^64 * frequency_j / 2 pi, axis_j), and the product with the integer position modulo 2^64 is exact, so
 // far positions lose nothing (a 32-bit product of position 100000 and frequency 1 is off by up to 0.004).
-// A CTA takes RO_TOKENS tokens: every (token, pair) is turned into its cosine and sine once, for all heads of q and k.
-// Bound by HBM: every element of q and k is read and written once.
-constexpr int RO_THREADS = 256, RO_TOKENS = 4, RO_MAX_HALF = 256;
+// A CTA takes up to RO_TOKENS tokens: every (token, pair) is turned into its cosine and sine once, for all heads of q and k.  A warp takes as many
+// heads side by side as its lanes hold vectors of, three times over before it stores anything, so that the memory has enough to do.
+// Bound by HBM: every element of q and k is read and written once.  2 x 4096 tokens, 64 / 8 heads of 128 in bf16: 53 us, 0.88 of the measured copy rate (67 us with a vector at a time).
+constexpr int RO_THREADS = 256, RO_TOKENS = 4, RO_MAX_HALF = 256, RO_BATCH = 3;
 struct RotaryArgs {
   const void* src[2];   // q, k
   void* dst[2];
@@ -115,50 +154,73 @@ struct RotaryArgs {
   const longlong2* table; // [half]
   long long tokens;
   int half;
+  int cta_tokens;
   float sign;  // -1: the inverse
 };
 template <typename T, typename POS>
 __global__ void __launch_bounds__(RO_THREADS) rotary_kernel(RotaryArgs a) {
-  __shared__ float cs[RO_TOKENS][RO_MAX_HALF], sn[RO_TOKENS][RO_MAX_HALF];
-  const long long t0 = blockIdx.x * (long long)RO_TOKENS;
-  const int n = (int)min((long long)RO_TOKENS, a.tokens - t0);
+  // of each eight values the first four, then behind those of all vectors the other four: neighbouring lanes read neighbouring 16 bytes
+  __shared__ __align__(16) float cs[RO_TOKENS][RO_MAX_HALF], sn[RO_TOKENS][RO_MAX_HALF];
+  const long long t0 = blockIdx.x * (long long)a.cta_tokens;
+  const int n = (int)min((long long)a.cta_tokens, a.tokens - t0);
   const POS* pos = reinterpret_cast<const POS*>(a.positions);
-  for (int i = threadIdx.x; i < n * a.half; i += RO_THREADS) {
-    const int t = i / a.half, j = i - t * a.half;
+  const int half = a.half, vecs = half / 8;
+  for (int i = threadIdx.x; i < n * half; i += RO_THREADS) {
+    const int t = i / half, j = i - t * half;
     const longlong2 f = __ldg(a.table + j);
     const unsigned long long turn = (unsigned long long)f.x * (unsigned long long)(long long)pos[f.y * a.axis_stride + t0 + t];
     float c, s;
     sincospif((float)(int)(turn >> 32) * 4.656612873077393e-10f, &s, &c);  // 2^-31: half turns in [-1, 1]
-    cs[t][j] = c;
-    sn[t][j] = s * a.sign;
+    const int at = (j & 4 ? half / 2 : 0) + (j >> 3) * 4 + (j & 3);
+    cs[t][at] = c;
+    sn[t][at] = s * a.sign;
   }
   __syncthreads();
-  const int vecs = a.half / 8, per_token = (a.heads[0] + a.heads[1]) * vecs;
-  for (int i = threadIdx.x; i < n * per_token; i += RO_THREADS) {
-    const int t = i / per_token, r = i - t * per_token;
-    int h = r / vecs;
-    const int v = (r - h * vecs) * 8;
-    const int w = h >= a.heads[0];
-    if (w) h -= a.heads[0];
-    const T* src = reinterpret_cast<const T*>(a.src[w]) + (t0 + t) * a.src_token[w] + h * a.src_head[w] + v;
-    T* dst = reinterpret_cast<T*>(a.dst[w]) + (t0 + t) * a.dst_token[w] + (long long)h * 2 * a.half + v;
-    float x[8], y[8], ox[8], oy[8];
-    load_f8<T>(src, x);
-    load_f8<T>(src + a.half, y);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int abreast = 32 / vecs, hl = lane / vecs, v = lane - hl * vecs;  // heads of a warp, this lane's head and vector
+  const int heads = a.heads[0] + a.heads[1], blocks = (heads + abreast - 1) / abreast;
+  int t = 0, hb = warp;
+  for (int u = warp; u < n * blocks; u += RO_BATCH * (RO_THREADS / 32)) {
+    Raw8<T> x[RO_BATCH], y[RO_BATCH];
+    T* dst[RO_BATCH];
+    int token[RO_BATCH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float c = cs[t][v + j], s = sn[t][v + j];
-      ox[j] = x[j] * c - y[j] * s;
-      oy[j] = y[j] * c + x[j] * s;
+    for (int k = 0; k < RO_BATCH; ++k, hb += RO_THREADS / 32) {
+      while (hb >= blocks) { hb -= blocks; ++t; }
+      int h = hb * abreast + hl;
+      dst[k] = nullptr;
+      token[k] = t;
+      if (t < n && hl < abreast && h < heads) {
+        const int w = h >= a.heads[0];
+        if (w) h -= a.heads[0];
+        const T* src = reinterpret_cast<const T*>(a.src[w]) + (t0 + t) * a.src_token[w] + h * a.src_head[w] + v * 8;
+        dst[k] = reinterpret_cast<T*>(a.dst[w]) + (t0 + t) * a.dst_token[w] + (long long)h * 2 * half + v * 8;
+        x[k] = load_raw8<T>(src);
+        y[k] = load_raw8<T>(src + half);
+      }
     }
-    store_f8<T>(dst, ox);
-    store_f8<T>(dst + a.half, oy);
+#pragma unroll
+    for (int k = 0; k < RO_BATCH; ++k) {
+      if (dst[k] == nullptr) continue;
+      const float *ct = cs[token[k]], *st = sn[token[k]];
+      const float4 c0 = reinterpret_cast<const float4*>(ct)[v], c1 = reinterpret_cast<const float4*>(ct + half / 2)[v];
+      const float4 s0 = reinterpret_cast<const float4*>(st)[v], s1 = reinterpret_cast<const float4*>(st + half / 2)[v];
+      const F8 c = {{f32x2(c0.x, c0.y), f32x2(c0.z, c0.w), f32x2(c1.x, c1.y), f32x2(c1.z, c1.w)}};
+      const F8 s = {{f32x2(s0.x, s0.y), f32x2(s0.z, s0.w), f32x2(s1.x, s1.y), f32x2(s1.z, s1.w)}};
+      const F8 m = {{f32x2(-s0.x, -s0.y), f32x2(-s0.z, -s0.w), f32x2(-s1.x, -s1.y), f32x2(-s1.z, -s1.w)}};
+      const F8 fx = unpack8<T>(x[k]), fy = unpack8<T>(y[k]);
+      store8<T>(dst[k], fma8(fy, m, mul8(fx, c)));
+      store8<T>(dst[k] + half, fma8(fx, s, mul8(fy, c)));
+    }
   }
 }
 
 template <typename T>
-int rotary_launch(const RotaryArgs& a, int pos_64, cudaStream_t st) {
-  const long long ctas = (a.tokens + RO_TOKENS - 1) / RO_TOKENS;
+int rotary_launch(RotaryArgs a, int pos_64, cudaStream_t st) {
+  // few tokens: one each, on as many SMs as there are
+  const long long share = a.tokens / (2 * yf_num_sms());
+  a.cta_tokens = share < 1 ? 1 : share > RO_TOKENS ? RO_TOKENS : (int)share;
+  const long long ctas = (a.tokens + a.cta_tokens - 1) / a.cta_tokens;
   if (ctas > 0x7fffffffll) return -1;
   if (pos_64) rotary_kernel<T, long long><<<(int)ctas, RO_THREADS, 0, st>>>(a);
   else rotary_kernel<T, int><<<(int)ctas, RO_THREADS, 0, st>>>(a);
@@ -172,12 +234,13 @@ int rotary_launch(const RotaryArgs& a, int pos_64, cudaStream_t st) {
 // window: keys at a distance of at least this are hidden (0: none are).
 extern "C" int yf_document_mask(const void* ids, int ids_64, const void* prefix, int* spans, int* key_spans, int* positions, int* padding,
                                 int B, int S, long long ids_stride, long long prefix_stride, int window, void* stream) {
-  if (B <= 0 || S <= 0 || S > 0x40000000 || window < 0 || !ids || !spans || !key_spans || !positions || !padding) return -1;
+  if (B <= 0 || B > 65535 || S <= 0 || S > 0x40000000 || window < 0 || !ids || !spans || !key_spans || !positions || !padding) return -1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const uint8_t* p = reinterpret_cast<const uint8_t*>(prefix);
   int2 *s = reinterpret_cast<int2*>(spans), *k = reinterpret_cast<int2*>(key_spans);
-  if (ids_64) document_mask_kernel<long long><<<B, DM_THREADS, 0, st>>>(reinterpret_cast<const long long*>(ids), p, s, k, positions, padding, S, ids_stride, prefix_stride, window);
-  else document_mask_kernel<int><<<B, DM_THREADS, 0, st>>>(reinterpret_cast<const int*>(ids), p, s, k, positions, padding, S, ids_stride, prefix_stride, window);
+  const dim3 grid((S + DM_TILE - 1) / DM_TILE, B);
+  if (ids_64) document_mask_kernel<long long><<<grid, DM_TILE, 0, st>>>(reinterpret_cast<const long long*>(ids), p, s, k, positions, padding, S, ids_stride, prefix_stride, window);
+  else document_mask_kernel<int><<<grid, DM_TILE, 0, st>>>(reinterpret_cast<const int*>(ids), p, s, k, positions, padding, S, ids_stride, prefix_stride, window);
   return -(int)cudaGetLastError();
 }
 

@@ -434,8 +434,8 @@ def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None
         raise ValueError(f"document_mask: prefix must be bool {list(document_ids.shape)}, got {list(prefix.shape)} {prefix.dtype}")
     if not 0 <= window < 1 << 31:
         raise ValueError(f"document_mask: window must be at least 0 and below 2^31, got {window}")
-    if document_ids.shape[1] > 1 << 30:
-        raise ValueError(f"document_mask: rows of at most 2^30 tokens, got {document_ids.shape[1]}")
+    if document_ids.shape[0] > 65535 or document_ids.shape[1] > 1 << 30:
+        raise ValueError(f"document_mask: at most 65535 rows of at most 2^30 tokens, got {list(document_ids.shape)}")
     here = _device_of("document_mask", document_ids, prefix)
     if not document_ids.is_cuda:
         return _document_mask_ref(document_ids, prefix, window)
