@@ -442,8 +442,12 @@ def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None
     if not here:
         with torch.cuda.device(document_ids.device):
             return document_mask(document_ids, prefix, window)
-    ids, flags = (t if t is None or t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous() for t in (document_ids, prefix))
-    return DocumentMask(*kernels.document_mask(ids, flags, window))
+    if document_ids.shape[1] > 1:
+        if document_ids.stride(1) != 1:
+            document_ids = document_ids.contiguous()
+        if prefix is not None and prefix.stride(1) != 1:
+            prefix = prefix.contiguous()
+    return DocumentMask(*kernels.document_mask(document_ids, prefix, window))
 
 
 def _document_mask_ref(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -> DocumentMask:
@@ -517,7 +521,6 @@ class RotaryFn(torch.autograd.Function):
         return kernels.rotary(q, k, positions, table)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dq: torch.Tensor | None, dk: torch.Tensor | None) -> Any:  # type: ignore[override]
         if dq is None and dk is None:
             return None, None, None, None
@@ -566,7 +569,6 @@ class AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
         q, k, v, out, out_lo, lse, slopes, key_spans, padding = ctx.saved_tensors
         return *kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *ctx.args, slopes, key_spans, padding), None, None, None, None
@@ -645,14 +647,17 @@ class ResidualNormFn(torch.autograd.Function):
         return h, n
 
     @staticmethod
-    @torch.autograd.function.once_differentiable  # type: ignore[untyped-decorator]
     def backward(ctx: Any, dh: torch.Tensor | None, dn: torch.Tensor | None) -> Any:  # type: ignore[override]
         x, y, w, p, g, rstd = ctx.saved_tensors
         gate_rows, scale = ctx.args
         if x.numel() == 0:
             return *(None if t is None else torch.zeros_like(t) for t in (x, y, w, p, g)), None, None, None
-        a = _ParamGrad(ctx.params[0])
-        b = None if p is None else _ParamGrad(ctx.params[1])
+        weight, post = ctx.params
+        if _sink(weight) is None and (post is None or _sink(post) is None):
+            dw, dpost = torch.empty_like(w), None if p is None else torch.empty_like(p)
+            dx, dy, dgate = kernels.residual_norm_bwd(x, y, w, p, g, gate_rows, rstd, dh, dn, scale, dw, dpost)
+            return dx, dy, dw, dpost, dgate, None, None, None
+        a, b = _ParamGrad(weight), None if post is None else _ParamGrad(post)
         if b is None:
             dx, dy, dgate = kernels.residual_norm_bwd(x, y, w, None, g, gate_rows, rstd, dh, dn, scale, a.out, None, add_dw=a.add, dw_sumsq=a.sumsq)
         else:
@@ -700,16 +705,25 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     one type (bf16, fp16 or fp32); sums are fp32 and each result is rounded once.  ``D``: a multiple of 8 up to 8192 on CUDA."""
     if x.dim() < 1 or x.shape != y.shape:
         raise ValueError(f"residual_norm: x and y must have one shape [..., D], got {list(x.shape)} and {list(y.shape)}")
-    for t in (weight, post_weight):
-        if t is not None and t.shape != x.shape[-1:]:
+    dtype, others = x.dtype, (y, weight) if post_weight is None else (y, weight, post_weight)
+    for t in others[1:]:
+        if t.shape != x.shape[-1:]:
             raise ValueError(f"residual_norm: weights must be [{x.shape[-1]}], got {list(t.shape)}")
-    if any(t is not None and t.dtype != x.dtype for t in (y, weight, post_weight, gate)) or x.dtype not in kernels._DTYPES:
-        raise TypeError(f"residual_norm: all tensors must have one type (bf16, fp16 or fp32), got {[str(t.dtype) for t in (x, y, weight, post_weight, gate) if t is not None]}")
+    if gate is not None:
+        others = (*others, gate)
+    if dtype not in kernels._DTYPES:
+        raise TypeError(f"residual_norm: the type must be bf16, fp16 or fp32, got {dtype}")
+    grad = torch.is_grad_enabled()
+    wanted = grad and x.requires_grad
+    for t in others:
+        if t.dtype != dtype:
+            raise TypeError(f"residual_norm: all tensors must have one type, got {dtype} and {t.dtype}")
+        wanted = wanted or (grad and t.requires_grad)
     scale, eps = float(scale), float(eps)
     if not math.isfinite(scale) or not 0.0 < eps < math.inf:
         raise ValueError(f"residual_norm: scale must be finite and eps positive, got {scale} and {eps}")
     rows = 0 if gate is None else _gate_rows(gate, x)
-    here = _device_of("residual_norm", x, y, weight, post_weight, gate)
+    here = _device_of("residual_norm", x, *others)
     if not x.is_cuda:
         return _residual_norm_ref(x, y, weight, post_weight, gate, scale, eps)
     if x.shape[-1] % 8 or not 0 < x.shape[-1] <= 8192:
@@ -717,7 +731,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     if not here:
         with torch.cuda.device(x.device):
             return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, weight, post_weight, gate)):
+    if wanted:
         return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps)  # type: ignore[no-any-return]
     return kernels.residual_norm_fwd(x, y, weight, post_weight, gate, rows, scale, eps, keep=False)[:2]
 

@@ -502,9 +502,9 @@ def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: floa
     b, s, hq, _ = q.shape
     hkv = k.shape[2]
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((b, s, hq, 128), device=q.device, dtype=torch.bfloat16)
+    out = q.new_empty((b, s, hq, 128))
     out_lo = torch.empty_like(out) if keep else None
-    lse = torch.empty((b, hq, s), device=q.device, dtype=torch.float32)
+    lse = q.new_empty((b, hq, s), dtype=torch.float32)
     if b * s > 0:
         _check(_native.lib().yf_attn_fwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), lse.data_ptr(), b, s, hq, hkv,
                                               qs, ks, vs, hq * 128, scale, softcap, _ptr(slopes), _ptr(spans), _ptr(padding), _stream()), "yf_attn_fwd_mods")
@@ -516,16 +516,17 @@ def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
                   padding: torch.Tensor | None, head_parts: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`attn_fwd_mods`, whose results ``out``, ``out_lo`` and ``lse`` are.  ``head_parts``: as in :func:`attn_bwd`."""
     b, s, hq, _ = q.shape
-    hkv, dev = k.shape[2], q.device
-    dq, dk, dv = (torch.empty((b, s, h, 128), device=dev, dtype=torch.bfloat16) for h in (hq, hkv, hkv))
+    hkv = k.shape[2]
+    dq, dk = torch.empty_like(out), k.new_empty((b, s, hkv, 128))
+    dv = torch.empty_like(dk)
     if b * s == 0:
         return dq, dk, dv
     (q, qs), (k, ks), (v, vs), (dout, gs) = _rows(q), _rows(k), _rows(v), _rows(dout)
-    parts = _attn_bwd_head_parts(b, s, hq, hkv, dev.index) if head_parts == 0 else head_parts
+    parts = _attn_bwd_head_parts(b, s, hq, hkv, q.device.index) if head_parts == 0 else head_parts
     # scratch: the dQ accumulator, the parts' dK and dV, and D
     n_dq, n_delta = b * s * hq * 128, b * hq * s
     n_parts = parts * 2 * b * ((s + 127) // 128 * 128) * hkv * 128 if parts > 1 else 0
-    ws = torch.empty(n_dq + n_parts + n_delta, device=dev, dtype=torch.float32)
+    ws = q.new_empty(n_dq + n_parts + n_delta, dtype=torch.float32)
     at = ws.data_ptr()
     global _launches
     _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), dout.data_ptr(), lse.data_ptr(),
@@ -545,11 +546,11 @@ def document_mask(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -
     optional flags ``prefix [B,S]`` (bool)."""
     b, s = ids.shape
     assert ids.dtype in (torch.int32, torch.int64) and (prefix is None or prefix.dtype == torch.bool)
-    assert all(t is None or s < 2 or t.stride(1) == 1 for t in (ids, prefix))
-    dev = ids.device
-    spans, key_spans = torch.empty((2, b, s, 2), device=dev, dtype=torch.int32).unbind(0)
-    positions = torch.empty((b, s), device=dev, dtype=torch.int32)
-    padding = torch.empty((b, (s + 127) // 128), device=dev, dtype=torch.int32)
+    assert s < 2 or (ids.stride(1) == 1 and (prefix is None or prefix.stride(1) == 1))
+    spans = ids.new_empty((b, s, 2), dtype=torch.int32)
+    key_spans = torch.empty_like(spans)
+    positions = ids.new_empty((b, s), dtype=torch.int32)
+    padding = ids.new_empty((b, (s + 127) // 128), dtype=torch.int32)
     if b * s > 0:
         _check(_native.lib().yf_document_mask(ids.data_ptr(), int(ids.dtype == torch.int64), _ptr(prefix), spans.data_ptr(), key_spans.data_ptr(),
                                               positions.data_ptr(), padding.data_ptr(), b, s, ids.stride(0), 0 if prefix is None else prefix.stride(0),
@@ -577,7 +578,8 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
     assert some is not None and positions.is_contiguous() and table.is_contiguous() and table.dtype == torch.int64
     b, s, _, d = some.shape
     t, dtype = b * s, some.dtype
-    q_out, k_out = (None if x is None else torch.empty(x.shape, device=x.device, dtype=dtype) for x in (q, k))
+    q_out = None if q is None else q.new_empty(q.shape)
+    k_out = None if k is None else k.new_empty(k.shape)
     q, q_token, q_head = (None, 0, 0) if q is None else _tokens(q)
     k, k_token, k_head = (None, 0, 0) if k is None else _tokens(k)
     hq, hk = 0 if q is None else q.shape[2], 0 if k is None else k.shape[2]
@@ -603,9 +605,12 @@ def residual_norm_fwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, po
     d = x.shape[-1]
     t = x.numel() // d
     x, y, weight = _flat(x), _flat(y), _flat(weight)
-    post, gate = None if post is None else _flat(post), None if gate is None else _flat(gate)
+    if post is not None:
+        post = _flat(post)
+    if gate is not None:
+        gate = _flat(gate)
     h, n = torch.empty_like(x), torch.empty_like(x)
-    rstd = torch.empty((t, 2), device=x.device, dtype=torch.float32) if keep else None
+    rstd = x.new_empty((t, 2), dtype=torch.float32) if keep else None
     if t > 0:
         _check(_native.lib().yf_residual_norm_fwd(x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, h.data_ptr(),
                                                   n.data_ptr(), _ptr(rstd), t, d, scale, eps, _DTYPES[x.dtype], _stream()), "yf_residual_norm_fwd")
@@ -626,22 +631,31 @@ def residual_norm_bwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, po
                       dpost_sumsq: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """``(dx, dy, dgate)`` for at least one token; ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the
     weights' gradients and ``*_sumsq`` the squares of them."""
-    d = x.shape[-1]
+    d, dtype = x.shape[-1], x.dtype
     t = x.numel() // d
     x, y, weight = _flat(x), _flat(y), _flat(weight)
-    post, gate, dh, dn = (None if o is None else _flat(o) for o in (post, gate, dh, dn))
+    if post is not None:
+        post = _flat(post)
+    if gate is not None:
+        gate = _flat(gate)
+    if dh is not None:
+        dh = _flat(dh)
+    if dn is not None:
+        dn = _flat(dn)
     dx, dy = torch.empty_like(x), torch.empty_like(x)
     dgate = None if gate is None else torch.empty_like(gate)
-    rows = _residual_norm_parts(t, d, gate_rows, x.device.index)
-    two = post is not None or (gate is not None and gate_rows != t)
-    floats = (2 if two else 1) * rows * d
-    parts = torch.empty(floats, device=x.device, dtype=torch.float32)
-    kinds = [0 if o is None or o.dtype == x.dtype and not add else 2 if add else 1 for o, add in ((dw, add_dw), (dpost, add_dpost))]
-    assert all(o is None or (o.is_contiguous() and o.numel() == d and (kind == 0 or o.dtype == torch.float32)) for o, kind in zip((dw, dpost), kinds))
+    floats = _residual_norm_parts(t, d, gate_rows, x.device.index) * d * (2 if post is not None or (gate is not None and gate_rows != t) else 1)
+    parts = x.new_empty(floats, dtype=torch.float32)
+    dw_kind = 2 if add_dw else 0 if dw.dtype == dtype else 1
+    assert dw.is_contiguous() and dw.numel() == d and (dw_kind == 0 or dw.dtype == torch.float32)
+    dpost_kind = 0
+    if dpost is not None:
+        dpost_kind = 2 if add_dpost else 0 if dpost.dtype == dtype else 1
+        assert dpost.is_contiguous() and dpost.numel() == d and (dpost_kind == 0 or dpost.dtype == torch.float32)
     _check(_native.lib().yf_residual_norm_bwd(
         x.data_ptr(), y.data_ptr(), weight.data_ptr(), _ptr(post), _ptr(gate), gate_rows, rstd.data_ptr(), _ptr(dh), _ptr(dn), dx.data_ptr(),
-        dy.data_ptr(), dw.data_ptr(), kinds[0], _ptr(dw_sumsq), _ptr(dpost), kinds[1], _ptr(dpost_sumsq), _ptr(dgate), parts.data_ptr(), floats, t, d,
-        scale, _DTYPES[x.dtype], _stream()), "yf_residual_norm_bwd")
+        dy.data_ptr(), dw.data_ptr(), dw_kind, _ptr(dw_sumsq), _ptr(dpost), dpost_kind, _ptr(dpost_sumsq), _ptr(dgate), parts.data_ptr(), floats, t, d,
+        scale, _DTYPES[dtype], _stream()), "yf_residual_norm_bwd")
     global _launches
     _launches += 1  # the parameters' sums
     return dx, dy, dgate
