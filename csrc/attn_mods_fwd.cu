@@ -86,30 +86,56 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
   const int n_tiles_kv = (args.S + BKV - 1) / BKV;
   const int2* spans = args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
   const int* padding = args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * n_tiles_kv;
-  // half blocks [from, to) of the two tiles; none when the sequence ends before, for nothing but padding, or without a second tile
-  int from[2], to[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row0 = q0 + i * BQ, rows = min(BQ, args.S - row0);
-    from[i] = to[i] = 0;
-    if (i >= args.tiles || rows <= 0) continue;
-    if (spans == nullptr) {
-      to[i] = (row0 + rows + HKV - 1) / HKV;
-    } else if (__ldg(padding + row0 / BQ) < rows) {
-      from[i] = max(__ldg(spans + row0).x, 0) / HKV;
-      to[i] = min(__ldg(spans + row0 + rows - 1).y, args.S);
-      to[i] = max((to[i] + HKV - 1) / HKV, from[i]);
-    }
-    if (from[i] >= to[i]) from[i] = to[i] = 0;
-  }
-  const bool has0 = to[0] > 0, has1 = to[1] > 0;
-  const int j_first = (has0 && has1 ? min(from[0], from[1]) : has0 ? from[0] : from[1]) >> 1;
-  const int j_end = (max(to[0], to[1]) + 1) >> 1;
+  const bool second = args.tiles == 2 && q0 + BQ < args.S;
+  auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+    mbar_expect_tx(bar, TILE);
+    tma_load_3d(dst, map, bar, x, y, b);
+    tma_load_3d(dst + ATOM, map, bar, x + 64, y, b);
+  };
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&tma_q);
+    mbar_init(&q_full[0], 1);
+    mbar_init(&q_full[1], 1);
+    mbar_fence_init();
+    // Q does not depend on the ranges, whose loads take as long
+    load(sQ, &tma_q, &q_full[0], h * HD, q0);
+    if (second) load(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ);
     tma_prefetch_desc(&tma_k);
     tma_prefetch_desc(&tma_v);
     tma_prefetch_desc(&tma_o);
+  }
+  // half blocks [from, to) of the two tiles; none when the sequence ends before, for nothing but padding, or without a second tile
+  int from[2], to[2];
+  if (spans == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      from[i] = 0;
+      to[i] = (min(q0 + (i + 1) * BQ, args.S) + HKV - 1) / HKV;
+    }
+  } else {
+    int2 a[2], z[2];
+    int dead_rows[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // all loads at once: a row past the end stands for one in front of it
+      const int row0 = min(q0 + i * BQ, args.S - 1);
+      a[i] = __ldg(spans + row0);
+      z[i] = __ldg(spans + min(row0 + BQ - 1, args.S - 1));
+      dead_rows[i] = __ldg(padding + row0 / BQ);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      from[i] = max(a[i].x, 0) / HKV;
+      to[i] = dead_rows[i] >= min(BQ, args.S - q0 - i * BQ) ? 0 : (min(z[i].y, args.S) + HKV - 1) / HKV;
+    }
+  }
+  if (!second) to[1] = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (from[i] >= to[i]) from[i] = to[i] = 0;
+  const bool has0 = to[0] > 0, has1 = to[1] > 0;
+  const int j_first = (has0 && has1 ? min(from[0], from[1]) : has0 ? from[0] : from[1]) >> 1;
+  const int j_end = (max(to[0], to[1]) + 1) >> 1;
+
+  if (threadIdx.x == 0) {
     const int n_tiles = max(1, (has0 ? 1 : 0) + (has1 ? 1 : 0));  // one arrival each for a stage that is free again
     for (int s = 0; s < KST; ++s) {
       mbar_init(&k_full[s], 1);
@@ -118,9 +144,6 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     for (int s = 0; s < VST; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&q_full[s], 1);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
@@ -142,11 +165,6 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
 
   if (warp == 0) {
     // the whole warp, since it clears the padded rows of the V tiles that have some; K of a block comes before V of the block before
-    auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
-      mbar_expect_tx(bar, TILE);
-      tma_load_3d(dst, map, bar, x, y, b);
-      tma_load_3d(dst + ATOM, map, bar, x + 64, y, b);
-    };
     int dead_rows = padding != nullptr && j_first < j_end ? __ldg(padding + j_first) : 0, landed = 0;
     int ks = 0, kp = 1, vs = 0, vp = 1;
     for (int j = j_first; j <= j_end && j_first < j_end; ++j) {
@@ -154,9 +172,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       if (lane == 0 && j < j_end) {
         ok = mbar_wait(&k_empty[ks], kp, 400);
         if (ok) {
-          if (j == j_first && has0) load(sQ, &tma_q, &q_full[0], h * HD, q0);
           load(sK + ks * TILE, &tma_k, &k_full[ks], hkv * HD, j * BKV);
-          if (j == j_first && has1) load(sQ + TILE, &tma_q, &q_full[1], h * HD, q0 + BQ);
         }
         if (++ks == KST) { ks = 0; kp ^= 1; }
       }
@@ -176,6 +192,9 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       }
       if (++vs == VST) { vs = 0; vp ^= 1; }
     }
+    // a tile without keys: its Q has to land before the block ends
+    if (lane == 0 && !has0) mbar_wait(&q_full[0], 0, 403);
+    if (lane == 0 && !has1 && second) mbar_wait(&q_full[1], 0, 403);
   } else if (warp == 1) {
     // O += P V, the tiles in turn
     if (j_first < j_end && elect_one()) {
@@ -403,7 +422,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           tma_store_commit();
         }
       }
-      if (lane == 0) tma_store_wait0();
+      if (lane == 0) tma_store_wait_read0();  // the rest of the way is not this block's
       if (half == 0 && qrow < args.S)
         args.lse[((long long)b * args.Hq + h) * args.S + qrow] =
             (l > 0.f) ? (m_run * ((MODS & (MOD_CAP | MOD_BIAS)) ? 0.6931471805599453f : args.scale) + logf(l)) : -INFINITY;
