@@ -93,22 +93,18 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
   // ranges of queries by key, padded tokens by tile
   const int2* spans = args.mods.spans == nullptr ? nullptr : args.mods.spans + (long long)b * args.S;
   const int* padding = args.mods.spans == nullptr ? nullptr : args.mods.padding + (long long)b * n_kt;
-  int i_start = kv0 / BQ, per_head = n_qt - i_start;  // query tiles [i_start, + per_head)
-  if (spans != nullptr) {
-    const int keys = min(BKV, args.S - kv0);
-    i_start = max(__ldg(spans + kv0).x, 0) / BQ;
-    per_head = min((__ldg(spans + kv0 + keys - 1).y + BQ - 1) / BQ, n_qt) - i_start;
-    if (__ldg(padding + jt) >= keys || per_head < 0) per_head = 0;  // nothing but padding
-  }
-  const int n_it = per_head * heads;
-
   if (threadIdx.x == 0) {
+    mbar_init(kv_land, 1);
+    mbar_fence_init();
+    // K and V do not depend on the ranges, whose loads take as long
+    mbar_expect_tx(kv_land, 2 * TILE);
+    tma_load_3d(sK, &tma_k, kv_land, hk * HD, kv0, b);
+    tma_load_3d(sK + ATOM, &tma_k, kv_land, hk * HD + 64, kv0, b);
+    tma_load_3d(sV, &tma_v, kv_land, hk * HD, kv0, b);
+    tma_load_3d(sV + ATOM, &tma_v, kv_land, hk * HD + 64, kv0, b);
     tma_prefetch_desc(&tma_q);
-    tma_prefetch_desc(&tma_k);
-    tma_prefetch_desc(&tma_v);
     tma_prefetch_desc(&tma_do);
     tma_prefetch_desc(&tma_dq);
-    mbar_init(kv_land, 1);
     mbar_init(kv_full, 1);
     mbar_init(all_done, 1);
     for (int i = 0; i < STAGES; ++i) {
@@ -125,6 +121,18 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     }
     mbar_fence_init();
   }
+  int i_start = kv0 / BQ, per_head = n_qt - i_start;  // query tiles [i_start, + per_head)
+  int dead_keys = 0;                                  // padded ones of this tile
+  if (spans != nullptr) {
+    const int keys = min(BKV, args.S - kv0);
+    const int2 a = __ldg(spans + kv0), z = __ldg(spans + kv0 + keys - 1);
+    dead_keys = __ldg(padding + jt);
+    i_start = max(a.x, 0) / BQ;
+    per_head = min((z.y + BQ - 1) / BQ, n_qt) - i_start;
+    if (dead_keys >= keys || per_head < 0) per_head = 0;  // nothing but padding
+  }
+  const int n_it = per_head * heads;
+
   if (warp == 21) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -137,11 +145,6 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
 
   if (warp == 20) {
     if (n_it > 0 && elect_one()) {
-      mbar_expect_tx(kv_land, 2 * TILE);
-      tma_load_3d(sK, &tma_k, kv_land, hk * HD, kv0, b);
-      tma_load_3d(sK + ATOM, &tma_k, kv_land, hk * HD + 64, kv0, b);
-      tma_load_3d(sV, &tma_v, kv_land, hk * HD, kv0, b);
-      tma_load_3d(sV + ATOM, &tma_v, kv_land, hk * HD + 64, kv0, b);
       int h = h0, i = 0;
       for (int it = 0, st = 0, ph = 1; it < n_it; ++it) {
         if (!mbar_wait(&q_empty[st], ph, 500)) break;
@@ -172,10 +175,10 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         dl[e] = ok ? args.delta[at + r] : 0.f;
       }
     };
-    if (n_it > 0) {
-      fetch();
-      if (__all_sync(0xffffffffu, mbar_wait(kv_land, 0, 502))) {
-        if (padding != nullptr && __ldg(padding + jt) > 0) {  // dQ^T = K^T dS^T would multiply what padding holds by zeros
+    if (n_it > 0) fetch();
+    if (__all_sync(0xffffffffu, mbar_wait(kv_land, 0, 502))) {  // (without queries too: the tiles have to land before the block ends)
+      if (n_it > 0) {
+        if (dead_keys > 0) {  // dQ^T = K^T dS^T would multiply what padding holds by zeros
           zero_padded_rows(sK, ATOM, BKV, kv0, args.S, spans);
           fence_proxy_async_smem();
           __syncwarp();
@@ -395,7 +398,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         if (lane == 0) {
           tma_store_3d(p == 0 ? &tma_dv : &tma_dk, stage, hk * HD + half * 64, kv0 + (warp & 3) * 32, b);
           tma_store_commit();
-          tma_store_wait0();
+          tma_store_wait_read0();  // the rest of the way is not this block's
         }
       }
     }
@@ -433,7 +436,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       }
       if (++i == per_head) { i = 0; ++h; }
     }
-    if (lane == 0) tma_store_wait0();  // this warp's reduce-adds have completed
+    if (lane == 0) tma_store_wait_read0();
     tc_fence_before();
   }
 
