@@ -56,7 +56,7 @@ template <int N>
 YF_DEVINL void cap_scores(uint32_t (&s)[N], const AttnMods& m) {
   float far = 0.f;
 #pragma unroll
-  for (int t = 0; t < N; ++t) far = fmaxf(far, fabsf(__uint_as_float(s[t])));
+  for (int t = 0; t < N; t += 2) far = fmax3_abs(far, __uint_as_float(s[t]), __uint_as_float(s[t + 1]));
   if (far <= m.poly_max) {
     const uint64_t p0 = f32x2(m.poly[0], m.poly[0]), p1 = f32x2(m.poly[1], m.poly[1]), p2 = f32x2(m.poly[2], m.poly[2]),
                    p3 = f32x2(m.poly[3], m.poly[3]);

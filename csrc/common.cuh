@@ -97,18 +97,6 @@ YF_DEVINL bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// the same without being put to sleep, for a thread that watches several barriers
-YF_DEVINL bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // Bounded wait.  Returns false when the wait gave up (timeout or global abort).
 YF_DEVINL bool mbar_wait(uint64_t* bar, uint32_t parity, int site) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -148,6 +136,33 @@ YF_DEVINL void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
+}
+// Takes a block of this launch that has not started yet, so that the caller does its work: a block that is done with its own pays neither
+// for another's start nor for its end.  The answer, 16 bytes of shared memory on a boundary of 16, comes in with `bar`; after one that says there
+// was none left no other may be asked for.
+YF_DEVINL void claim_block(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+YF_DEVINL bool claimed_block(const void* answer, uint3& at) {
+  uint32_t got;
+  asm volatile(
+      "{\n"
+      ".reg .b128 a;\n"
+      ".reg .pred p;\n"
+      "ld.shared.b128 a, [%4];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "mov.u32 %1, 0;\n"
+      "mov.u32 %2, 0;\n"
+      "mov.u32 %3, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, a;\n"
+      "}\n"
+      : "=&r"(got), "=&r"(at.x), "=&r"(at.y), "=&r"(at.z)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got != 0;
 }
 YF_DEVINL void tma_store_2d(const CUtensorMap* m, const void* smem_src, int x, int y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
@@ -397,6 +412,17 @@ YF_DEVINL uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t v;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
   return v;
+}
+// the largest of three, and of three magnitudes; NaN only where all are
+YF_DEVINL float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+YF_DEVINL float fmax3_abs(float a, float b, float c) {
+  float r;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 YF_DEVINL uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   uint64_t v;
