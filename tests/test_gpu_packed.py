@@ -524,3 +524,139 @@ def test_packed_layer_equals_its_documents_alone():
     _done()
     for g, t in zip(grads, total):
         assert ((g.float() - t).norm() / t.norm()).item() < 2.0**-6
+
+
+# ----------------------------------------------------------------------------------------- more work than the GPU holds at once, places far apart
+def _uneven_rows(s):
+    """Rows of nothing but padding, with padding in front, in the middle, behind, of one document and of many."""
+    ids = torch.zeros(6, s, dtype=torch.int64)
+    ids[0] = -1
+    ids[1, : s * 3 // 7] = -2
+    ids[2, s // 5 : s * 4 // 7] = -1
+    ids[3, s // 2 :] = -1
+    ids[5] = _ids(1, s, 30, True)[0]
+    return ids
+
+
+@pytest.mark.parametrize("softcap,biased", [(0.0, False), (30.0, False), (30.0, True)])
+def test_attention_of_more_tiles_than_fit(softcap, biased):
+    """Blocks that go on with other heads and sequences, of other lengths and without any: what the sequences give alone, to the bit, and the
+    definition."""
+    from yafsdp_b200.ops import functional as Fn
+
+    b, s, hq, hkv = 6, 700, 32, 8
+    ids = _uneven_rows(s).to(DEV)
+    mask = Fn.document_mask(ids)
+    slopes = torch.tensor([2.0 ** (-8.0 * (h + 1) / hq) for h in range(hq)], device=DEV) if biased else None
+    q, k, v = (t.detach() for t in _qkv(b, s, hq, hkv))
+    out = Fn.attention(q, k, v, mask, softcap=softcap, slopes=slopes)
+    for i in range(b):
+        alone = Fn.attention(*(t[i : i + 1] for t in (q, k, v)), Fn.document_mask(ids[i : i + 1]), softcap=softcap, slopes=slopes)
+        assert torch.equal(alone[0], out[i]), i
+    _check(b, s, hq, hkv, mask, softcap, slopes)
+
+
+def test_attention_rows_far_apart():
+    """A projection's rows at a pitch that takes their offsets past 32 bits: what the same rows give side by side."""
+    from yafsdp_b200.ops import functional as Fn
+    from yafsdp_b200.ops import kernels
+
+    s, pitch = 33000, 1 << 16
+    wide = torch.empty(1, s, pitch, device=DEV, dtype=torch.bfloat16)
+    near = _qkv(1, s, 2, 1)
+    q, k, v = (wide[..., at : at + t.shape[2] * 128].unflatten(-1, (-1, 128)) for t, at in zip(near, (65024, 128, 4096)))
+    for far, t in zip((q, k, v), near):
+        far.copy_(t.detach())
+    mask = Fn.document_mask(_ids(1, s, 900, True).to(DEV))
+    dout = torch.randn(1, s, 2, 128, device=DEV).bfloat16()
+    results = []
+    for args in ((q, k, v), [t.detach().contiguous() for t in near]):
+        out, low, lse = kernels.attn_fwd_mods(*args, 0.1, 0.0, None, mask.spans, mask.padding)
+        results.append((out, low, lse, *kernels.attn_bwd_mods(*args, out, low, dout, lse, 0.1, 0.0, None, mask.key_spans, mask.padding)[1:]))
+    _done()
+    assert all(torch.equal(a, z) for a, z in zip(*results))
+
+
+def test_rotary_and_residual_norm_past_32_bits():
+    """The last tokens of tensors of more than 2^31 elements: what they give alone."""
+    from yafsdp_b200.ops import functional as Fn
+
+    t, d = 263000, 8192
+    x, y, dh, dn = (torch.empty(t, d, device=DEV, dtype=torch.bfloat16) for _ in range(4))
+    for big in (x, y, dh, dn):
+        big[:-5].zero_()
+        big[-5:] = torch.randn(5, d, device=DEV).bfloat16()
+    w = torch.ones(d, device=DEV, dtype=torch.bfloat16)
+    ends = []
+    for cut in (slice(None), slice(-5, None)):
+        leaves = [z[cut].requires_grad_() for z in (x, y)]
+        h, n = Fn.residual_norm(*leaves, w)
+        grads = torch.autograd.grad((h, n), leaves, (dh[cut], dn[cut]))
+        ends.append([z[-5:].clone() for z in (h.detach(), n.detach(), *grads)])
+        del h, n, grads
+    assert all(torch.equal(a, z) for a, z in zip(*ends))
+    axes = Fn.RotaryAxes(128, 1e4)
+    positions = torch.arange(t, device=DEV)[None]
+    q = x.detach().view(1, t, 64, 128)
+    far = Fn.rotary(q, q[:, :, :1], positions, axes)[0][:, -5:].clone()
+    assert torch.equal(far, Fn.rotary(q[:, -5:], q[:, -5:, :1], positions[:, -5:], axes)[0])
+    _done()
+
+
+def test_residual_norm_in_a_sharded_module():
+    """Weights of a sharded module, one of them used twice, over two backward passes: their fp32 gradients are the sums of what the calls give one by
+    one to within the roundings of those, and the norm is theirs."""
+    import torch.distributed as dist
+
+    from yafsdp_b200 import MixedPrecisionPolicy, fully_shard
+    from yafsdp_b200.ops import functional as Fn
+    from yafsdp_b200.optim import clip_grad_norm_
+
+    d = 520
+
+    class Steps(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            gen = torch.Generator(device=DEV).manual_seed(0)
+            self.w, self.post, self.gate = (torch.nn.Parameter((1 + 0.1 * torch.randn(d, device=DEV, generator=gen)).bfloat16().float()) for _ in range(3))
+
+        def forward(self, x, y):
+            h, n = Fn.residual_norm(x, y, self.w, post_weight=self.post, gate=self.gate, scale=0.5)
+            return Fn.residual_norm(h, n, self.w)
+
+    torch.cuda.set_device(0)
+    created = not dist.is_initialized()
+    if created:
+        dist.init_process_group("nccl", store=dist.HashStore(), rank=0, world_size=1)
+    try:
+        model = Steps()
+        w, post, gate = (p.detach().bfloat16() for p in (model.w, model.post, model.gate))
+        fully_shard(model, mp_policy=MixedPrecisionPolicy(param_dtype=torch.bfloat16, reduce_dtype=torch.float32))
+        total = {name: [torch.zeros(d, device=DEV, dtype=torch.float64) for _ in range(2)] for name in ("w", "post", "gate")}
+        for step in range(2):
+            x, y, dh, dn = (torch.randn(1, 77, d, device=DEV).bfloat16() for _ in range(4))
+            torch.autograd.backward(model(x, y), (dh, dn))
+            one, two = w.clone().requires_grad_(), w.clone().requires_grad_()
+            p, g = post.clone().requires_grad_(), gate.clone().requires_grad_()
+            h, n = Fn.residual_norm(x, y, one, post_weight=p, gate=g, scale=0.5)
+            for name, grad in zip(("w", "w", "post", "gate"), torch.autograd.grad(Fn.residual_norm(h, n, two), (one, two, p, g), (dh, dn))):
+                total[name][0] += grad.double()
+                total[name][1] += grad.double().abs()
+        _done()
+        grads = {name: p.grad._local_tensor for name, p in model.named_parameters()}
+        for name, (want, mass) in total.items():
+            # each bf16 gradient is off by half a step of its own; where the module adds bf16 gradients (the gate), its sums are fp32
+            assert ((grads[name].view(-1).double() - want).abs() <= 1.01 * 2.0**-8 * mass + 1e-12).all(), name
+        norm = torch.stack([g.double().norm() for g in grads.values()]).norm()
+        assert abs(clip_grad_norm_(model, 1e9).item() / norm.item() - 1.0) < 1e-5
+    finally:
+        if created:
+            dist.destroy_process_group()
+
+
+def test_attention_refuses_too_many_rows():
+    from yafsdp_b200.ops import functional as Fn
+
+    t = torch.empty(65536, 1, 1, 128, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        Fn.attention(t, t, t)

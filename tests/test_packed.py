@@ -159,3 +159,23 @@ def test_rotary_axes_layouts():
 def test_refusals(call, error):
     with pytest.raises(error):
         call()
+
+
+def test_hand_made_masks():
+    m = Fn.document_mask(torch.zeros(2, 130, dtype=torch.int64))
+    parts = {n: getattr(m, n) for n in ("spans", "key_spans", "positions", "padding")}
+    assert Fn.DocumentMask(**{n: t[:1] for n, t in parts.items()}).spans.shape == (1, 130, 2)
+    for name, wrong in (("spans", m.spans[..., :1]), ("key_spans", m.key_spans[:, :129]), ("positions", m.positions[0]), ("padding", m.padding[:, :1]),
+                        ("spans", m.spans.long()), ("padding", m.padding.float()), ("key_spans", m.key_spans.transpose(0, 1).contiguous().transpose(0, 1)),
+                        ("positions", m.positions.to("meta"))):
+        with pytest.raises(ValueError):
+            Fn.DocumentMask(**{**parts, name: wrong})
+
+
+@pytest.mark.parametrize("call", [
+    lambda t, w: Fn.attention(t, t, t, softcap=1e-13), lambda t, w: Fn.attention(t, t, t, softcap=1e13), lambda t, w: Fn.attention(t, t, t, scale=1e-13),
+    lambda t, w: Fn.attention(t, t, t, scale=1e13), lambda t, w: Fn.residual_norm(t, t, w, post_weight=w),
+])
+def test_refused_values(call):
+    with pytest.raises(ValueError):
+        call(torch.zeros(1, 2, 2, 16), torch.ones(16))

@@ -416,12 +416,23 @@ def _device_of(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> 
 class DocumentMask:
     """Which tokens of a packed batch see each other (:func:`document_mask`): query ``i`` of a row sees the keys ``spans[i, 0] <= j <
     spans[i, 1]``, key ``j`` is seen by the queries ``key_spans[j, 0] <= i < key_spans[j, 1]``.  ``positions``: index of a token in its
-    document.  ``padding``: padded tokens in every 128 of a row."""
+    document.  ``padding``: padded tokens in every 128 of a row.  Neither end of
+    a span moves back along a row, and both views say the same: the kernels rely on it."""
 
     spans: torch.Tensor  # [B, S, 2] int32
     key_spans: torch.Tensor  # [B, S, 2] int32
     positions: torch.Tensor  # [B, S] int32
     padding: torch.Tensor  # [B, ceil(S / 128)] int32
+
+    def __post_init__(self) -> None:
+        parts = (self.positions, self.padding, self.spans, self.key_spans)
+        pos = self.positions
+        b, s = pos.shape if pos.dim() == 2 else (-1, -1)
+        if self.spans.shape != (b, s, 2) or self.key_spans.shape != (b, s, 2) or self.padding.shape != (b, (s + 127) // 128):
+            raise ValueError(f"DocumentMask: spans and key_spans [B, S, 2], positions [B, S], padding [B, ceil(S / 128)] expected, got {[list(t.shape) for t in parts[2:] + parts[:2]]}")
+        for t in parts:
+            if t.dtype != torch.int32 or t.device != pos.device or not t.is_contiguous():
+                raise ValueError("DocumentMask: int32 tensors without gaps on one device expected")
 
 
 def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None, window: int = 0) -> DocumentMask:
@@ -590,10 +601,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
         raise TypeError(f"attention: q, k and v must have one type, got {q.dtype}, {k.dtype}, {v.dtype}")
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
-        raise ValueError(f"attention: scale must be positive and softcap not negative, got {scale} and {softcap}")
-    if mask is not None and (mask.spans.shape[:2] != q.shape[:2] or mask.key_spans.shape[:2] != q.shape[:2]):
-        raise ValueError(f"attention: the mask is for {list(mask.spans.shape[:2])} tokens, q has {list(q.shape[:2])}")
+    if not 1e-12 <= scale <= 1e12 or not (softcap == 0.0 or 1e-12 <= softcap <= 1e12):  # beyond, their squares and ratios leave fp32
+        raise ValueError(f"attention: scale must be from 1e-12 to 1e12 and softcap zero or from 1e-12 to 1e12, got {scale} and {softcap}")
+    if mask is not None and mask.positions.shape != q.shape[:2]:
+        raise ValueError(f"attention: the mask is for {list(mask.positions.shape)} tokens, q has {list(q.shape[:2])}")
     if slopes is not None and slopes.shape != (q.shape[2],):
         raise ValueError(f"attention: slopes must have one value for each of {q.shape[2]} query heads, got {list(slopes.shape)}")
     if slopes is not None and slopes.requires_grad:
@@ -603,6 +614,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
         return _attention_ref(q, k, v, mask, scale, softcap, slopes)
     if q.dtype != torch.bfloat16 or q.shape[3] != 128:
         raise TypeError(f"attention: the CUDA kernels take bf16 heads of 128, got {q.dtype} heads of {q.shape[3]}")
+    if q.shape[0] > 65535 or q.shape[1] > 1 << 23:
+        raise ValueError(f"attention: the CUDA kernels take at most 65535 rows of at most 2^23 tokens, got {list(q.shape[:2])}")
     if not here:
         with torch.cuda.device(q.device):
             return attention(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes)
@@ -709,6 +722,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     for t in others[1:]:
         if t.shape != x.shape[-1:]:
             raise ValueError(f"residual_norm: weights must be [{x.shape[-1]}], got {list(t.shape)}")
+    if post_weight is weight:  # one launch finishes both gradients, which then have one place to go
+        raise ValueError("residual_norm: weight and post_weight must be two tensors")
     if gate is not None:
         others = (*others, gate)
     if dtype not in kernels._DTYPES:
