@@ -451,8 +451,8 @@ static int attn_bwd_launch(int head_parts, float* dkv_parts, const float* rope, 
     long long blocks = (items + 255) / 256;
     const long long cap = (long long)yf_num_sms() * 8;
     if (blocks > cap) blocks = cap;
-    attn_convert_kernel<<<(int)blocks, 256, 0, st>>>(dq_accum, a.dkv_parts, head_parts, rope, reinterpret_cast<__nv_bfloat16*>(dq), a.dk, a.dv, B, S, Hq, Hkv,
-                                                     dq_stride, dkv_stride, scale);
+    attn_convert_kernel<false><<<(int)blocks, 256, 0, st>>>(dq_accum, a.dkv_parts, head_parts, rope, reinterpret_cast<__nv_bfloat16*>(dq), a.dk, a.dv, B, S, Hq, Hkv,
+                                                            dq_stride, dkv_stride, scale, nullptr);
   }
   return -(int)cudaGetLastError();
 }

@@ -106,11 +106,20 @@ YF_DEVINL const float4* rope_at(const float* rope, int pos, int dim) {
   return rope == nullptr ? nullptr : reinterpret_cast<const float4*>(rope + ((long long)pos * 64 + dim) * 2);
 }
 
+// Whether token t, the i-th of its sequence, sees one key only; spans null: causal.  Its probability is 1 whatever q and k are, so they get no
+// gradient from it: zeros, not what is left of the difference of two equal sums.
+YF_DEVINL bool sees_one_key(const int2* spans, long long t, int i) {
+  if (spans == nullptr) return i == 0;
+  const int2 s = __ldg(spans + t);
+  return s.y - s.x == 1;
+}
+
 // dq (bf16, strided rows) = scale * dq_accum (fp32, dense rows of 128 Hq); with dkv_parts also dk = scale * the sum of the parts' dK and
-// dv = that of their dV, in the order of the parts.  `rope` ([S, 64, 2]: cos, sin): dq and dk go back through the rotation.
+// dv = that of their dV, in the order of the parts.  RANGES: rows of dq that see one key are zeros.  `rope` ([S, 64, 2]: cos, sin): dq and dk go back through the rotation.
+template <bool RANGES>
 __global__ void __launch_bounds__(256) attn_convert_kernel(const float* __restrict__ dq_acc, const float4* __restrict__ dkv_parts, int parts, const float* __restrict__ rope,
                                     __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv, int B,
-                                    int S, int Hq, int Hkv, long long dq_stride, long long dkv_stride, float scale) {
+                                    int S, int Hq, int Hkv, long long dq_stride, long long dkv_stride, float scale, const int2* __restrict__ spans) {
   const long long first = blockIdx.x * (long long)blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
   const long long n_dq = (long long)B * S * Hq * 8;
   const int n_kt = (S + BKV - 1) / BKV;
@@ -127,6 +136,10 @@ __global__ void __launch_bounds__(256) attn_convert_kernel(const float* __restri
         const float4 x = src[j], y = src[16 + j];
         a[4 * j] = x.x; a[4 * j + 1] = x.y; a[4 * j + 2] = x.z; a[4 * j + 3] = x.w;
         z[4 * j] = y.x; z[4 * j + 1] = y.y; z[4 * j + 2] = y.z; z[4 * j + 3] = y.w;
+      }
+      if (RANGES && sees_one_key(spans, t, (int)(t % S))) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = z[j] = 0.f;
       }
       store_gradient(dq + t * dq_stride + h * HD + v, a, z, rope_at(rope, (int)(t % S), v), scale);
     } else {  // a warp: eight keys x four groups of dims (whole lines read, 64 contiguous bytes per key written)

@@ -49,6 +49,7 @@ struct BwdArgs {
   int head_group;      // order of the CTAs (head_group_order)
   int head_parts;      // CTAs that share a key tile of a KV head, each with a part of its query heads
   float scale, scale_log2;
+  const int2* query_spans;  // [B, S] ranges of keys by query; null: causal
   AttnMods mods;
 };
 
@@ -362,6 +363,9 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       tc_fence_after();
       const uint32_t src = (p == 0 ? tdV : tdK) + lane_off + half * 64;
       const float f = p == 0 ? 1.f : args.scale;
+      // a key that only one query sees, which sees nothing else
+      bool alone = false;
+      if (p == 1 && span.y - span.x == 1) alone = sees_one_key(args.query_spans, (long long)b * args.S + span.x, span.x);
       uint8_t* stage = sRing + p * 2 * QTILE + half * ATOM + (warp & 3) * 32 * 128;
 #pragma unroll 1
       for (int c = 0; c < 2; ++c) {
@@ -369,7 +373,8 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         if (n_it > 0) {
           tmem_ld32(src + c * 32, r);
           tmem_ld_wait();
-        } else {
+        }
+        if (n_it == 0 || alone) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
         }
@@ -472,15 +477,16 @@ int capped_blocks(long long threads) {
 
 }  // namespace
 
-// Backward of yf_attn_fwd_mods: key_spans and padding as yf_document_mask gives them (both null: causal), out_lo as the forward pass left it,
+// Backward of yf_attn_fwd_mods: spans, key_spans and padding as yf_document_mask gives them (all null: causal), out_lo as the forward pass left it,
 // or null.  Scratch, results and head_parts as in yf_attn_bwd_parts.
 extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse,
                                 float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv,
                                 int B, int S, int Hq, int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride,
                                 long long do_stride, long long dq_stride, long long dkv_stride, float scale, float softcap, const float* slopes,
-                                const int* key_spans, const int* padding, void* stream) {
+                                const int* spans, const int* key_spans, const int* padding, void* stream) {
   if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || (Hq % Hkv)) return -1;
-  if (!(softcap >= 0.f) || !(scale > 0.f) || (key_spans != nullptr) != (padding != nullptr) || (reinterpret_cast<uintptr_t>(key_spans) & 7)) return -1;
+  if (!(softcap >= 0.f) || !(scale > 0.f) || (key_spans != nullptr) != (padding != nullptr) || (key_spans != nullptr) != (spans != nullptr)) return -1;
+  if ((reinterpret_cast<uintptr_t>(key_spans) | reinterpret_cast<uintptr_t>(spans)) & 7) return -1;
   if (head_parts < 1 || (Hq / Hkv) % head_parts || (head_parts > 1) != (dkv_parts != nullptr)) return -1;
   const int n_kt = (S + BKV - 1) / BKV;
   if (dkv_parts != nullptr && dkv_floats < 4 * part_tile(head_parts, B, 0, n_kt, 0, Hkv, 0, 0)) return -1;
@@ -512,6 +518,7 @@ extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, con
   a.head_group = head_group_size(n_kt, B * Hkv * head_parts, T * Hq * HD * 4, yf_num_sms());  // the dQ accumulator
   a.scale = scale;
   a.scale_log2 = scale * LOG2E;
+  a.query_spans = reinterpret_cast<const int2*>(spans);
   a.mods = attn_mods(scale, softcap, slopes, key_spans, padding);
   // D, and the dQ accumulator cleared on the way
   const auto pre = out_lo != nullptr ? attn_delta_kernel<true> : attn_delta_kernel<false>;
@@ -521,8 +528,8 @@ extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, con
                                   : (slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS> : launch<MOD_SPANS>);
   if (int rc = main(m, a, (int)ctas, st)) return rc;
   const long long items = T * Hq * 8 + (dkv_parts ? (long long)B * n_kt * Hkv * 2 * BKV * 8 : 0);
-  attn_convert_kernel<<<capped_blocks(items), 256, 0, st>>>(dq_accum, a.dkv_parts, head_parts, nullptr, reinterpret_cast<__nv_bfloat16*>(dq),
+  attn_convert_kernel<true><<<capped_blocks(items), 256, 0, st>>>(dq_accum, a.dkv_parts, head_parts, nullptr, reinterpret_cast<__nv_bfloat16*>(dq),
                                                             reinterpret_cast<__nv_bfloat16*>(dk), reinterpret_cast<__nv_bfloat16*>(dv), B, S, Hq, Hkv,
-                                                            dq_stride, dkv_stride, scale);
+                                                            dq_stride, dkv_stride, scale, a.query_spans);
   return -(int)cudaGetLastError();
 }

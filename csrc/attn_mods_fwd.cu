@@ -18,10 +18,12 @@
 // warps rescales its rows of O in TMEM and their sums); the final division by the row sum makes the result exact again.  A row's bits depend
 // on the 32 rows that share its warps.
 // Bound: per 64 keys of two tiles the products take 1280 cycles (an MMA of 16 x 128 rows 48 at N = 64 and 64 at N = 128), the exponentials 1024, on
-// different pipes; about 2000 pass, in the chain S, softmax, P V of a half.  S for 128 keys at once, 1024 cycles of products, takes more of it (599 us
-// at the sizes below: its next S waits for the whole P), as does one thread that issues for both tiles (643 us).
-// bf16, 32 heads, causal, 1 x 8192: 522 us, 1050 TFLOP/s; in packed documents of 5 to 8000 tokens 139 us, 158 with a block for each piece; scores
-// capped 650 us.  64 heads, 2 x 4096 with prefixes and a distance bias 848 us.
+// different pipes; about 2100 pass.  A softmax warp spends 600 to 1000 of its 2000 on exponentials and the rest on latencies (S out of TMEM 350,
+// the maximum 150, the pair's barrier 240, P into TMEM and the next S 400), and the four of an SM partition tend to do either together.  What was tried:
+// S for 128 keys at once, 1024 cycles of products (599 us at the sizes below: its next S waits for the whole P); one thread that issues for both tiles
+// (643); a warp for 64 keys, the two of a row in turn (562: S waits for a longer softmax); the tiles' exponentials in turn (540).
+// bf16, 32 heads, causal, 1 x 8192: 545 us, 1010 TFLOP/s; in packed documents of 5 to 8000 tokens 145 us, 163 with a block for each piece; scores
+// capped 655 us.  64 heads, 2 x 4096 with prefixes and a distance bias 870 us.
 #include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
@@ -404,6 +406,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       const int qrow = now[0].x * args.tiles * BQ + i * BQ + q * 32 + lane;
       float m_run = -INFINITY;                 // reference maximum of the exponent
       float l_run = 0.f;                       // sum over this thread's keys
+      float l_off = 0.f;                       // what rounding to bf16 adds to the largest of every 32 keys
       int2 span = make_int2(0, qrow + 1);      // keys [x, y) of this row
       if (args.mods.spans != nullptr || qrow >= args.S) span = qrow < args.S ? __ldg(args.mods.spans + (long long)now[0].z * args.S + qrow) : make_int2(0, 0);
       const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[now[0].y] * LOG2E : 0.f;
@@ -461,6 +464,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
               tmem_st16(tO + c * 16, r);
             }
             l_run *= alpha;
+            l_off *= alpha;
           }
           m_run = m_new;
         }
@@ -476,6 +480,8 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           packed[e] = pack_bf16x2(p0, p1);
         }
         tmem_st16(tS + u * HKV + half * 16, packed);
+        const float top = fast_exp2(fmaf(mx, to_log2, neg_ms));
+        l_off += __bfloat162float(__float2bfloat16_rn(top)) - top;
         const float2 two = f32x2_split(sum);
         l_run += two.x + two.y;
         tmem_st_wait();
@@ -502,11 +508,17 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[i * 2 + u], ((ph >> u) & 1) ^ 1, 424 + i));
         *mine = l_run;
         if (named_bar_or(bar, 64, !alive)) alive = false;
+        l_run = half == 0 ? l_run + *theirs : *theirs + l_run;
+        named_bar_sync(bar, 64);
+        *mine = l_off;
+        named_bar_sync(bar, 64);
+        l_off += *theirs;
       }
       if (worked && alive) {
         tc_fence_after();
-        const float l = half == 0 ? l_run + *theirs : *theirs + l_run;
-        const float inv = (l > 0.f) ? 1.f / l : 0.f;
+        // P V has the rounded P of the largest keys, and so has the sum that it is divided by (0.0021 instead of 0.0023 of O off over documents of
+        // some 400 tokens, and one key alone gives exactly its V).  The backward pass works with unrounded P: lse takes their sum.
+        const float l = l_run, inv = (l > 0.f) ? 1.f / (l + l_off) : 0.f;
         // The warp's 32 rows x 64 columns go out through the place of Q, which the tile's last product has read, and TMA (which leaves out the
         // rows past the end): a thread's own 16 bytes at a time touch 32 lines with each instruction.
         uint8_t* stage = sQ + q_stage(places, i) * TILE + half * ATOM + q * 32 * 128;

@@ -107,8 +107,8 @@ int yf_attn_bwd_parts(const void* q, const void* k, const void* v, const void* o
                       int Hkv, long long q_stride, long long kv_stride, long long o_stride, long long do_stride, long long dq_stride,
                       long long dkv_stride, float scale, int causal, void* stream);
 
-/* The same with scores capped at +-softcap (0: not), less slopes[h] * distance (fp32, null: not), and ranges of keys (queries in the backward
-   pass) for every token, as yf_document_mask gives them (null: causal).  A token without keys: zeros, lse -inf.  out_lo (may be null): what rounding
+/* The same with scores capped at +-softcap (0: not), less slopes[h] * distance (fp32, null: not), and ranges of keys (and of queries, in the
+   backward pass) for every token, as yf_document_mask gives them (null: causal).  A token without keys: zeros, lse -inf.  out_lo (may be null): what rounding
    the output left over, laid out like it. */
 int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, int B, int S, int Hq, int Hkv, long long q_stride,
                      long long k_stride, long long v_stride, long long out_stride, float scale, float softcap, const float* slopes, const int* spans,
@@ -116,7 +116,8 @@ int yf_attn_fwd_mods(const void* q, const void* k, const void* v, void* out, voi
 int yf_attn_bwd_mods(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse,
                      float* delta, float* dq_accum, float* dkv_parts, long long dkv_floats, int head_parts, void* dq, void* dk, void* dv, int B, int S, int Hq,
                      int Hkv, long long q_stride, long long k_stride, long long v_stride, long long o_stride, long long do_stride,
-                     long long dq_stride, long long dkv_stride, float scale, float softcap, const float* slopes, const int* key_spans, const int* padding, void* stream);
+                     long long dq_stride, long long dkv_stride, float scale, float softcap, const float* slopes, const int* spans, const int* key_spans, const int* padding,
+                     void* stream);
 
 // No counterpart in the reference.  yf_attn_bwd for callers that cannot allocate device memory (a plain C host
 // without a tensor framework, or a job whose own pool already holds the whole GPU): the delta / dQ-accumulator

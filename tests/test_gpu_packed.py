@@ -268,7 +268,7 @@ def test_attention_shared_key_tiles(hq, hkv):
         out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, 0.1, cap, sl, m.spans, m.padding)
         dout, got = torch.randn_like(out), []
         for parts in [p for p in range(1, hq // hkv + 1) if (hq // hkv) % p == 0]:
-            got.append(kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, 0.1, cap, sl, m.key_spans, m.padding, head_parts=parts))
+            got.append(kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, 0.1, cap, sl, m.spans, m.key_spans, m.padding, head_parts=parts))
         _done()
         for g in got[1:]:
             for a, z in zip(g, got[0]):
@@ -572,7 +572,7 @@ def test_attention_rows_far_apart():
     results = []
     for args in ((q, k, v), [t.detach().contiguous() for t in near]):
         out, low, lse = kernels.attn_fwd_mods(*args, 0.1, 0.0, None, mask.spans, mask.padding)
-        results.append((out, low, lse, *kernels.attn_bwd_mods(*args, out, low, dout, lse, 0.1, 0.0, None, mask.key_spans, mask.padding)[1:]))
+        results.append((out, low, lse, *kernels.attn_bwd_mods(*args, out, low, dout, lse, 0.1, 0.0, None, mask.spans, mask.key_spans, mask.padding)[1:]))
     _done()
     assert all(torch.equal(a, z) for a, z in zip(*results))
 
@@ -660,3 +660,26 @@ def test_attention_refuses_too_many_rows():
     t = torch.empty(65536, 1, 1, 128, device=DEV, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         Fn.attention(t, t, t)
+
+
+@pytest.mark.parametrize("s,window,mean", [(1, 0, 1), (1, 1, 1), (300, 1, 50), (300, 0, 1), (300, 0, 3)])
+@pytest.mark.parametrize("softcap,biased,hkv", [(0.0, False, 4), (30.0, True, 1)])
+def test_tokens_that_see_one_key(s, window, mean, softcap, biased, hkv):
+    """The probability of an only key is 1: the output is its value to the bit, and neither q nor a key that nothing else looks at gets a gradient."""
+    from yafsdp_b200.ops import functional as Fn
+
+    b, hq = 3, 4
+    mask = Fn.document_mask((_ids(b, s, mean, False) if mean > 1 else torch.arange(s).expand(b, s)).to(DEV), window=window)
+    slopes = torch.rand(hq, device=DEV) if biased else None
+    for m in (mask, None) if s == 1 else (mask,):
+        q, k, v = _qkv(b, s, hq, hkv)
+        out = Fn.attention(q, k, v, m, softcap=softcap, slopes=slopes)
+        dq, dk, dv = torch.autograd.grad(out, (q, k, v), torch.randn_like(out))
+        one = mask.spans[..., 1] - mask.spans[..., 0] == 1
+        at = mask.spans[..., 0].long()
+        values = v.detach().repeat_interleave(hq // hkv, 2).gather(1, at[..., None, None].expand(b, s, hq, 128))
+        assert one.any() and torch.equal(out[one], values[one])
+        assert (dq[one] == 0).all() and (one.all() or (dq[~one] != 0).any())
+        only = (mask.key_spans[..., 1] - mask.key_spans[..., 0] == 1) & one.gather(1, mask.key_spans[..., 0].long().clamp(max=s - 1))
+        assert (dk[only] == 0).all() and (dv != 0).any()
+    _done()

@@ -175,7 +175,7 @@ def _declare(l: ctypes.CDLL) -> None:
         "yf_attn_bwd_parts": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _F, _I, _P],
         "yf_attn_bwd_noalloc": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _F, _I, _P],
         "yf_attn_fwd_mods": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _F, _F, _P, _P, _P, _P],
-        "yf_attn_bwd_mods": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _F, _F, _P, _P, _P, _P],
+        "yf_attn_bwd_mods": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _F, _F, _P, _P, _P, _P, _P],
         "yf_document_mask": [_P, _I, _P, _P, _P, _P, _P, _I, _I, _L, _L, _I, _P],
         "yf_rotary": [_P, _P, _P, _P, _P, _I, _L, _P, _L, _I, _I, _I, _L, _L, _L, _L, _L, _L, _I, _I, _P],
         "yf_residual_norm_fwd": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _F, _F, _I, _P],

@@ -575,14 +575,14 @@ class AttentionFn(torch.autograd.Function):
                 slopes: torch.Tensor | None) -> torch.Tensor:
         spans, key_spans, padding = (None, None, None) if mask is None else (mask.spans, mask.key_spans, mask.padding)
         out, out_lo, lse = kernels.attn_fwd_mods(q, k, v, scale, softcap, slopes, spans, padding)
-        ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes, key_spans, padding)
+        ctx.save_for_backward(q, k, v, out, out_lo, lse, slopes, spans, key_spans, padding)
         ctx.args = (scale, softcap)
         return out
 
     @staticmethod
     def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
-        q, k, v, out, out_lo, lse, slopes, key_spans, padding = ctx.saved_tensors
-        return *kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *ctx.args, slopes, key_spans, padding), None, None, None, None
+        q, k, v, out, out_lo, lse, slopes, spans, key_spans, padding = ctx.saved_tensors
+        return *kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *ctx.args, slopes, spans, key_spans, padding), None, None, None, None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None = None, *, scale: float | None = None, softcap: float = 0.0,

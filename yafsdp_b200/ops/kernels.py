@@ -512,8 +512,8 @@ def attn_fwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: floa
 
 
 def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, out_lo: torch.Tensor | None, dout: torch.Tensor,
-                  lse: torch.Tensor, scale: float, softcap: float, slopes: torch.Tensor | None, key_spans: torch.Tensor | None,
-                  padding: torch.Tensor | None, head_parts: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                  lse: torch.Tensor, scale: float, softcap: float, slopes: torch.Tensor | None, spans: torch.Tensor | None,
+                  key_spans: torch.Tensor | None, padding: torch.Tensor | None, head_parts: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(dq, dk, dv)`` of :func:`attn_fwd_mods`, whose results ``out``, ``out_lo`` and ``lse`` are.  ``head_parts``: as in :func:`attn_bwd`."""
     b, s, hq, _ = q.shape
     hkv = k.shape[2]
@@ -532,7 +532,7 @@ def attn_bwd_mods(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.
     _check(_native.lib().yf_attn_bwd_mods(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(out_lo), dout.data_ptr(), lse.data_ptr(),
                                           at + 4 * (n_dq + n_parts), at, at + 4 * n_dq if n_parts else None, n_parts, parts, dq.data_ptr(), dk.data_ptr(),
                                           dv.data_ptr(), b, s, hq, hkv, qs, ks, vs, hq * 128, gs, hq * 128, hkv * 128, scale, softcap, _ptr(slopes),
-                                          _ptr(key_spans), _ptr(padding), _stream()), "yf_attn_bwd_mods")
+                                          _ptr(spans), _ptr(key_spans), _ptr(padding), _stream()), "yf_attn_bwd_mods")
     _launches += 2  # delta pre-pass and dq conversion post-pass
     return dq, dk, dv
 
