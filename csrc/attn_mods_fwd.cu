@@ -11,9 +11,8 @@
 //   warps 18, 19  MMA: S = Q K^T, one warp for each tile, half block by half block
 //   warps 2-9     softmax of tile 0, warps 10-17 of tile 1: two threads per query row (TMEM lane == row), 32 keys of a half block each
 // A tile's output leaves through the place of its Q, which is why there are three: the next piece's first tile has its Q, and S, while this one's goes out.
-// TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  S_i is two halves of 64 columns which take turns; a half's P (bf16, 32 columns)
-// takes the place of part of its S, whose row its two threads have read into registers, and is the MMA's A operand from there, under the softmax of
-// the other half.
+// TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  S_i is two halves of 64 columns which take turns; a thread's P (bf16, 16 columns)
+// takes the place of half of the S that it has read into registers, and is the MMA's A operand from there, under the softmax of the other half.
 // The exponent's reference maximum is only moved when some row of a warp has grown by more than 2^8 since it was set (then its pair of
 // warps rescales its rows of O in TMEM and their sums); the final division by the row sum makes the result exact again.  A row's bits depend
 // on the 32 rows that share its warps.
@@ -22,8 +21,8 @@
 // the maximum 150, the pair's barrier 240, P into TMEM and the next S 400), and the four of an SM partition tend to do either together.  What was tried:
 // S for 128 keys at once, 1024 cycles of products (599 us at the sizes below: its next S waits for the whole P); one thread that issues for both tiles
 // (643); a warp for 64 keys, the two of a row in turn (562: S waits for a longer softmax); the tiles' exponentials in turn (540).
-// bf16, 32 heads, causal, 1 x 8192: 545 us, 1010 TFLOP/s; in packed documents of 5 to 8000 tokens 145 us, 163 with a block for each piece; scores
-// capped 655 us.  64 heads, 2 x 4096 with prefixes and a distance bias 870 us.
+// bf16, 32 heads, causal, 1 x 8192: 520 us, 1055 TFLOP/s; in packed documents of 5 to 8000 tokens 143 us, 160 with a block for each piece; scores
+// capped 660 us.  64 heads, 2 x 4096 with prefixes and a distance bias 870 us.
 #include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
@@ -316,8 +315,8 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
             const uint64_t v = dV + (uint32_t)(vs * (TILE >> 4) + u * (HKV * 128 >> 4));
             const uint32_t p = tmem_base + i * 128 + u * HKV;
 #pragma unroll
-            for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V
-              tc_mma_bf16_ts(tmem_base + 256 + i * 128, p + e * 8, v + e * (2048 >> 4), idesc_o, t != lo || e != 0);
+            for (int e = 0; e < HKV / 16; ++e)  // 16 keys: 8 TMEM columns of P, 16 rows of V; two of them a thread
+              tc_mma_bf16_ts(tmem_base + 256 + i * 128, p + (e >> 1) * 32 + (e & 1) * 8, v + e * (2048 >> 4), idesc_o, t != lo || e != 0);
             tc_commit(&o_done[i * 2 + u]);
           }
           tc_commit(&v_empty[vs]);
@@ -410,6 +409,13 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       int2 span = make_int2(0, qrow + 1);      // keys [x, y) of this row
       if (args.mods.spans != nullptr || qrow >= args.S) span = qrow < args.S ? __ldg(args.mods.spans + (long long)now[0].z * args.S + qrow) : make_int2(0, 0);
       const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[now[0].y] * LOG2E : 0.f;
+      float top = -INFINITY;                   // exponent of the largest P, of the half block before for a while
+      // Under the next half block's maximum (causal 520 us, 529 at once), or at once where caps make the registers scarce (660 us, 680 later).
+      constexpr bool LATER = !(MODS & MOD_CAP);
+      auto add_off = [&]() {
+        const float p = fast_exp2(top);
+        l_off += __bfloat162float(__float2bfloat16_rn(p)) - p;
+      };
       const bool worked = lo < hi;
       for (int t = lo; t < hi; ++t) {
         const int u = t & 1;
@@ -441,8 +447,8 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           mx2[1] = fmax3(mx2[1], __uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3]));
         }
         const float mx = fmaxf(fmax3(mx2[0], __uint_as_float(sc[30]), __uint_as_float(sc[31])), mx2[1]);
+        if (LATER) add_off();
         const bool grew = !alive || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * to_log2 > RESCALE_LOG2));
-        // Behind this barrier both threads of a row have read their parts of S, so P may take its place.
         if (named_bar_or(bar, 64, grew)) {
           if (*gone == t + 1) { alive = false; break; }  // not a later half block's: who gives up there waits for this warp there
           *mine = mx;
@@ -479,9 +485,9 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           sum = add_f32x2(sum, f32x2(p0, p1));
           packed[e] = pack_bf16x2(p0, p1);
         }
-        tmem_st16(tS + u * HKV + half * 16, packed);
-        const float top = fast_exp2(fmaf(mx, to_log2, neg_ms));
-        l_off += __bfloat162float(__float2bfloat16_rn(top)) - top;
+        tmem_st16(tS + u * HKV + half * 32, packed);
+        top = fmaf(mx, to_log2, neg_ms);
+        if (!LATER) add_off();
         const float2 two = f32x2_split(sum);
         l_run += two.x + two.y;
         tmem_st_wait();
@@ -506,6 +512,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         // the output of the last half block, and the sum of both threads
         const int u = (hi - 1) & 1;
         alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[i * 2 + u], ((ph >> u) & 1) ^ 1, 424 + i));
+        if (LATER) add_off();
         *mine = l_run;
         if (named_bar_or(bar, 64, !alive)) alive = false;
         l_run = half == 0 ? l_run + *theirs : *theirs + l_run;
