@@ -5,9 +5,8 @@
 #pragma once
 #include "common.cuh"
 
-constexpr int MOD_SPANS = 1;  // ranges from memory, or causal without any
-constexpr int MOD_CAP = 2;
-constexpr int MOD_BIAS = 4;
+constexpr int MOD_CAP = 1;
+constexpr int MOD_BIAS = 2;
 
 struct AttnMods {
   const int2* spans;    // [B, S] by query (forward) or by key (backward); null: causal

@@ -16,8 +16,11 @@
 //   warp 23          the query rows' statistics for the ring, read one step ahead; clears padded rows of tiles that have some
 // TMEM (512 columns): dV, dK (128 each) and two sets (even / odd steps) of [S^T | dP^T], 64 columns each: P^T and dS^T
 // (bf16, 8 + 8 columns per 16 queries) replace S^T once it has been read, dQ^T replaces dP^T.  So the softmax of one step runs under
-// the MMAs of its neighbours.  Bound: about 1700 cycles of MMA per step (S^T, dP^T and dQ^T with N = 64 are limited by the
-// 128 bytes per cycle that shared memory delivers: 48 instead of 32 cycles per instruction).
+// the MMAs of its neighbours.  Bound: about 1700 cycles of MMA per step (S^T, dP^T and dQ^T with N = 64 take 48 instead of 32 cycles per
+// instruction: shared memory delivers 128 bytes a cycle), and about 2300 of the shared-memory port with what else a step moves through it, 176 KB of
+// operands, 32 of loads, 16 of dS^T and 64 of dQ^T; 2750 pass.
+// bf16, 32 heads, causal, 1 x 8192: 1510 us with the passes before and after (82), 910 TFLOP/s; scores capped 1700; 32 / 8 heads in packed documents
+// of 5 to 8000 tokens 425.  Straight from registers (`red`) dQ took 1670 instead of 1520; with K and V loaded behind the ranges, 1520.
 // D = rowsum(dO * O) comes from a small pre-pass; scale and bf16 of dQ are applied by a post-pass, of dK at the end.
 #include "attn_bwd_common.cuh"
 #include "attn_mods.cuh"
@@ -524,8 +527,8 @@ extern "C" int yf_attn_bwd_mods(const void* q, const void* k, const void* v, con
   const auto pre = out_lo != nullptr ? attn_delta_kernel<true> : attn_delta_kernel<false>;
   pre<<<capped_blocks(T * Hq * 16), 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(out), reinterpret_cast<const __nv_bfloat16*>(out_lo),
                                                   reinterpret_cast<const __nv_bfloat16*>(dout), delta, dq_accum, B, S, Hq, o_stride, do_stride);
-  const auto main = softcap > 0.f ? (slopes != nullptr ? launch<MOD_SPANS | MOD_CAP | MOD_BIAS> : launch<MOD_SPANS | MOD_CAP>)
-                                  : (slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS> : launch<MOD_SPANS>);
+  const auto main = softcap > 0.f ? (slopes != nullptr ? launch<MOD_CAP | MOD_BIAS> : launch<MOD_CAP>)
+                                  : (slopes != nullptr ? launch<MOD_BIAS> : launch<0>);
   if (int rc = main(m, a, (int)ctas, st)) return rc;
   const long long items = T * Hq * 8 + (dkv_parts ? (long long)B * n_kt * Hkv * 2 * BKV * 8 : 0);
   attn_convert_kernel<true><<<capped_blocks(items), 256, 0, st>>>(dq_accum, a.dkv_parts, head_parts, nullptr, reinterpret_cast<__nv_bfloat16*>(dq),

@@ -633,6 +633,6 @@ extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, voi
   a.mods = attn_mods(scale, softcap, slopes, spans, padding);
   a.mods.out_lo = reinterpret_cast<__nv_bfloat16*>(out_lo);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (softcap > 0.f) return slopes != nullptr ? launch<MOD_SPANS | MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<MOD_SPANS | MOD_CAP>(*mq, *mk, *mv, *mo, *ml, a, st);
-  return slopes != nullptr ? launch<MOD_SPANS | MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<MOD_SPANS>(*mq, *mk, *mv, *mo, *ml, a, st);
+  if (softcap > 0.f) return slopes != nullptr ? launch<MOD_CAP | MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<MOD_CAP>(*mq, *mk, *mv, *mo, *ml, a, st);
+  return slopes != nullptr ? launch<MOD_BIAS>(*mq, *mk, *mv, *mo, *ml, a, st) : launch<0>(*mq, *mk, *mv, *mo, *ml, a, st);
 }
