@@ -628,6 +628,7 @@ extern "C" int yf_attn_fwd_mods(const void* q, const void* k, const void* v, voi
   a.S = S; a.B = B; a.Hq = Hq; a.Hkv = Hkv;
   a.scale = scale;
   a.scale_log2 = scale * LOG2E;
+  // 1 x 512 tokens, 32 heads 13.0 us with one tile a piece, 15.2 with two; 1 x 777, 16 heads 17.1 and 19.7; 1 x 333, 40 heads 11.4 and 11.1
   a.tiles = (long long)((S + BQ - 1) / BQ) * Hq * B <= yf_num_sms() ? 1 : 2;
   a.more = (long long)((S + BQ * a.tiles - 1) / (BQ * a.tiles)) * Hq * B > yf_num_sms();
   a.mods = attn_mods(scale, softcap, slopes, spans, padding);
