@@ -19,10 +19,10 @@
 // Bound: per 64 keys of two tiles the products take 1280 cycles (an MMA of 16 x 128 rows 48 at N = 64 and 64 at N = 128), the exponentials 1024, on
 // different pipes; about 2100 pass.  A softmax warp spends 600 to 1000 of its 2000 on exponentials and the rest on latencies (S out of TMEM 350,
 // the maximum 150, the pair's barrier 240, P into TMEM and the next S 400), and the four of an SM partition tend to do either together.  What was tried:
-// S for 128 keys at once, 1024 cycles of products (599 us at the sizes below: its next S waits for the whole P); one thread that issues for both tiles
+// S for 128 keys at once, 1024 cycles of products (599 us at the sizes below, 515 with halves then: its next S waits for the whole P); one thread that issues for both tiles
 // (643); a warp for 64 keys, the two of a row in turn (562: S waits for a longer softmax); the tiles' exponentials in turn (540).
-// bf16, 32 heads, causal, 1 x 8192: 520 us, 1055 TFLOP/s; in packed documents of 5 to 8000 tokens 143 us, 160 with a block for each piece; scores
-// capped 660 us.  64 heads, 2 x 4096 with prefixes and a distance bias 870 us.
+// bf16, 32 heads, causal, 1 x 8192: 502 us, 1095 TFLOP/s; in packed documents of 5 to 8000 tokens 137 us, 155 with a block for each piece; scores
+// capped 675 us.  64 heads, 2 x 4096 with prefixes and a distance bias 832 us.
 #include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
@@ -392,7 +392,6 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     constexpr float RESCALE_LOG2 = 8.f;      // move the reference maximum when a row's maximum exceeds it by 2^8
     // scores that were transformed are in units of log2 already
     const float to_log2 = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
-    const uint64_t to_log2_2 = f32x2(to_log2, to_log2);
     uint32_t ph = 0;                         // phase of s_full and o_done, a bit for each half
     bool alive = true;
     for (int n = 0;; ++n) {
@@ -410,9 +409,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       if (args.mods.spans != nullptr || qrow >= args.S) span = qrow < args.S ? __ldg(args.mods.spans + (long long)now[0].z * args.S + qrow) : make_int2(0, 0);
       const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[now[0].y] * LOG2E : 0.f;
       float top = -INFINITY;                   // exponent of the largest P, of the half block before for a while
-      // Under the next half block's maximum (causal 520 us, 529 at once), or at once where caps make the registers scarce (660 us, 680 later).
-      constexpr bool LATER = !(MODS & MOD_CAP);
-      auto add_off = [&]() {
+      auto add_off = [&]() {  // under the next half block's maximum (causal 520 us, 529 at once)
         const float p = fast_exp2(top);
         l_off += __bfloat162float(__float2bfloat16_rn(p)) - p;
       };
@@ -425,13 +422,10 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         ph ^= 1u << u;
         const int kv0 = t * HKV + half * 32;
         uint32_t sc[32];
-        if (alive) {
-          tc_fence_after();
-          tmem_ld32(tS + u * HKV + half * 32, sc);
-          tmem_ld_wait();
-        } else {
-          *gone = t + 1;
-        }
+        if (!alive) *gone = t + 1;
+        tc_fence_after();
+        tmem_ld32(tS + u * HKV + half * 32, sc);  // (of a dead walk too: branches around it cost a move for each score)
+        tmem_ld_wait();
         if (MODS & MOD_CAP) cap_scores(sc, args.mods);
         if (MODS & MOD_BIAS) add_bias(sc, (MODS & MOD_CAP) ? 1.f : sl2, slope, (float)(kv0 - qrow), span.y > qrow + 1 ? 0 : -1);
         if (kv0 < span.x || kv0 + 32 > span.y) {  // the ends of a row's range
@@ -447,7 +441,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           mx2[1] = fmax3(mx2[1], __uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3]));
         }
         const float mx = fmaxf(fmax3(mx2[0], __uint_as_float(sc[30]), __uint_as_float(sc[31])), mx2[1]);
-        if (LATER) add_off();
+        add_off();
         const bool grew = !alive || (mx != -INFINITY && (m_run == -INFINITY || (mx - m_run) * to_log2 > RESCALE_LOG2));
         if (named_bar_or(bar, 64, grew)) {
           if (*gone == t + 1) { alive = false; break; }  // not a later half block's: who gives up there waits for this warp there
@@ -475,19 +469,18 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
           m_run = m_new;
         }
         const float neg_ms = (m_run == -INFINITY) ? 0.f : -m_run * to_log2;
-        const uint64_t neg_ms_2 = f32x2(neg_ms, neg_ms);
         uint64_t sum = f32x2(0.f, 0.f);
         uint32_t packed[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 y = f32x2_split(fma_f32x2(f32x2(__uint_as_float(sc[2 * e]), __uint_as_float(sc[2 * e + 1])), to_log2_2, neg_ms_2));
+          // (pairs of products in one instruction cost moves here, 520 us)
+          const float2 y = make_float2(fmaf(__uint_as_float(sc[2 * e]), to_log2, neg_ms), fmaf(__uint_as_float(sc[2 * e + 1]), to_log2, neg_ms));
           const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
           sum = add_f32x2(sum, f32x2(p0, p1));
           packed[e] = pack_bf16x2(p0, p1);
         }
         tmem_st16(tS + u * HKV + half * 32, packed);
         top = fmaf(mx, to_log2, neg_ms);
-        if (!LATER) add_off();
         const float2 two = f32x2_split(sum);
         l_run += two.x + two.y;
         tmem_st_wait();
@@ -512,7 +505,7 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
         // the output of the last half block, and the sum of both threads
         const int u = (hi - 1) & 1;
         alive = alive && __all_sync(0xffffffffu, mbar_wait(&o_done[i * 2 + u], ((ph >> u) & 1) ^ 1, 424 + i));
-        if (LATER) add_off();
+        add_off();
         *mine = l_run;
         if (named_bar_or(bar, 64, !alive)) alive = false;
         l_run = half == 0 ? l_run + *theirs : *theirs + l_run;
