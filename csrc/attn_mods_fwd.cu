@@ -13,16 +13,17 @@
 // A tile's output leaves through the place of its Q, which is why there are three: the next piece's first tile has its Q, and S, while this one's goes out.
 // TMEM (512 columns): S_0, S_1, O_0, O_1, 128 columns of fp32 each.  S_i is two halves of 64 columns which take turns; a thread's P (bf16, 16 columns)
 // takes the place of half of the S that it has read into registers, and is the MMA's A operand from there, under the softmax of the other half.
-// The exponent's reference maximum is only moved when some row of a warp has grown by more than 2^8 since it was set (then its pair of
+// The exponent's reference maximum is only moved when some row of a warp has grown by more than 2^40 since it was set (then its pair of
 // warps rescales its rows of O in TMEM and their sums); the final division by the row sum makes the result exact again.  A row's bits depend
 // on the 32 rows that share its warps.
 // Bound: per 64 keys of two tiles the products take 1280 cycles (an MMA of 16 x 128 rows 48 at N = 64 and 64 at N = 128), the exponentials 1024, on
 // different pipes; about 2100 pass.  A softmax warp spends 600 to 1000 of its 2000 on exponentials and the rest on latencies (S out of TMEM 350,
 // the maximum 150, the pair's barrier 240, P into TMEM and the next S 400), and the four of an SM partition tend to do either together.  What was tried:
-// S for 128 keys at once, 1024 cycles of products (599 us at the sizes below, 515 with halves then: its next S waits for the whole P); one thread that issues for both tiles
-// (643); a warp for 64 keys, the two of a row in turn (562: S waits for a longer softmax); the tiles' exponentials in turn (540).
-// bf16, 32 heads, causal, 1 x 8192: 502 us, 1095 TFLOP/s; in packed documents of 5 to 8000 tokens 137 us, 155 with a block for each piece; scores
-// capped 675 us.  64 heads, 2 x 4096 with prefixes and a distance bias 832 us.
+// S for 128 keys at once, 1024 cycles of products (599 us at the sizes below, where halves took 515: its next S waits for the whole P); one thread that
+// issues for both tiles (643); a warp for 64 keys, the two of a row in turn (562: S waits for a longer softmax); the tiles' exponentials in turn (540); the
+// exponentials before it is known whether a row has grown (511, packed 144: they are taken twice too often).
+// bf16, 32 heads, causal, 1 x 8192: 502 us, 1095 TFLOP/s; in packed documents of 5 to 8000 tokens 135 us, 155 with a block for each piece; scores
+// capped 672 us.  64 heads, 2 x 4096 with prefixes and a distance bias 757 us.
 #include "attn_mods.cuh"
 #include "common.cuh"
 #include "yafsdp_b200.h"
@@ -389,7 +390,9 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     float* theirs = sRow + (i * 2 + (half ^ 1)) * BQ + q * 32 + lane;
     volatile int* gone = dead + i * 4 + q;
     const float sl2 = args.scale_log2;
-    constexpr float RESCALE_LOG2 = 8.f;      // move the reference maximum when a row's maximum exceeds it by 2^8
+    // The reference maximum is moved when a row's maximum exceeds it by 2^40: P, its sums and O in fp32 keep their relative accuracy at any
+    // reference, and stay finite for V up to 10^22 over 10^4 keys.  (By 2^8, with the distance bias of the 64 heads 832 instead of 757 us.)
+    constexpr float RESCALE_LOG2 = 40.f;
     // scores that were transformed are in units of log2 already
     const float to_log2 = (MODS & (MOD_CAP | MOD_BIAS)) ? 1.f : sl2;
     uint32_t ph = 0;                         // phase of s_full and o_done, a bit for each half

@@ -39,7 +39,11 @@ def spans_of(ids, prefix, window):
 def attention(q, k, v, seen, scale, softcap, slopes, dout=None):
     """Output, gradients and, for each, how far bf16 kernels may be off: probabilities, score gradients and results are rounded to bf16
     (half a step each, relative), the row sums D = dO . O read the rounded output; everything else is fp32, 2^-14 of the terms in all
-    (exponents up to 2^6 and their exponentials to 2^-20, sums of some hundred terms).  ``seen``: [B, S, S]."""
+    (exponents up to 2^6 and their exponentials to 2^-20, sums of some hundred terms).  ``seen``: [B, S, S].
+
+    With weights w_j = p_j / l, roundings d_j <= u of them, and those of some keys T (the largest ones) taken into the sum that is divided by, the
+    output before its own rounding is sum (1 + d_j) w_j v_j / (1 + sum_T d_j w_j), off to first order by sum_T d_j w_j (v_j - o) + sum_rest d_j w_j v_j
+    <= u (mass + |o| sum_T w_j) <= u (mass + |o|), where mass = sum w_j |v_j|."""
     u, f = 2.0**-8, 2.0**-14
     q, k, v = (t.double() for t in (q, k, v))
     b, s, hq, d = q.shape
@@ -56,7 +60,7 @@ def attention(q, k, v, seen, scale, softcap, slopes, dout=None):
     p = x.masked_fill(~seen[:, None] & some, -math.inf).softmax(-1) * some
     o = torch.einsum("bhij,bjhd->bihd", p, ve)
     mass = torch.einsum("bhij,bjhd->bihd", p, ve.abs())
-    o_off = u * (mass + o.abs()) + f * mass
+    o_off = u * (mass + 2 * o.abs()) + f * mass  # roundings of P, taken into its sum or not, and of the output
     if dout is None:
         return o, o_off
     g = dout.double()
