@@ -683,3 +683,27 @@ def test_tokens_that_see_one_key(s, window, mean, softcap, biased, hkv):
         only = (mask.key_spans[..., 1] - mask.key_spans[..., 0] == 1) & one.gather(1, mask.key_spans[..., 0].long().clamp(max=s - 1))
         assert (dk[only] == 0).all() and (dv != 0).any()
     _done()
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_attention_of_scores_that_grow_along_the_row(turned):
+    """Keys ten times as long at the end of a row as at its start, or the other way round: references that have to move by more than 2^40, or that
+    stay far above what comes later."""
+    from yafsdp_b200.ops import functional as Fn
+
+    b, s, hq, hkv = 2, 300, 4, 2
+    q, k, v = (t.detach() for t in _qkv(b, s, hq, hkv))
+    growth = 1 + torch.arange(s, device=DEV) / 32
+    k = (k.float() * (growth.flip(0) if turned else growth)[:, None, None]).bfloat16()
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = Fn.attention(q, k, v)
+    dout = torch.randn(out.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    _done()
+    want = oracle.attention(q.detach(), k.detach(), v.detach(), _seen(None, b, s), 128**-0.5, 0.0, None, dout)
+    scores = torch.einsum("bihd,bjhd->bhij", q.detach().float(), k.detach().float().repeat_interleave(2, 2)) * 128**-0.5 * 1.4427
+    scores = scores.masked_fill(~_seen(None, b, s)[:, None], -math.inf)
+    moved = scores.amax(-1) - scores[..., :64].amax(-1)
+    assert turned or (moved > 40).any()
+    for name, got, w in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
+        oracle.close(got.detach(), w, name)
