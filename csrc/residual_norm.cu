@@ -62,7 +62,7 @@ struct NormArgs {
   const void *x, *y, *weight, *post, *gate;  // post, gate: may be null
   void *h, *n;
   float* rstd;  // [T, 2]: r_y (with post), r_h; may be null
-  const void *dh, *dn;  // either may be null: zeros
+  const void *dh, *dn;  // one of them may be null: zeros
   void *dx, *dy, *dgate;
   float *w_parts, *z_parts;  // [CTAs, D]: sums of dn hhat and of g yhat (g y without post; gate g yhat with a gate per token)
   float scale, eps;
@@ -221,10 +221,11 @@ __global__ void __launch_bounds__(BLOCK<TPR>, BWD_BLOCKS<TPR>) residual_norm_bwd
   Ring<T, TPR> ring;
   ring.src[0] = a.x;
   ring.src[1] = a.y;
-  ring.src[2] = a.dh ? a.dh : a.dn;
+  // the gradients that there are, then the gate
+  const int at_dn = a.dh ? 3 : 2, at_gate = at_dn + (a.dn ? 1 : 0);
+  ring.src[2] = a.dh ? a.dh : a.dn ? a.dn : a.gate;
   ring.src[3] = a.dh && a.dn ? a.dn : a.gate;
   ring.src[4] = a.gate;
-  const int at_dn = a.dh ? 3 : 2, at_gate = at_dn + (a.dn ? 1 : 0);
   ring.start(smem, bars, group, a.stages, at_gate + (TOKEN_GATE ? 1 : 0), a.D);
   if (threadIdx.x == 0) {
     for (int i = 0; i < ROWS * MAX_STAGES; ++i) mbar_init(&bars[i], 1);
@@ -548,7 +549,7 @@ extern "C" int yf_residual_norm_parts(int T, int D, int gate_rows) {
   return n > 0x7fffffff ? -1 : (int)n;
 }
 
-// Gradients of yf_residual_norm_fwd.  dh, dn: either may be null (zeros).  parts: yf_residual_norm_parts rows of D floats, twice as many with
+// Gradients of yf_residual_norm_fwd.  dh, dn: one of them may be null (zeros).  parts: yf_residual_norm_parts rows of D floats, twice as many with
 // post or gate; parts_floats says how many there are.  dw, dpost: kind 0 the type of the activations, 1 fp32, 2 fp32 that is added to;
 // *_sumsq (optional): += the squares of what was written.
 extern "C" int yf_residual_norm_bwd(const void* x, const void* y, const void* weight, const void* post, const void* gate, int gate_rows,
@@ -557,7 +558,7 @@ extern "C" int yf_residual_norm_bwd(const void* x, const void* y, const void* we
                                     float scale, int dtype, void* stream) {
   const void* ptrs[] = {x, y, weight, post, gate, rstd, dh, dn, dx, dy, dgate, parts};
   if (bad_shape(T, D, gate_rows, gate, dtype) || !x || !y || !weight || !rstd || !dx || !dy || !dw || !parts || misaligned(ptrs, 12)) return -1;
-  if ((post != nullptr) != (dpost != nullptr) || (gate != nullptr) != (dgate != nullptr)) return -1;
+  if ((!dh && !dn) || (post != nullptr) != (dpost != nullptr) || (gate != nullptr) != (dgate != nullptr)) return -1;
   if (dw_kind < 0 || dw_kind > 2 || dpost_kind < 0 || dpost_kind > 2) return -1;
   const bool token_gate = gate != nullptr && gate_rows == T;
   const int groups = gate == nullptr || token_gate ? 1 : gate_rows;

@@ -707,3 +707,36 @@ def test_attention_of_scores_that_grow_along_the_row(turned):
     assert turned or (moved > 40).any()
     for name, got, w in zip(("out", "dq", "dk", "dv"), (out, *grads), want):
         oracle.close(got.detach(), w, name)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sample", "token"])
+@pytest.mark.parametrize("post", [False, True])
+def test_residual_norm_gradients_of_one_result_or_none(gate, post):
+    """One of the two gradients missing is a gradient of zeros, whatever the gate; both missing: no input gets one, and the C entry refuses."""
+    from yafsdp_b200.ops import functional as Fn
+    from yafsdp_b200.ops import kernels
+
+    x, y, w, p, g, dh, dn = _norm_case((3, 37, 512), gate, post, torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, y, w, p, g) if t is not None]
+    for which, given in ((0, dh), (1, dn)):
+        one = torch.autograd.grad(Fn.residual_norm(x, y, w, post_weight=p, gate=g)[which], leaves, given, allow_unused=True)
+        both = torch.autograd.grad(Fn.residual_norm(x, y, w, post_weight=p, gate=g), leaves, (dh, dn * 0) if which == 0 else (dh * 0, dn))
+        assert all(torch.equal(a, z) for a, z in zip(one, both))
+
+    class NoGradient(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, h, n):
+            return h.sum() * 0
+
+        @staticmethod
+        def backward(ctx, grad):
+            return None, None
+
+    NoGradient.apply(*Fn.residual_norm(x, y, w, post_weight=p, gate=g)).backward()
+    assert all(t.grad is None for t in leaves)
+    rows = {"none": 0, "channel": 1, "sample": 3, "token": 111}[gate]
+    plain = [None if t is None else t.detach() for t in (x, y, w, p, g)]
+    rstd = kernels.residual_norm_fwd(*plain, rows, 1.0, 1e-5)[2]
+    with pytest.raises(RuntimeError):
+        kernels.residual_norm_bwd(*plain, rows, rstd, None, None, 1.0, torch.empty_like(w), torch.empty_like(w) if post else None)
+    _done()

@@ -179,3 +179,34 @@ def test_hand_made_masks():
 def test_refused_values(call):
     with pytest.raises(ValueError):
         call(torch.zeros(1, 2, 2, 16), torch.ones(16))
+
+
+class _NoGradient(torch.autograd.Function):
+    """Something behind an operator that has no gradient for what it was given."""
+
+    @staticmethod
+    def forward(ctx, *tensors):
+        return tensors[0].sum() * 0.0
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, None
+
+
+def test_residual_norm_without_any_gradient(monkeypatch):
+    """Neither result has a gradient: neither has any input, and no kernel is asked for one."""
+    from yafsdp_b200.ops import kernels
+
+    def forward(x, y, weight, post, gate, gate_rows, scale, eps):
+        return *Fn._residual_norm_ref(x, y, weight, post, gate, scale, eps), torch.ones(x.numel() // x.shape[-1], 2)
+
+    def backward(*args, **kwargs):
+        raise AssertionError("a kernel without a gradient to read")
+
+    monkeypatch.setattr(kernels, "residual_norm_fwd", forward)
+    monkeypatch.setattr(kernels, "residual_norm_bwd", backward)
+    x, y, gate = (torch.randn(3, 8, requires_grad=True) for _ in range(3))
+    w, post = (torch.ones(8, requires_grad=True) for _ in range(2))
+    results = Fn.ResidualNormFn.apply(x, y, w, post, gate, 3, 1.0, 1e-5)
+    _NoGradient.apply(*results).backward()
+    assert all(t.grad is None for t in (x, y, w, post, gate))

@@ -661,6 +661,8 @@ class ResidualNormFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx: Any, dh: torch.Tensor | None, dn: torch.Tensor | None) -> Any:  # type: ignore[override]
+        if dh is None and dn is None:  # nothing behind this step has a gradient: there is none for its inputs, and no sink is begun
+            return (None,) * 8
         x, y, w, p, g, rstd = ctx.saved_tensors
         gate_rows, scale = ctx.args
         if x.numel() == 0:

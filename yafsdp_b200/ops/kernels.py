@@ -629,7 +629,7 @@ def residual_norm_bwd(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, po
                       rstd: torch.Tensor, dh: torch.Tensor | None, dn: torch.Tensor | None, scale: float, dw: torch.Tensor, dpost: torch.Tensor | None,
                       *, add_dw: bool = False, add_dpost: bool = False, dw_sumsq: torch.Tensor | None = None,
                       dpost_sumsq: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    """``(dx, dy, dgate)`` for at least one token; ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the
+    """``(dx, dy, dgate)`` for at least one token; one of ``dh`` and ``dn`` may be ``None`` (zeros); ``dw`` and ``dpost`` (the activations' type or fp32; ``add_*``: fp32, added to) receive the
     weights' gradients and ``*_sumsq`` the squares of them."""
     d, dtype = x.shape[-1], x.dtype
     t = x.numel() // d
