@@ -106,12 +106,12 @@ YF_DEVINL const float4* rope_at(const float* rope, int pos, int dim) {
   return rope == nullptr ? nullptr : reinterpret_cast<const float4*>(rope + ((long long)pos * 64 + dim) * 2);
 }
 
-// Whether token t, the i-th of its sequence, sees one key only; spans null: causal.  Its probability is 1 whatever q and k are, so they get no
+// Whether token t, the i-th of its sequence of S, sees one key only; spans null: causal.  Its probability is 1 whatever q and k are, so they get no
 // gradient from it: zeros, not what is left of the difference of two equal sums.
-YF_DEVINL bool sees_one_key(const int2* spans, long long t, int i) {
+YF_DEVINL bool sees_one_key(const int2* spans, long long t, int i, int S) {
   if (spans == nullptr) return i == 0;
   const int2 s = __ldg(spans + t);
-  return s.y - s.x == 1;
+  return min(s.y, S) - max(s.x, 0) == 1;
 }
 
 // dq (bf16, strided rows) = scale * dq_accum (fp32, dense rows of 128 Hq); with dkv_parts also dk = scale * the sum of the parts' dK and
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256) attn_convert_kernel(const float* __restri
         a[4 * j] = x.x; a[4 * j + 1] = x.y; a[4 * j + 2] = x.z; a[4 * j + 3] = x.w;
         z[4 * j] = y.x; z[4 * j + 1] = y.y; z[4 * j + 2] = y.z; z[4 * j + 3] = y.w;
       }
-      if (RANGES && sees_one_key(spans, t, (int)(t % S))) {
+      if (RANGES && sees_one_key(spans, t, (int)(t % S), S)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) a[j] = z[j] = 0.f;
       }

@@ -9,7 +9,7 @@ constexpr int MOD_CAP = 1;
 constexpr int MOD_BIAS = 2;
 
 struct AttnMods {
-  const int2* spans;    // [B, S] by query (forward) or by key (backward); null: causal
+  const int2* spans;    // [B, S] by query (forward) or by key (backward), cut to the row; null: causal
   const int* padding;   // [B, ceil(S / 128)] padded tokens of every 128; null with spans
   const float* slopes;  // [Hq]
   __nv_bfloat16* out_lo;  // forward: what rounding the output to bf16 left over, laid out like it; null: not kept.  D = rowsum(dO * O) wants

@@ -132,7 +132,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     const int2 a = __ldg(spans + kv0), z = __ldg(spans + kv0 + keys - 1);
     dead_keys = __ldg(padding + jt);
     i_start = max(a.x, 0) / BQ;
-    per_head = min((z.y + BQ - 1) / BQ, n_qt) - i_start;
+    per_head = (min(z.y, args.S) + BQ - 1) / BQ - i_start;
     if (dead_keys >= keys || per_head < 0) per_head = 0;  // nothing but padding
   }
   const int n_it = per_head * heads;
@@ -280,7 +280,10 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
     const float sl2 = args.scale_log2;
     uint8_t* ds_row = sdS + p * DS_BYTES + row * 128;
     int2 span = make_int2(key, args.S);       // queries [x, y) that see this key
-    if (spans != nullptr || key >= args.S) span = key < args.S ? __ldg(spans + key) : make_int2(0, 0);
+    if (spans != nullptr || key >= args.S) {
+      span = key < args.S ? __ldg(spans + key) : make_int2(0, 0);
+      span = make_int2(max(span.x, 0), min(span.y, args.S));  // ranges put together by hand may reach beyond the row
+    }
     const float cap_sq = (MODS & MOD_CAP) ? -1.f / (args.mods.cap_log2 * args.mods.cap_log2) : 0.f;
     int h = h0 + (n_it == 0 ? 0 : p / per_head);
     bool alive = true;
@@ -368,7 +371,7 @@ attn_mods_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       const float f = p == 0 ? 1.f : args.scale;
       // a key that only one query sees, which sees nothing else
       bool alone = false;
-      if (p == 1 && span.y - span.x == 1) alone = sees_one_key(args.query_spans, (long long)b * args.S + span.x, span.x);
+      if (p == 1 && span.y - span.x == 1) alone = sees_one_key(args.query_spans, (long long)b * args.S + span.x, span.x, args.S);
       uint8_t* stage = sRing + p * 2 * QTILE + half * ATOM + (warp & 3) * 32 * 128;
 #pragma unroll 1
       for (int c = 0; c < 2; ++c) {

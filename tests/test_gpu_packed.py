@@ -740,3 +740,31 @@ def test_residual_norm_gradients_of_one_result_or_none(gate, post):
     with pytest.raises(RuntimeError):
         kernels.residual_norm_bwd(*plain, rows, rstd, None, None, 1.0, torch.empty_like(w), torch.empty_like(w) if post else None)
     _done()
+
+
+@pytest.mark.parametrize("beyond", [1, 100, 2**31 - 1])
+@pytest.mark.parametrize("window", [0, 40])
+def test_attention_under_ranges_beyond_the_row(beyond, window):
+    """A mask put together by hand whose ranges start before their row or end behind it: the same as cut to the row, to the bit (but dQ)."""
+    from yafsdp_b200.ops import functional as Fn
+
+    b, s, hq, hkv = 2, 300, 4, 2
+    ids = _ids(b, s, 60, True).to(DEV)
+    ids[0, -1] = 77  # a document of the row's last token: it sees itself alone
+    flags = torch.zeros(b, s, device=DEV, dtype=torch.bool)
+    flags[1, -30:] = True
+    ids[1, -30:] = 99  # a prefix up to the row's end
+    mask = Fn.document_mask(ids, flags, window)
+    far = min(s + beyond, 2**31 - 1)
+    wide = Fn.DocumentMask(*(torch.where(t == s, far, torch.where(t == 0, -beyond, t)) for t in (mask.spans, mask.key_spans)), mask.positions, mask.padding)
+    assert (wide.spans != mask.spans).any() and (wide.key_spans != mask.key_spans).any()
+    results = []
+    for m in (mask, wide):
+        q, k, v = _qkv(b, s, hq, hkv)
+        out = Fn.attention(q, k, v, m)
+        dout = torch.randn(out.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).bfloat16()
+        results.append((out.detach(), *torch.autograd.grad(out, (q, k, v), dout)))
+    _done()
+    for i, (a, z) in enumerate(zip(*results)):
+        assert torch.allclose(a.float(), z.float(), rtol=2.0**-7, atol=1e-4) if i == 1 else torch.equal(a, z), i
+    assert (results[1][1][0, -1] == 0).all() and (results[1][2][0, -1] == 0).all()

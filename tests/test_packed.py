@@ -210,3 +210,12 @@ def test_residual_norm_without_any_gradient(monkeypatch):
     results = Fn.ResidualNormFn.apply(x, y, w, post, gate, 3, 1.0, 1e-5)
     _NoGradient.apply(*results).backward()
     assert all(t.grad is None for t in (x, y, w, post, gate))
+
+
+def test_attention_under_ranges_beyond_the_row():
+    torch.manual_seed(0)
+    ids = torch.tensor([[3, 3, 3, 4, 5, 5, 5], [-1, 4, 4, 6, 6, 6, 6]])
+    m = Fn.document_mask(ids, ids == 6)
+    wide = Fn.DocumentMask(*(torch.where(t == 7, 2**31 - 1, torch.where(t == 0, -9, t)) for t in (m.spans, m.key_spans)), m.positions, m.padding)
+    q, k, v = (torch.randn(2, 7, 2, 16) for _ in range(3))
+    assert torch.equal(Fn.attention(q, k, v, wide), Fn.attention(q, k, v, m))

@@ -417,7 +417,7 @@ class DocumentMask:
     """Which tokens of a packed batch see each other (:func:`document_mask`): query ``i`` of a row sees the keys ``spans[i, 0] <= j <
     spans[i, 1]``, key ``j`` is seen by the queries ``key_spans[j, 0] <= i < key_spans[j, 1]``.  ``positions``: index of a token in its
     document.  ``padding``: padded tokens in every 128 of a row.  Neither end of
-    a span moves back along a row, and both views say the same: the kernels rely on it."""
+    a span moves back along a row, and both views say the same: the kernels rely on it.  What a span has beyond the row counts for nothing."""
 
     spans: torch.Tensor  # [B, S, 2] int32
     key_spans: torch.Tensor  # [B, S, 2] int32
