@@ -29,6 +29,8 @@ constexpr int FWD_BLOCKS = NV == 2 ? 3 : 2;  // per SM
 template <int TPR>
 constexpr int BWD_BLOCKS = TPR < 512 ? 2 : 1;
 constexpr int MAX_STAGES = 4;
+// Rows are counted in 32 bits; up to here a walker's next rows still are, which lie up to 4 x 2368 behind its own.
+constexpr int MAX_ROWS = 0x7fffffff - (1 << 20);
 // What the rings of an SM's blocks take together: 160 KB, which leaves room for the L1 that the weights come from, and more only for rows of which
 // not even one would fit.
 constexpr int RING_BYTES = 160 * 1024, RING_BYTES_MOST = 192 * 1024;
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(BLOCK<TPR>, FWD_BLOCKS<TPR, NV>) residual_norm
   const int group = threadIdx.x / TPR, tr = threadIdx.x % TPR;
   const int nvec = a.D / 8;
   const int walkers = gridDim.x * ROWS, each = (a.T + walkers - 1) / walkers;
-  const int first = min((long long)(blockIdx.x * ROWS + group) * each, (long long)a.T), end = min(first + each, a.T);
+  const int first = min((long long)(blockIdx.x * ROWS + group) * each, (long long)a.T), end = min((long long)first + each, (long long)a.T);
   Ring<T, TPR> ring;
   ring.start(smem, bars, group, a.stages, a.token_gate ? 3 : 2, a.D);
   ring.src[0] = a.x;
@@ -516,14 +518,14 @@ bool misaligned(const void* const* p, int n) {
   return (bits & 15) != 0;
 }
 bool bad_shape(int T, int D, int gate_rows, const void* gate, int dtype) {
-  if (T <= 0 || D <= 0 || D % 8 || D > 8192 || dtype < 0 || dtype > 2) return true;
+  if (T <= 0 || T > MAX_ROWS || D <= 0 || D % 8 || D > 8192 || dtype < 0 || dtype > 2) return true;
   return gate != nullptr ? gate_rows <= 0 || T % gate_rows != 0 : gate_rows != 0;
 }
 
 }  // namespace
 
 // x, y, h, n: [T, D] without gaps; weight, post: [D]; gate: [gate_rows, D], row t / (T / gate_rows) for token t (gate_rows 0 without one); all
-// of one type (dtype 0 bf16, 1 fp16, 2 fp32), 16-byte aligned, D a multiple of 8 up to 8192.  rstd: [T, 2] fp32 for the backward
+// of one type (dtype 0 bf16, 1 fp16, 2 fp32), 16-byte aligned, D a multiple of 8 up to 8192, T up to 2^31 - 2^20 - 1.  rstd: [T, 2] fp32 for the backward
 // pass, or null.
 extern "C" int yf_residual_norm_fwd(const void* x, const void* y, const void* weight, const void* post, const void* gate, int gate_rows, void* h,
                                     void* n, float* rstd, int T, int D, float scale, float eps, int dtype, void* stream) {
@@ -543,7 +545,7 @@ extern "C" int yf_residual_norm_fwd(const void* x, const void* y, const void* we
 
 // Rows of [rows, D] fp32 scratch that the backward pass wants (twice that with a post norm or a gate).
 extern "C" int yf_residual_norm_parts(int T, int D, int gate_rows) {
-  if (T <= 0 || D <= 0 || D % 8 || D > 8192 || gate_rows < 0 || (gate_rows > 0 && T % gate_rows)) return -1;
+  if (T <= 0 || T > MAX_ROWS || D <= 0 || D % 8 || D > 8192 || gate_rows < 0 || (gate_rows > 0 && T % gate_rows)) return -1;
   const int groups = gate_rows == 0 || gate_rows == T ? 1 : gate_rows;
   const long long n = (long long)groups * ctas_per_group(T, D, groups);
   return n > 0x7fffffff ? -1 : (int)n;

@@ -768,3 +768,14 @@ def test_attention_under_ranges_beyond_the_row(beyond, window):
     for i, (a, z) in enumerate(zip(*results)):
         assert torch.allclose(a.float(), z.float(), rtol=2.0**-7, atol=1e-4) if i == 1 else torch.equal(a, z), i
     assert (results[1][1][0, -1] == 0).all() and (results[1][2][0, -1] == 0).all()
+
+
+def test_residual_norm_refuses_rows_beyond_32_bits():
+    from yafsdp_b200.ops import functional as Fn
+    from yafsdp_b200.ops import kernels
+
+    w = torch.ones(8, device=DEV, dtype=torch.bfloat16)
+    for rows in (kernels.MAX_NORM_ROWS + 1, 2**31 + 1, 2**32 + 1):  # one row, many times
+        x = w.expand(rows, 8)
+        with pytest.raises(ValueError):
+            Fn.residual_norm(x, x, w)

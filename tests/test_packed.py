@@ -219,3 +219,15 @@ def test_attention_under_ranges_beyond_the_row():
     wide = Fn.DocumentMask(*(torch.where(t == 7, 2**31 - 1, torch.where(t == 0, -9, t)) for t in (m.spans, m.key_spans)), m.positions, m.padding)
     q, k, v = (torch.randn(2, 7, 2, 16) for _ in range(3))
     assert torch.equal(Fn.attention(q, k, v, wide), Fn.attention(q, k, v, m))
+
+
+def test_residual_norm_rows_that_are_counted():
+    """The C entry refuses more rows than 32 bits can walk over (their number plus a step's would overflow)."""
+    from yafsdp_b200 import _native
+    from yafsdp_b200.ops import kernels
+
+    parts = _native.lib().yf_residual_norm_parts
+    for rows in (kernels.MAX_NORM_ROWS + 1, 2**31 - 1):
+        assert parts(rows, 8, 0) == -1
+    # rows that fill every block
+    assert parts(kernels.MAX_NORM_ROWS, 8, 0) == parts(1 << 24, 8, 0) > 1

@@ -717,7 +717,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     """The residual step between two blocks, in one kernel: ``h = x + scale * gate * u``, where ``u`` is the block's output ``y``, normalised
     with ``post_weight`` if that is given, and ``n = rmsnorm(h) * weight``, the input of the next block.  Returns ``(h, n)``.  ``x``, ``y``: ``[...,
     D]``; weights ``[D]``; ``gate``: ``[D]`` for every channel, ``[B, 1, D]`` for every sample of ``[B, S, D]``, or the shape of ``x``.  All of
-    one type (bf16, fp16 or fp32); sums are fp32 and each result is rounded once.  ``D``: a multiple of 8 up to 8192 on CUDA."""
+    one type (bf16, fp16 or fp32); sums are fp32 and each result is rounded once.  ``D``: a multiple of 8 up to 8192, and
+    at most 2^31 - 2^20 - 1 rows, on CUDA."""
     if x.dim() < 1 or x.shape != y.shape:
         raise ValueError(f"residual_norm: x and y must have one shape [..., D], got {list(x.shape)} and {list(y.shape)}")
     dtype, others = x.dtype, (y, weight) if post_weight is None else (y, weight, post_weight)
@@ -745,6 +746,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
         return _residual_norm_ref(x, y, weight, post_weight, gate, scale, eps)
     if x.shape[-1] % 8 or not 0 < x.shape[-1] <= 8192:
         raise ValueError(f"residual_norm: the CUDA kernels take widths that are multiples of 8 up to 8192, got {x.shape[-1]}")
+    if x.numel() // x.shape[-1] > kernels.MAX_NORM_ROWS:
+        raise ValueError(f"residual_norm: the CUDA kernels take at most {kernels.MAX_NORM_ROWS} rows, got {x.numel() // x.shape[-1]}")
     if not here:
         with torch.cuda.device(x.device):
             return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)

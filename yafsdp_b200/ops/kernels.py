@@ -591,6 +591,9 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
 
 
 # --------------------------------------------------------------------------------------- the residual step between two blocks
+MAX_NORM_ROWS = 2**31 - 2**20 - 1
+
+
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """``t`` without gaps from a 16-byte boundary on; a copy where it is laid out otherwise."""
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
