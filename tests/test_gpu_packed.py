@@ -779,3 +779,32 @@ def test_residual_norm_refuses_rows_beyond_32_bits():
         x = w.expand(rows, 8)
         with pytest.raises(ValueError):
             Fn.residual_norm(x, x, w)
+
+
+def _three_calls(dtype=torch.bfloat16):
+    """The operators with gradients, each as a function of all its inputs that may have one."""
+    from yafsdp_b200.ops import functional as Fn
+
+    mask = Fn.document_mask(_ids(2, 40, 9, True).to(DEV))
+    q, k, v = (t.detach() for t in _qkv(2, 40, 4, 2))
+    x, y, w, post, gate, _, _ = _norm_case((2, 40, 512), "sample", True, dtype)
+    axes = Fn.RotaryAxes(128, 1e4)
+    return {"rotary": (lambda *a: Fn.rotary(*a, mask.positions, axes), (q, k)), "attention": (lambda *a: Fn.attention(*a, mask, softcap=9.0), (q, k, v)),
+            "residual_norm": (lambda *a: Fn.residual_norm(a[0], a[1], a[2], post_weight=a[3], gate=a[4]), (x, y, w, post, gate))}
+
+
+@pytest.mark.parametrize("name", ["rotary", "attention", "residual_norm"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_tangents_are_refused(name, grad):
+    """The kernels have no forward-mode derivative: a tangent is refused, whichever input has it, and not dropped."""
+    from torch.autograd import forward_ad
+
+    call, tensors = _three_calls()[name]
+    first = lambda out: out if torch.is_tensor(out) else out[0]  # noqa: E731
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        for i, t in enumerate(tensors):
+            duals = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else z for j, z in enumerate(tensors)]
+            with pytest.raises(RuntimeError, match="jvp"):
+                call(*duals)
+        assert torch.equal(first(call(*tensors)), first(call(*tensors)))  # no tangent anywhere
+    _done()

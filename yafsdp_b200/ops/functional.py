@@ -19,6 +19,7 @@ from typing import Any
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import kernels
 
@@ -412,6 +413,11 @@ def _device_of(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> 
     return dev.type != "cuda" or dev.index == torch._C._cuda_getDevice()
 
 
+def _tangents() -> bool:
+    """Whether tensors may carry forward-mode tangents, which only an autograd function refuses: a kernel reads their values alone."""
+    return forward_ad._current_level >= 0
+
+
 @dataclass(frozen=True)
 class DocumentMask:
     """Which tokens of a packed batch see each other (:func:`document_mask`): query ``i`` of a row sees the keys ``spans[i, 0] <= j <
@@ -555,7 +561,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: Rota
         with torch.cuda.device(q.device):
             return rotary(q, k, positions, axes)
     positions, table = positions.contiguous(), axes.table(q.device)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad)) or _tangents():
         return RotaryFn.apply(q, k, positions, table)  # type: ignore[no-any-return]
     return kernels.rotary(q, k, positions, table)  # type: ignore[return-value]
 
@@ -621,7 +627,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
             return attention(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes)
     if slopes is not None:
         slopes = _c(slopes.float())
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _tangents():
         return AttentionFn.apply(q, k, v, mask, scale, softcap, slopes)  # type: ignore[no-any-return]
     spans, padding = (None, None) if mask is None else (mask.spans, mask.padding)
     return kernels.attn_fwd_mods(q, k, v, scale, softcap, slopes, spans, padding, keep=False)[0]
@@ -751,7 +757,7 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, *, pos
     if not here:
         with torch.cuda.device(x.device):
             return residual_norm(x, y, weight, post_weight=post_weight, gate=gate, scale=scale, eps=eps)
-    if wanted:
+    if wanted or _tangents():
         return ResidualNormFn.apply(x, y, weight, post_weight, gate, rows, scale, eps)  # type: ignore[no-any-return]
     return kernels.residual_norm_fwd(x, y, weight, post_weight, gate, rows, scale, eps, keep=False)[:2]
 
