@@ -808,3 +808,25 @@ def test_forward_mode_tangents_are_refused(name, grad):
                 call(*duals)
         assert torch.equal(first(call(*tensors)), first(call(*tensors)))  # no tangent anywhere
     _done()
+
+
+@pytest.mark.parametrize("name,power", [("rotary", 2), ("attention", 1), ("attention", 2), ("residual_norm", 1), ("residual_norm", 2)])
+def test_second_derivatives_are_refused(name, power):
+    """A gradient taken with ``create_graph`` is right, and a derivative of it is refused, not zero, also where the loss reaches the inputs on another
+    way.  (The derivative of the gradient of a sum of what ``rotary`` gives is zero.)"""
+    call, tensors = _three_calls()[name]
+    leaves = [t.clone().requires_grad_() for t in tensors]
+
+    def total():
+        out = call(*leaves)
+        return sum(t.float().pow(power).sum() for t in (out if isinstance(out, tuple) else (out,)))
+
+    once = torch.autograd.grad(total(), leaves)
+    loss = total()
+    grads = torch.autograd.grad(loss, leaves, create_graph=True)
+    for i, (a, z) in enumerate(zip(grads, once)):
+        assert torch.allclose(a.float(), z.float(), rtol=2.0**-7, atol=1e-4) if name == "attention" and i == 0 else torch.equal(a, z)
+    for take in (lambda t: torch.autograd.grad(t, leaves, retain_graph=True), lambda t: torch.autograd.grad(t, leaves[:1], retain_graph=True), lambda t: t.backward(retain_graph=True)):
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            take(loss + sum(g.float().pow(2).sum() for g in grads))
+    _done()

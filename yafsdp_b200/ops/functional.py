@@ -13,6 +13,7 @@ device the native path is the only one: there is no fallback to library kernels.
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Any
@@ -418,6 +419,35 @@ def _tangents() -> bool:
     return forward_ad._current_level >= 0
 
 
+class _RefuseDerivative(torch.autograd.Function):
+    """Passes on ``n`` tensors; a derivative of them with respect to the others is refused."""
+
+    @staticmethod
+    def forward(ctx: Any, n: int, *tensors: torch.Tensor | None) -> Any:  # type: ignore[override]
+        return tuple(None if t is None else t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx: Any, *grads: torch.Tensor | None) -> Any:  # type: ignore[override]
+        raise RuntimeError("the gradients of these kernels have no derivative: they can be differentiated once only")
+
+
+def _once(backward: Any) -> Any:
+    """A ``backward(ctx, saved, *grads)`` whose results cannot be differentiated, neither through the incoming gradients nor through what was
+    saved.  (``once_differentiable`` sees incoming gradients with a history only, and its error is left out where ``torch.autograd.grad``
+    is asked for tensors that the loss reaches on another way too: the derivative would be lost.)"""
+
+    @functools.wraps(backward)
+    def once(ctx: Any, *grads: torch.Tensor | None) -> Any:
+        saved = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return backward(ctx, saved, *grads)
+        with torch.no_grad():
+            out = backward(ctx, saved, *grads)
+        return _RefuseDerivative.apply(len(out), *out, *saved, *grads)
+
+    return once
+
+
 @dataclass(frozen=True)
 class DocumentMask:
     """Which tokens of a packed batch see each other (:func:`document_mask`): query ``i`` of a row sees the keys ``spans[i, 0] <= j <
@@ -538,10 +568,11 @@ class RotaryFn(torch.autograd.Function):
         return kernels.rotary(q, k, positions, table)
 
     @staticmethod
-    def backward(ctx: Any, dq: torch.Tensor | None, dk: torch.Tensor | None) -> Any:  # type: ignore[override]
+    @_once
+    def backward(ctx: Any, saved: Any, dq: torch.Tensor | None, dk: torch.Tensor | None) -> Any:  # type: ignore[override]
         if dq is None and dk is None:
             return None, None, None, None
-        return *kernels.rotary(dq, dk, *ctx.saved_tensors, backward=True), None, None
+        return *kernels.rotary(dq, dk, *saved, backward=True), None, None
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> tuple[torch.Tensor, torch.Tensor]:
@@ -586,8 +617,9 @@ class AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    def backward(ctx: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
-        q, k, v, out, out_lo, lse, slopes, spans, key_spans, padding = ctx.saved_tensors
+    @_once
+    def backward(ctx: Any, saved: Any, dout: torch.Tensor) -> Any:  # type: ignore[override]
+        q, k, v, out, out_lo, lse, slopes, spans, key_spans, padding = saved
         return *kernels.attn_bwd_mods(q, k, v, out, out_lo, dout, lse, *ctx.args, slopes, spans, key_spans, padding), None, None, None, None
 
 
@@ -666,10 +698,11 @@ class ResidualNormFn(torch.autograd.Function):
         return h, n
 
     @staticmethod
-    def backward(ctx: Any, dh: torch.Tensor | None, dn: torch.Tensor | None) -> Any:  # type: ignore[override]
+    @_once
+    def backward(ctx: Any, saved: Any, dh: torch.Tensor | None, dn: torch.Tensor | None) -> Any:  # type: ignore[override]
         if dh is None and dn is None:  # nothing behind this step has a gradient: there is none for its inputs, and no sink is begun
             return (None,) * 8
-        x, y, w, p, g, rstd = ctx.saved_tensors
+        x, y, w, p, g, rstd = saved
         gate_rows, scale = ctx.args
         if x.numel() == 0:
             return *(None if t is None else torch.zeros_like(t) for t in (x, y, w, p, g)), None, None, None
