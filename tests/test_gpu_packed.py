@@ -830,3 +830,18 @@ def test_second_derivatives_are_refused(name, power):
         with pytest.raises(RuntimeError, match="differentiated once"):
             take(loss + sum(g.float().pow(2).sum() for g in grads))
     _done()
+
+
+def test_rotary_trains_after_inference_mode():
+    """The table of frequencies that an evaluation under ``inference_mode`` made serves the training behind it."""
+    from yafsdp_b200.ops import functional as Fn
+
+    axes = Fn.RotaryAxes(64, 1e4)
+    q, k = torch.randn(2, 33, 4, 64, device=DEV).bfloat16(), torch.randn(2, 33, 2, 64, device=DEV).bfloat16()
+    positions = torch.randint(0, 1000, (2, 33), device=DEV)
+    with torch.inference_mode():
+        want = [t.clone() for t in Fn.rotary(q, k, positions, axes)]
+    q.requires_grad_()
+    out = Fn.rotary(q, k, positions, axes)
+    assert all(torch.equal(a, z) for a, z in zip(out, want))
+    assert torch.autograd.grad(out[0].sum(), q)[0].shape == q.shape

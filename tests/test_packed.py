@@ -231,3 +231,10 @@ def test_residual_norm_rows_that_are_counted():
         assert parts(rows, 8, 0) == -1
     # rows that fill every block
     assert parts(kernels.MAX_NORM_ROWS, 8, 0) == parts(1 << 24, 8, 0) > 1
+
+
+def test_rotary_table_outlives_inference_mode():
+    axes = Fn.RotaryAxes(32, 1e4)
+    with torch.inference_mode():
+        first = axes.table(torch.device("cpu"))
+    assert axes.table(torch.device("cpu")) is first and not first.is_inference()

@@ -555,7 +555,8 @@ class RotaryAxes:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("RotaryAxes: call rotary() or table() on this device once before capturing a graph")
             turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequency]
-            t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64).to(device)
+            with torch.inference_mode(False):  # a later call may save it for its backward pass
+                t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64).to(device)
             self._tables[device] = t
         return t
 
