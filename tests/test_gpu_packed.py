@@ -845,3 +845,11 @@ def test_rotary_trains_after_inference_mode():
     out = Fn.rotary(q, k, positions, axes)
     assert all(torch.equal(a, z) for a, z in zip(out, want))
     assert torch.autograd.grad(out[0].sum(), q)[0].shape == q.shape
+
+
+def test_rotary_table_of_the_current_device():
+    from yafsdp_b200.ops import functional as Fn
+
+    axes = Fn.RotaryAxes(64, 1e4)
+    table = axes.table(torch.device("cuda"))
+    assert axes.table(torch.device("cuda", torch.cuda.current_device())) is table and axes.table("cuda") is table

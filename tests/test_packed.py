@@ -238,3 +238,8 @@ def test_rotary_table_outlives_inference_mode():
     with torch.inference_mode():
         first = axes.table(torch.device("cpu"))
     assert axes.table(torch.device("cpu")) is first and not first.is_inference()
+
+
+def test_rotary_table_by_name():
+    axes = Fn.RotaryAxes(32, 1e4)
+    assert axes.table("cpu") is axes.table(torch.device("cpu"))

@@ -547,9 +547,12 @@ class RotaryAxes:
         self.frequency = [theta ** (-2.0 * j / head_dim) for j in range(half)]
         self._tables: dict[torch.device, torch.Tensor] = {}
 
-    def table(self, device: torch.device) -> torch.Tensor:
+    def table(self, device: torch.device | str) -> torch.Tensor:
         """``[head_dim / 2, 2]`` int64: the fraction of a turn per position in 2^-64, and the axis.  Made once per device, outside of graph
         captures."""
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:  # what a tensor's device says
+            device = torch.device("cuda", torch.cuda.current_device())
         t = self._tables.get(device)
         if t is None:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
