@@ -243,3 +243,20 @@ def test_rotary_table_outlives_inference_mode():
 def test_rotary_table_by_name():
     axes = Fn.RotaryAxes(32, 1e4)
     assert axes.table("cpu") is axes.table(torch.device("cpu"))
+
+
+def test_cpu_tensors_under_another_default_device():
+    """What the forms for CPU tensors make on the way is on the CPU whatever the default device is."""
+    torch.manual_seed(0)
+    ids, q, k = torch.tensor([[4, 4, 4, -1], [0, 1, 1, 1]]), torch.randn(2, 4, 2, 16), torch.randn(2, 4, 1, 16)
+
+    def call():
+        m, axes = Fn.document_mask(ids, ids == 1, 2), Fn.RotaryAxes(16, 1e4)
+        empty = Fn.document_mask(ids[:, :0])
+        out = [Fn.attention(q, k, k, mask, softcap=3.0) for mask in (m, None)]
+        return [m.spans, m.key_spans, m.positions, m.padding, empty.spans, empty.positions, *Fn.rotary(q, k, m.positions, axes), *out, axes.table("cpu")]
+
+    want = call()
+    with torch.device("meta"):
+        got = call()
+    assert all(torch.equal(a, z) for a, z in zip(got, want))

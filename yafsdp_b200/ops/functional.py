@@ -499,11 +499,11 @@ def document_mask(document_ids: torch.Tensor, prefix: torch.Tensor | None = None
 
 def _document_mask_ref(ids: torch.Tensor, prefix: torch.Tensor | None, window: int) -> DocumentMask:
     b, s = ids.shape
-    at = torch.arange(s).expand(b, s)
+    at = torch.arange(s, device=ids.device).expand(b, s)
     if b * s == 0:
-        empty = torch.zeros((b, s, 2), dtype=torch.int32)
-        return DocumentMask(empty, empty.clone(), torch.zeros((b, s), dtype=torch.int32), torch.zeros((b, (s + 127) // 128), dtype=torch.int32))
-    starts = torch.cat([torch.ones((b, 1), dtype=torch.bool), ids[:, 1:] != ids[:, :-1]], 1)
+        empty = ids.new_zeros((b, s, 2), dtype=torch.int32)
+        return DocumentMask(empty, empty.clone(), ids.new_zeros((b, s), dtype=torch.int32), ids.new_zeros((b, (s + 127) // 128), dtype=torch.int32))
+    starts = torch.cat([ids.new_ones((b, 1), dtype=torch.bool), ids[:, 1:] != ids[:, :-1]], 1)
     start = torch.where(starts, at, 0).cummax(1).values
     end = torch.where(starts.roll(-1, 1), at + 1, s).flip(1).cummin(1).values.flip(1)
     lead, run_end = torch.zeros_like(starts), end
@@ -559,7 +559,7 @@ class RotaryAxes:
                 raise RuntimeError("RotaryAxes: call rotary() or table() on this device once before capturing a graph")
             turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequency]
             with torch.inference_mode(False):  # a later call may save it for its backward pass
-                t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64).to(device)
+                t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64, device="cpu").to(device)
             self._tables[device] = t
         return t
 
@@ -603,7 +603,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: Rota
 
 def _rotary_ref(t: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
     pos = positions.reshape(-1, *t.shape[:2])[axes.axis].permute(1, 2, 0).double()
-    ang = pos * torch.tensor(axes.frequency, dtype=torch.float64)
+    ang = pos * torch.tensor(axes.frequency, dtype=torch.float64, device=t.device)
     cos, sin = ang.cos().float().unsqueeze(2), ang.sin().float().unsqueeze(2)
     a, b = t.float().chunk(2, dim=-1)
     return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(t.dtype)
@@ -672,7 +672,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentM
 def _attention_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: DocumentMask | None, scale: float, softcap: float,
                    slopes: torch.Tensor | None) -> torch.Tensor:
     s, group = q.shape[1], q.shape[2] // k.shape[2]
-    at = torch.arange(s)
+    at = torch.arange(s, device=q.device)
     if mask is None:
         seen = (at[None, :] <= at[:, None])[None]
     else:
