@@ -1,5 +1,6 @@
 """The operators around packed documents in 64 bits, with bounds on what roundings may move (shared by the CPU and GPU tests)."""
 
+import decimal
 import math
 
 import torch
@@ -34,6 +35,19 @@ def spans_of(ids, prefix, window):
                 positions[r, t] = t - i
             i = end
     return spans, key_spans, positions
+
+
+def turned(positions, theta, head_dim):
+    """(cosines, sines), float64 lists of rows of head_dim / 2, of positions (whole numbers) times theta^(-2 j / head_dim), the angles in 80 digits."""
+    with decimal.localcontext() as c:
+        c.prec = 80
+        # pi by Machin's formula: 16 atan(1/5) - 4 atan(1/239)
+        unit = 10**90
+        atan = lambda n: sum((-1) ** i * (unit // n ** (2 * i + 1)) // (2 * i + 1) for i in range(70))  # noqa: E731
+        two_pi = decimal.Decimal(2 * (16 * atan(5) - 4 * atan(239))) / unit
+        step = [(decimal.Decimal(theta).ln() * -2 * j / head_dim).exp() / two_pi for j in range(head_dim // 2)]
+        angles = [[float((f * p) % 1 * two_pi) for f in step] for p in positions]
+    return [[math.cos(a) for a in row] for row in angles], [[math.sin(a) for a in row] for row in angles]
 
 
 def attention(q, k, v, seen, scale, softcap, slopes, dout=None):

@@ -853,3 +853,16 @@ def test_rotary_table_of_the_current_device():
     axes = Fn.RotaryAxes(64, 1e4)
     table = axes.table(torch.device("cuda"))
     assert axes.table(torch.device("cuda", torch.cuda.current_device())) is table and axes.table("cuda") is table
+
+
+@pytest.mark.parametrize("theta", [1e4, 5e5])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_rotary_at_far_positions(theta, dtype):
+    """Angles to 2^-32 of a turn up to positions of 2^32, in all quarters of a turn, and to what the frequency's last bit leaves over beyond."""
+    from test_packed import FAR, far_positions
+
+    near = list(range(0, 4000, 7)) + [p for p in FAR if dtype == torch.int64 or abs(p) < 2**31]
+    got, want, off = far_positions(theta, DEV, torch.tensor(near, dtype=dtype))
+    _done()
+    # cosines and sines of at most an eighth of a turn to two units (2^-23 each), the turn by what the float leaves over to half of one
+    assert ((got - want).abs() <= 5 * 2.0**-24 * want.abs() + off).all()

@@ -260,3 +260,25 @@ def test_cpu_tensors_under_another_default_device():
     with torch.device("meta"):
         got = call()
     assert all(torch.equal(a, z) for a, z in zip(got, want))
+
+
+FAR = [0, 1, -1, 3999, 100000, 2**20 + 3, 2**30 + 1, 2**31 - 1, 5 - 2**31, 2**32, 2**33 + 7, 2**40 + 11, 3 - 2**45, 2**53 + 1, 2**62 + 9]
+
+
+def far_positions(theta, device, positions):
+    """(cosines and sines that ``rotary`` turns by, those of the definition, how far the angle may be off) at the positions."""
+    ones = torch.zeros(1, len(positions), 1, 64, device=device)
+    ones[..., :32] = 1.0
+    got = Fn.rotary(ones, ones, positions[None].to(device), Fn.RotaryAxes(64, theta))[0][0, :, 0].double().cpu()
+    want = torch.tensor(oracle.turned(positions.tolist(), theta, 64), dtype=torch.float64).transpose(0, 1).reshape(len(positions), 64)
+    # half a unit of a frequency of 2^-64 turns for each position, and of the fraction's 32 bits
+    return got, want, 2.0 * math.pi * (2.0**-33 + positions.double().abs() * 2.0**-65)[:, None]
+
+
+@pytest.mark.parametrize("theta", [1e4, 5e5])
+def test_rotary_at_far_positions(theta):
+    got, want, off = far_positions(theta, "cpu", torch.tensor(FAR))
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + off).all()
+    near = torch.tensor([p for p in FAR if abs(p) < 2**31], dtype=torch.int32)
+    got, want, off = far_positions(theta, "cpu", near)
+    assert ((got - want).abs() <= 2.0**-24 * want.abs() + off).all()

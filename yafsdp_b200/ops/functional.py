@@ -13,6 +13,7 @@ device the native path is the only one: there is no fallback to library kernels.
 
 from __future__ import annotations
 
+import decimal
 import functools
 import math
 from dataclasses import dataclass
@@ -520,6 +521,9 @@ def _document_mask_ref(ids: torch.Tensor, prefix: torch.Tensor | None, window: i
     return DocumentMask(torch.stack([lo, hi], -1).int(), torch.stack([first, stop], -1).int(), torch.where(pad, 0, at - start).int(), padding.int())
 
 
+_PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803")
+
+
 class RotaryAxes:
     """Frequencies of rotary positions with one or several axes.  Pair ``j`` of a head (dims ``j`` and ``j + head_dim / 2``) turns by
     ``positions[axis of j] * theta ** (-2 j / head_dim)``.  ``sections``: how many pairs follow each axis (their sum is ``head_dim / 2``; one
@@ -545,6 +549,11 @@ class RotaryAxes:
                         left[a] -= 1
                         self.axis.append(a)
         self.frequency = [theta ** (-2.0 * j / head_dim) for j in range(half)]
+        with decimal.localcontext() as c:  # in turns of 2^-64, from more than the 53 bits of a float: far positions multiply what is missing
+            base = decimal.Decimal(float(theta))
+            c.prec = 60 + max(0, -base.adjusted())
+            whole = decimal.Decimal(2) ** 64 / (2 * _PI)
+            self._turns = [int((base ** (decimal.Decimal(-2 * j) / head_dim) * whole).to_integral_value()) % 2**64 for j in range(half)]
         self._tables: dict[torch.device, torch.Tensor] = {}
 
     def table(self, device: torch.device | str) -> torch.Tensor:
@@ -557,9 +566,8 @@ class RotaryAxes:
         if t is None:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("RotaryAxes: call rotary() or table() on this device once before capturing a graph")
-            turns = [round(f / (2.0 * math.pi) * 2.0**64) % 2**64 for f in self.frequency]
             with torch.inference_mode(False):  # a later call may save it for its backward pass
-                t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(turns, self.axis)], dtype=torch.int64, device="cpu").to(device)
+                t = torch.tensor([[f - 2**64 if f >= 2**63 else f, a] for f, a in zip(self._turns, self.axis)], dtype=torch.int64, device="cpu").to(device)
             self._tables[device] = t
         return t
 
@@ -581,7 +589,8 @@ class RotaryFn(torch.autograd.Function):
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> tuple[torch.Tensor, torch.Tensor]:
     """``q [B, S, Hq, D]`` and ``k [B, S, Hk, D]`` (bf16, fp16 or fp32) turned by ``positions`` (int32 or int64): ``[B, S]`` for one axis, else
-    ``[axes, B, S]``.  Angles are exact to 2^-31 of a turn at any position."""
+    ``[axes, B, S]``.  Angles are exact to 2^-32 of a turn at positions of up to 2^32 in size,
+    beyond that to 2^-65 of a turn for each position; cosines and sines are fp32."""
     if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != axes.head_dim or k.shape[3] != axes.head_dim:
         raise ValueError(f"rotary: q and k must be [B, S, heads, {axes.head_dim}] of the same batch, got {list(q.shape)} and {list(k.shape)}")
     if q.dtype != k.dtype or q.dtype not in kernels._DTYPES:
@@ -602,8 +611,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: Rota
 
 
 def _rotary_ref(t: torch.Tensor, positions: torch.Tensor, axes: RotaryAxes) -> torch.Tensor:
-    pos = positions.reshape(-1, *t.shape[:2])[axes.axis].permute(1, 2, 0).double()
-    ang = pos * torch.tensor(axes.frequency, dtype=torch.float64, device=t.device)
+    pos = positions.reshape(-1, *t.shape[:2])[axes.axis].permute(1, 2, 0).long()
+    ang = (pos * axes.table(t.device)[:, 0]).double() * (2.0 * math.pi / 2.0**64)  # modulo a whole turn
     cos, sin = ang.cos().float().unsqueeze(2), ang.sin().float().unsqueeze(2)
     a, b = t.float().chunk(2, dim=-1)
     return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(t.dtype)
