@@ -409,8 +409,10 @@ attn_mods_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_con
       float l_run = 0.f;                       // sum over this thread's keys
       float l_off = 0.f;                       // what rounding to bf16 adds to the largest of every 32 keys
       int2 span = make_int2(0, qrow + 1);      // keys [x, y) of this row
-      if (args.mods.spans != nullptr || qrow >= args.S) span = qrow < args.S ? __ldg(args.mods.spans + (long long)now[0].z * args.S + qrow) : make_int2(0, 0);
-      span = make_int2(max(span.x, 0), min(span.y, args.S));  // ranges put together by hand may reach beyond the row
+      if (args.mods.spans != nullptr || qrow >= args.S) {
+        span = qrow < args.S ? __ldg(args.mods.spans + (long long)now[0].z * args.S + qrow) : make_int2(0, 0);
+        span = make_int2(max(span.x, 0), min(span.y, args.S));  // ranges put together by hand may reach beyond the row
+      }
       const float slope = (MODS & MOD_BIAS) ? args.mods.slopes[now[0].y] * LOG2E : 0.f;
       float top = -INFINITY;                   // exponent of the largest P, of the half block before for a while
       auto add_off = [&]() {  // under the next half block's maximum (causal 520 us, 529 at once)
