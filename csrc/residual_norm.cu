@@ -46,12 +46,16 @@ YF_DEVINL bool group_bar_or(int tpr, int group, bool flag) {
   if (group == 2) return named_bar_or(3, tpr, flag);
   return named_bar_or(4, tpr, flag);
 }
-// sum over the TPR threads of a row; false when one of them says so.  `slots`: one float per warp of the block, not used again before the row's
+// sum over the TPR threads of a row; false when one of them says so.  What they have read before it is read behind it.  `slots`: one float per warp of the block, not used again before the row's
 // threads have met at another barrier.
 template <int TPR>
 YF_DEVINL bool row_sum(float& v, float* slots, int group, bool ok = true) {
   v = warp_sum(v);
-  if (TPR == 32) return __all_sync(0xffffffffu, ok);
+  if (TPR == 32) {
+    ok = __all_sync(0xffffffffu, ok);
+    __syncwarp();  // the vote does not order memory: what the lanes have read of a stage comes before the copy into it
+    return ok;
+  }
   if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
   if (group_bar_or(TPR, group, !ok)) return false;
   v = 0.f;
