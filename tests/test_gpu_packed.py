@@ -866,3 +866,34 @@ def test_rotary_at_far_positions(theta, dtype):
     _done()
     # cosines and sines of at most an eighth of a turn to two units (2^-23 each), the turn by what the float leaves over to half of one
     assert ((got - want).abs() <= 5 * 2.0**-24 * want.abs() + off).all()
+
+
+def _long_rows(s):
+    """Documents that start or end beside the places up to which a tile of 1024 tokens reads at once: its neighbours and then 4096 tokens at a time."""
+    ids = torch.zeros(8, s, dtype=torch.int64)  # 0: one document
+    for row, at in ((1, 1024), (2, 1023), (3, 4096 + 1024), (4, 4096 + 1025)):
+        ids[row, at:] = 5  # two
+    ids[5, s - 1 :] = 6  # the last token alone
+    ids[6, :1500] = ids[6, -2500:] = -1  # padding at either end
+    ids[7, 9000:9010] = -3  # and in the middle
+    return ids
+
+
+@pytest.mark.parametrize("s", [20000, 13312, 9217])
+@pytest.mark.parametrize("window", [0, 6000])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_document_mask_of_long_documents(s, window, dtype):
+    """Starts, ends and unflagged tokens many tiles away, with and without prefixes."""
+    from yafsdp_b200.ops import functional as Fn
+
+    ids = _long_rows(s).to(dtype)
+    at = torch.arange(s)
+    # nothing flagged; all; all but one token far from the row's ends; the first tokens of a document; the last ones
+    flags = [torch.zeros_like(ids, dtype=torch.bool), torch.ones_like(ids, dtype=torch.bool), *((at != p).expand_as(ids) for p in (0, 1030, 7000, s - 2)),
+             (at < 5500).expand_as(ids), (at > 3000).expand_as(ids)]
+    for prefix in (None, *flags):
+        want = Fn._document_mask_ref(ids, prefix, window)
+        got = Fn.document_mask(ids.to(DEV), None if prefix is None else prefix.contiguous().to(DEV), window)
+        for name in ("spans", "key_spans", "positions", "padding"):
+            assert torch.equal(getattr(got, name).cpu(), getattr(want, name)), name
+    _done()

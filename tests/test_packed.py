@@ -282,3 +282,15 @@ def test_rotary_at_far_positions(theta):
     near = torch.tensor([p for p in FAR if abs(p) < 2**31], dtype=torch.int32)
     got, want, off = far_positions(theta, "cpu", near)
     assert ((got - want).abs() <= 2.0**-24 * want.abs() + off).all()
+
+
+def test_document_mask_of_long_documents():
+    ids = torch.zeros(3, 9217, dtype=torch.int64)
+    ids[1, 5120:] = 5
+    ids[2, :1500] = ids[2, -2500:] = -1
+    at = torch.arange(9217)
+    for prefix in (None, (at != 7000).expand_as(ids), (at < 5500).expand_as(ids)):
+        for window in (0, 6000):
+            m = Fn.document_mask(ids, prefix, window)
+            for got, want in zip((m.spans, m.key_spans, m.positions), oracle.spans_of(ids, prefix, window)):
+                assert torch.equal(got, want)
