@@ -549,11 +549,14 @@ class RotaryAxes:
                         left[a] -= 1
                         self.axis.append(a)
         self.frequency = [theta ** (-2.0 * j / head_dim) for j in range(half)]
-        with decimal.localcontext() as c:  # in turns of 2^-64, from more than the 53 bits of a float: far positions multiply what is missing
-            base = decimal.Decimal(float(theta))
-            c.prec = 60 + max(0, -base.adjusted())
-            whole = decimal.Decimal(2) ** 64 / (2 * _PI)
-            self._turns = [int((base ** (decimal.Decimal(-2 * j) / head_dim) * whole).to_integral_value()) % 2**64 for j in range(half)]
+        base = decimal.Decimal(float(theta))
+        # in turns of 2^-64, from more than the 53 bits of a float: far positions multiply what is missing
+        with decimal.localcontext(decimal.Context(prec=60 + max(0, -base.adjusted()))):
+            turn, ratio = decimal.Decimal(2) ** 64 / (2 * _PI), base ** (decimal.Decimal(-2) / head_dim)
+            self._turns = []
+            for _ in range(half):
+                self._turns.append(int(turn.to_integral_value()) % 2**64)
+                turn *= ratio
         self._tables: dict[torch.device, torch.Tensor] = {}
 
     def table(self, device: torch.device | str) -> torch.Tensor:
