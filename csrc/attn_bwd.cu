@@ -396,6 +396,38 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant
   }
 }
 
+// CTAs per key tile of a KV head.  With grouped-query attention a KV head's key tiles are few and their walks long (every
+// query head of the group): the walk is cut by query heads where that is estimated to end sooner.  The main kernel takes its longest
+// walk or its share of all steps, 1.5 us a step and 8 us a CTA (start, end, first loads); the parts' sums (131 KB a CTA) are read at
+// 3.7 TB/s.  Measured, the whole backward pass, us, in 1 / 2 / 4 / 8 parts (* the choice):
+//   1 x 333 tokens, 64 / 8 heads 88 / 56 / 42 / 42*;  1 x 777, 64 / 8 166 / 103 / 72* / 92;  1 x 2048, 64 / 8 396 / 253* / 290 / 331;
+//   1 x 8192, 64 / 8 3422* / 3335 / 3455 / 3457;  8 x 300, 32 / 8 85* / 97 / 121;  4 x 1024, 32 / 8 162* / 204 / 255;
+//   1 x 4096, 32 / 8 455 / 479* / 542;  1 x 4096, 28 / 4 653 whole, 432* in seven.
+// (Cut until there were three CTAs per SM, 8 x 300 took 113, 4 x 1024 204 and 1 x 777 92 us.)
+// The backward pass under masks takes the same estimate, which knows of no ranges.  Packed rows, documents of 60 / 400 / 1200 tokens on average (replays of
+// a graph):  1 x 2048, 32 / 8 58 / 70* / 89, 112 / 85* / 103, 124 / 97* / 112;  1 x 4096, 32 / 8 119 / 139* / 173, 185 / 178* / 216, 209 / 215* / 256;
+//   1 x 8192, 32 / 8 206* / 258 / 338, 302* / 376 / 470, 426* / 462 / 589;  1 x 777, 64 / 8 64 / 50 / 56* / 71 (documents of 60);  1 x 8192, 64 / 8
+//   862* / 824 / 951 / 1073 (of 1200).  So it is the best or within 5 % of it, but for short documents, where it costs up to a fifth.
+int head_parts_for(int B, int S, int Hq, int Hkv) {
+  const int group = Hq / Hkv, n_kt = (S + BKV - 1) / BKV, n_qt = (S + BQ - 1) / BQ;
+  const float sms = (float)yf_num_sms(), walks = (float)n_kt * (float)Hkv * (float)B;
+  // steps of all walks, under the causal mask (key tile j starts at query tile 2 j)
+  const float longest = (float)n_qt * (float)group;
+  const float steps = (float)n_kt * (float)(n_qt - n_kt + 1) * (float)Hq * (float)B;
+  int best = 1;
+  float best_us = 0.f;
+  for (int parts = 1; parts <= group; ++parts) {
+    if (group % parts) continue;
+    const float walk = longest / (float)parts * 1.5f + 8.f, share = (steps * 1.5f + walks * (float)parts * 8.f) / sms;
+    const float us = (walk > share ? walk : share) + (parts > 1 ? walks * (float)parts * (131072.f / 3.7e6f) : 0.f);
+    if (parts == 1 || us < best_us) {
+      best = parts;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 // The three launches of one backward pass (delta pre-pass, main kernel, dQ conversion), shared by both entry points.

@@ -21,6 +21,7 @@
 // operands, 32 of loads, 16 of dS^T and 64 of dQ^T; 2750 pass.
 // bf16, 32 heads, causal, 1 x 8192: 1510 us with the passes before and after (82), 910 TFLOP/s; scores capped 1700; 32 / 8 heads in packed documents
 // of 5 to 8000 tokens 425.  Straight from registers (`red`) dQ took 1670 instead of 1520; with K and V loaded behind the ranges, 1520.
+// With a distance bias 8 to 16 bytes a thread spill.
 // D = rowsum(dO * O) comes from a small pre-pass; scale and bf16 of dQ are applied by a post-pass, of dK at the end.
 #include "attn_bwd_common.cuh"
 #include "attn_mods.cuh"

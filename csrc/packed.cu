@@ -16,7 +16,8 @@ namespace {
 // in shared memory, for the 1024 tokens before and after the tile as well; a token finds the start of its document as the last bit before it and
 // the end as the next one behind it.  Only documents longer than that make a CTA read on to the left or the right.  Every CTA works on its
 // own: 4 x 32768 tokens 8 us (with one CTA per row, and running maxima over the row, 90 us).  Bound by the latency of the loads and of
-// four passes through shared memory.
+// four passes through shared memory.  The CTAs of one long document all read it to its ends, so its time grows with the square of its length: 8192 tokens 5.5 us, 131072
+// 49, 2^20 1.7 ms.
 constexpr int DM_TILE = 1024, DM_WORDS = DM_TILE / 32;
 
 // Positions around i whose bits are set in 3 x DM_WORDS words that start at position `origin`: the last one <= i, and the first one > i;
@@ -144,7 +145,8 @@ __global__ void __launch_bounds__(DM_TILE) document_mask_kernel(const ID* __rest
 // of the float are turned by the rest.  (The whole fraction as a float would be off by up to 2^-26.)
 // A CTA takes up to RO_TOKENS tokens: every (token, pair) is turned into its cosine and sine once, for all heads of q and k.  A warp takes as many
 // heads side by side as its lanes hold vectors of, three times over before it stores anything, so that the memory has enough to do.
-// Bound by HBM: every element of q and k is read and written once.  2 x 4096 tokens, 64 / 8 heads of 128 in bf16: 53 us, 0.88 of the measured copy rate (67 us with a vector at a time).
+// Bound by HBM: every element of q and k is read and written once.  2 x 4096 tokens, 64 / 8 heads of 128 in bf16: 50 to 53 us, 0.88 of the measured copy rate or
+// more (67 us with a vector at a time).
 constexpr int RO_THREADS = 256, RO_TOKENS = 4, RO_MAX_HALF = 256, RO_BATCH = 3;
 struct RotaryArgs {
   const void* src[2];   // q, k

@@ -7,9 +7,14 @@
 //   e = scale gate g,  dy = r_y (e post - yhat mean(e post yhat)),
 //   dweight = sum dn hhat,  dpost = sum e yhat,  dgate = scale sum g u  over the tokens that share the row.
 // Bound by HBM: forward reads x, y and writes h, n once; backward reads x, y, dh, dn and writes dx, dy once.  h is formed anew in
-// the backward pass: the rounded h would take as many bytes and lose bits.  All sums are fp32, in a fixed order.
+// the backward pass: the rounded h would take as many bytes and lose bits.  All sums are fp32, and in a fixed order but for
+// the squares of the weights' gradients, which the parameter kernel's blocks add to their target by atomics.
 // 8192 x 8192 in bf16: 107 us forward, 159 backward, 5.0 TB/s of 6.5 for a copy (133 and 204 with plain loads): a row's two reductions stand behind each
 // other.  Blocks of 512 threads forward take as long, three blocks per SM spill (120), 320 threads for rows of 5120 gain nothing.
+// Further from a copy's rate: backward above width 4096 with fewer rows or a width between the classes (one block of 512 threads per SM waits at both
+// reductions; 4096 x 5120 53 to 75 us by gate and post norm, at most 4.8 TB/s, 2048 x 8192 39 to 54), width 512 (8192 rows 7 to 8 us forward and 16 to 26 backward, with everything in the L2:
+// a warp has 2 to 4 rows, so starts and ends count), and fp32, whose backward kernels spill 32 to 436 bytes a thread (4096 x 4096 80 us; bf16 and fp16 up
+// to 132 with a gate per token at widths to 2048).
 #include "common.cuh"
 #include "vec8.cuh"
 #include "yafsdp_b200.h"

@@ -897,3 +897,19 @@ def test_document_mask_of_long_documents(s, window, dtype):
         for name in ("spans", "key_spans", "positions", "padding"):
             assert torch.equal(getattr(got, name).cpu(), getattr(want, name)), name
     _done()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_attention_of_scores_up_to_a_billion(packed):
+    """Scores so large that fp32 has no fractions of them: the largest take all, shared evenly, and nothing overflows."""
+    from yafsdp_b200.ops import functional as Fn
+
+    b, s, hq, hkv = 2, 300, 4, 2
+    mask = Fn.document_mask(_ids(b, s, 70, True).to(DEV)) if packed else None
+    _, _, v = (t.detach() for t in _qkv(b, s, hq, hkv))
+    # powers of two, whose products and sums are exact: 128 * 2^10 * 2^0 to 2^15, by 0.2 up to 0.86e9
+    q = torch.full((b, s, hq, 128), 2.0**10, device=DEV, dtype=torch.bfloat16)
+    k = (2.0 ** (torch.arange(s, device=DEV) * 7 % 16)).bfloat16()[None, :, None, None].expand(b, s, hkv, 128)
+    out = Fn.attention(q, k, v, mask, scale=0.2)
+    _done()
+    oracle.close(out, oracle.attention(q, k, v, _seen(mask, b, s), 0.2, 0.0, None))
