@@ -16,8 +16,8 @@ namespace {
 // in shared memory, for the 1024 tokens before and after the tile as well; a token finds the start of its document as the last bit before it and
 // the end as the next one behind it.  Only documents longer than that make a CTA read on to the left or the right.  Every CTA works on its
 // own: 4 x 32768 tokens 8 us (with one CTA per row, and running maxima over the row, 90 us).  Bound by the latency of the loads and of
-// four passes through shared memory.  The CTAs of one long document all read it to its ends, so its time grows with the square of its length: 8192 tokens 5.5 us, 131072
-// 49, 2^20 1.7 ms.
+// four passes through shared memory.  The CTAs of one long document all read it to its ends, so its time
+// grows with the square of its length: 8192 tokens 5.5 us, 131072 49, 2^20 1.7 ms.
 constexpr int DM_TILE = 1024, DM_WORDS = DM_TILE / 32;
 
 // Positions around i whose bits are set in 3 x DM_WORDS words that start at position `origin`: the last one <= i, and the first one > i;

@@ -12,9 +12,9 @@
 // 8192 x 8192 in bf16: 107 us forward, 159 backward, 5.0 TB/s of 6.5 for a copy (133 and 204 with plain loads): a row's two reductions stand behind each
 // other.  Blocks of 512 threads forward take as long, three blocks per SM spill (120), 320 threads for rows of 5120 gain nothing.
 // Further from a copy's rate: backward above width 4096 with fewer rows or a width between the classes (one block of 512 threads per SM waits at both
-// reductions; 4096 x 5120 53 to 75 us by gate and post norm, at most 4.8 TB/s, 2048 x 8192 39 to 54), width 512 (8192 rows 7 to 8 us forward and 16 to 26 backward, with everything in the L2:
-// a warp has 2 to 4 rows, so starts and ends count), and fp32, whose backward kernels spill 32 to 436 bytes a thread (4096 x 4096 80 us; bf16 and fp16 up
-// to 132 with a gate per token at widths to 2048).
+// reductions; 4096 x 5120 53 to 75 us by gate and post norm, 2048 x 8192 39 to 54: at most 5.1 TB/s); width 512 (8192 rows 7 to 8 us forward and 16
+// to 26 backward, with everything in the L2: a warp has 2 to 4 rows, so starts and ends count); and fp32, whose backward kernels spill 32 to 436
+// bytes a thread (4096 x 4096 80 us; bf16 and fp16 up to 132 with a gate per token at widths to 2048).
 #include "common.cuh"
 #include "vec8.cuh"
 #include "yafsdp_b200.h"
@@ -51,8 +51,8 @@ YF_DEVINL bool group_bar_or(int tpr, int group, bool flag) {
   if (group == 2) return named_bar_or(3, tpr, flag);
   return named_bar_or(4, tpr, flag);
 }
-// sum over the TPR threads of a row; false when one of them says so.  What they have read before it is read behind it.  `slots`: one float per warp of the block, not used again before the row's
-// threads have met at another barrier.
+// sum over the TPR threads of a row; false when one of them says so.  What they read before it is read behind it.  `slots`: one float per warp of
+// the block, not used again before the row's threads have met at another barrier.
 template <int TPR>
 YF_DEVINL bool row_sum(float& v, float* slots, int group, bool ok = true) {
   v = warp_sum(v);

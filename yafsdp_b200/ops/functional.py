@@ -553,7 +553,7 @@ class RotaryAxes:
         # in turns of 2^-64, from more than the 53 bits of a float: far positions multiply what is missing
         with decimal.localcontext(decimal.Context(prec=60 + max(0, -base.adjusted()))):
             turn, ratio = decimal.Decimal(2) ** 64 / (2 * _PI), base ** (decimal.Decimal(-2) / head_dim)
-            self._turns = []
+            self._turns: list[int] = []
             for _ in range(half):
                 self._turns.append(int(turn.to_integral_value()) % 2**64)
                 turn *= ratio
